@@ -33,6 +33,7 @@ extern "C" {
 
 #define MOC_F32 0
 #define MOC_BF16 1
+#define MOC_F16 2          /* gradients of moc_grad_clip only */
 
 #define MOC_NORM_NONE 0
 #define MOC_NORM_RMS 1
@@ -177,6 +178,32 @@ int64_t moc_token_route_scratch_bytes(const moc_token_route_desc* s, int32_t bac
 int moc_token_route_fwd(const moc_token_route_desc* s, void* scratch);
 int moc_token_route_bwd(const moc_token_route_desc* s, const float* g_weights, const float* g_losses, void* d_h, float* d_w,
                         float* d_bias, void* scratch);
+
+/* Selection from router logits of one's own [rows, num_chapters] (row stride ld elements, fp32 or bf16), by the other rules a
+ * router may have (the reference has softmax and top-k alone, router.py:112-140): s = softmax or sigmoid over the chapters behind the
+ * num_shared first; sel = s + balance_bias[c] (NULL: the logits' own order); of num_groups runs of chapters the top_groups best stay
+ * (by their largest sel, or with group_top2 by the sum of their two largest); the top_k largest, sel descending, id ascending, in the
+ * order of exact arithmetic.  weights = s of the chosen, divided by max(their sum, 1e-12) with renormalize.  A logit at or below
+ * -3.3895e38 (the lowest finite bfloat16; -inf too) is masked: chosen after all others, lowest id first, with weight 0.
+ * idx [rows, top_k] int64, weights [rows, top_k]; joint list as in moc_router_fwd: comb_idx / comb_w [rows, num_shared + top_k];
+ * row_stats [rows, 4] (16-byte aligned) goes to the backward pass; load [num_chapters] int32 (NULL: not wanted) = rows that chose
+ * each chapter.  Limits: 16384 chapters to choose from, top_k 128, 64 groups of equal size, top_k <= chapters of top_groups groups. */
+#define MOC_SCORE_SOFTMAX 0
+#define MOC_SCORE_SIGMOID 1
+typedef struct {
+  int32_t rows, num_chapters, top_k, num_shared;
+  int32_t score, num_groups, top_groups, group_top2, renormalize;
+  int32_t dtype;              /* of the logits and their gradient */
+  int64_t ld;
+  float routed_scale;         /* rho of the joint list */
+} moc_select_shape;
+int moc_select_fwd(const moc_select_shape* s, const void* logits, const float* balance_bias, int64_t* idx, float* weights,
+                   int32_t* comb_idx, float* comb_w, float* row_stats, int32_t* load, void* stream);
+/* d_logits [rows, num_chapters] (dense, written whole) from the gradients of weights and comb_w (either may be NULL). */
+int moc_select_bwd(const moc_select_shape* s, const void* logits, const int64_t* idx, const float* weights, const float* comb_w,
+                   const float* row_stats, const float* g_weights, const float* g_comb, void* d_logits, void* stream);
+/* bias[c] += rate * sign(mean load - load[c]) over the chapters behind the shared ones: balance without a loss term. */
+int moc_balance_bias_step(float* bias, const int32_t* load, int32_t num_chapters, int32_t num_shared, float rate, void* stream);
 
 /* Position-weighted pooling: pooled[b, :] = sum_t pos_weight[t] * h[b, t, :] (fp32 accumulation), and its
  * backward d_h[b, t, :] (+)= pos_weight[t] * d_pooled[b, :].  With the coefficients of the rolling-window rule this
@@ -431,6 +458,18 @@ int moc_decode_attn(const moc_decode_shape* s, const void* q, const void* kv_ban
                     const int32_t* comb_idx, const float* comb_w, void* out, float* lse, int32_t* status,
                     void* stream);
 
+/* The 8-bit form of the cache: values [rows, heads * 64] e4m3 = round(x / scale) with scales [rows / scale_rows, heads] fp32 =
+ * (largest |x| of the block's scale_rows rows and head) / 448; `heads` counts K and V heads (2 * HK for a kv_bank).  A block of
+ * zeros has scale 0; one with a NaN or infinity stands for NaN. */
+int moc_quantize_rows(const void* rows_bf16, int64_t rows, int32_t heads, int32_t head_dim, int32_t scale_rows, void* values,
+                      float* scales, void* stream);
+/* moc_decode_attn over either form: kv_scale NULL = bf16, else e4m3 values with their scales (tokens_per_chapter must be whole
+ * blocks of scale_rows).  counts [batch] (NULL: all): how many of each sequence's listed chapters count; what lies behind them
+ * is not read.  A sequence without any gets zeros and lse -inf. */
+int moc_decode_attn_cache(const moc_decode_shape* s, const void* q, const void* kv_bank, const float* kv_scale, int32_t scale_rows,
+                          int64_t bank_rows, const int32_t* comb_idx, const float* comb_w, const int32_t* counts, void* out,
+                          float* lse, int32_t* status, void* stream);
+
 /* The routing window of a generated token: dst [batch, dst_rows] = the last dst_rows rows of cache [batch, cache_rows]
  * followed by h [batch, h_rows]; rows of row_bytes (a multiple of 16) lie behind each other, *_stride bytes lead from one
  * sequence to the next (dst is dense).  model.py:630-660 concatenates and slices. */
@@ -457,6 +496,8 @@ typedef struct {
   void *stream, *side_stream;
   int32_t hidden_dim;      /* width of hidden; 0: that of the routing states */
   int32_t launches;        /* written by the call: the kernels it launched */
+  const float* kv_scale;   /* kv_bank is held in 8 bits (moc_quantize_rows), in blocks of scale_rows; NULL: bf16 */
+  int32_t scale_rows;
 } moc_decode_step_desc;
 int64_t moc_decode_step_arena_bytes(const moc_decode_step_desc* s);
 int moc_decode_step(moc_decode_step_desc* s);
@@ -576,6 +617,30 @@ int moc_token_mix_bwd(const moc_sparse_attn_shape* s, int32_t index_heads, const
                       float* d_w_heads, int32_t* status, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * A block's output merged into the residual stream, with the norm behind the block, a gate, and the norm in front of the next
+ * block (memory_block.py:549-558 adds the plain output; post-norm, gate and residual scale are not in the reference):
+ *   y = residual_scale * x + gate * norm(f),   n = norm(y) with weights of its own, of y before it is rounded
+ * x, y [rows, dim] in x_dtype, f, n in f_dtype; weights, gate and their gradients fp32.  gate NULL, [dim] (gate_seq 0) or
+ * [rows / gate_seq, dim]: one row for every gate_seq rows.  next_weight NULL: no n.  stats [rows, 4] (16-byte aligned; NULL: not
+ * wanted) goes to the backward pass.  Backward: d_y / d_n NULL: no gradient came; d_x and the gradients of weights and gate
+ * NULL: not wanted.  scratch: moc_gated_residual_bwd_scratch_bytes, 16-byte aligned. */
+typedef struct {
+  int64_t rows;
+  int32_t dim, kind;          /* dim 1..8192; MOC_NORM_RMS (no biases are read) or MOC_NORM_LAYERNORM, both norms */
+  int32_t x_dtype, f_dtype;
+  int32_t gate_seq;
+  float residual_scale, eps, next_eps;
+} moc_residual_shape;
+int moc_gated_residual_fwd(const moc_residual_shape* s, const void* x, const void* f, const float* weight, const float* bias,
+                           const float* gate, const float* next_weight, const float* next_bias, void* y, void* n, float* stats,
+                           void* stream);
+int64_t moc_gated_residual_bwd_scratch_bytes(const moc_residual_shape* s, int32_t with_gate);
+int moc_gated_residual_bwd(const moc_residual_shape* s, const void* x, const void* f, const float* weight, const float* bias,
+                           const float* gate, const float* next_weight, const float* stats, const void* d_y, const void* d_n,
+                           void* d_x, void* d_f, float* d_weight, float* d_bias, float* d_gate, float* d_next_weight,
+                           float* d_next_bias, void* scratch, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Optimizer step of the bank from a compact gradient.  Replaces torch.optim.AdamW over the bank parameter
  * (training/trainer.py:372-378, param group "memory_bank" :338-347) fed by the dense gradient of torch.gather's
  * backward: same update for EVERY row (rows of untouched chapters see a zero gradient: moments decay, decoupled
@@ -591,6 +656,29 @@ int moc_bank_adamw_step(float* param, float* exp_avg, float* exp_avg_sq, int64_t
                         int32_t max_unique, const float* grad_rows, float grad_scale, float lr, float beta1,
                         float beta2, float eps, float weight_decay, int64_t step, void* shadow_bf16,
                         void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The same with a scale that stands on the device: grad_scale * d_grad_scale[0] multiplies the gradient (d_grad_scale may be NULL),
+ * e.g. the coefficient moc_grad_clip leaves, without a host round trip. */
+int moc_bank_adamw_step_scaled(float* param, float* exp_avg, float* exp_avg_sq, int64_t bank_rows, int32_t dim,
+                               int32_t tokens_per_chapter, const int32_t* uniq, const int32_t* num_unique,
+                               int32_t max_unique, const float* grad_rows, float grad_scale, const float* d_grad_scale, float lr,
+                               float beta1, float beta2, float eps, float weight_decay, int64_t step, void* shadow_bf16,
+                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* Global gradient norm over many tensors and the clipped tensors (the reference: torch.nn.utils.clip_grad_norm_ over every
+ * parameter, training/trainer.py:876-880):  norm = sqrt(sum_i weight_i^2 sum g_i^2),  coefficient = min(1, max_norm / (norm + eps)),
+ * out_i = coefficient g_i (NaN stays NaN).  result [2] fp32 (device) = {norm, coefficient}.  `grads` is a host array; a tensor
+ * without `out` counts in the norm alone, `out` equal to `grad` is clipped in place.  Tensors must not overlap.  The number of
+ * launches is two for up to 680 tensors.  workspace: moc_grad_clip_workspace_bytes(count), of this call alone. */
+typedef struct {
+  const void* grad;        /* elems elements of `dtype` (MOC_F32, MOC_BF16 or MOC_F16), aligned to their type */
+  void* out;               /* as many of out_dtype, or NULL */
+  int64_t elems;
+  const int32_t* count;    /* device: the first *count blocks of `unit` elements exist (a compact bank gradient); NULL: all */
+  int32_t unit, dtype, out_dtype;
+  float weight;            /* factor of the gradient in the norm (1 / world of a sum over ranks) */
+} moc_grad_desc;
+int64_t moc_grad_clip_workspace_bytes(int32_t count);
+int moc_grad_clip(const moc_grad_desc* grads, int32_t count, double max_norm, double eps, float* result, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 /* out[0] = sum of squares of the first num_unique*T rows of a compact gradient: the bank's share of the global
  * gradient norm that the reference clips by (training/trainer.py:876-880).  workspace: 592 floats. */
 int moc_rows_sqnorm(const float* rows, const int32_t* num_unique, int32_t tokens_per_chapter, int32_t dim,

@@ -13,7 +13,7 @@ import torch
 
 from .build import LIB_PATH
 
-MOC_F32, MOC_BF16 = 0, 1
+MOC_F32, MOC_BF16, MOC_F16 = 0, 1, 2        # (fp16: gradients of moc_grad_clip only)
 ATTN_BWD_STATIC_MAX_FLOATS = 1 << 20   # MOC_ATTN_BWD_STATIC_MAX_FLOATS in include/moc_b200.h
 NORM_NONE, NORM_RMS, NORM_LAYERNORM = 0, 1, 2
 NORM_CODES = {None: NORM_NONE, "none": NORM_NONE, "rms": NORM_RMS, "layernorm": NORM_LAYERNORM}
@@ -89,7 +89,20 @@ class DecodeStepDesc(C.Structure):
     _fields_ = [("router", RouterShape), ("attn", DecodeShape)] + _fields(
         "i: hidden_dtype out_dim; l: bank_rows;"
         "p: routing_states hidden router_w router_b wq wo kv_bank idx weights comb_idx comb_w out arena status stream"
-        " side_stream; i: hidden_dim launches")
+        " side_stream; i: hidden_dim launches; p: kv_scale; i: scale_rows")
+
+
+class SelectShape(C.Structure):
+    _fields_ = _fields("i: rows num_chapters top_k num_shared score num_groups top_groups group_top2 renormalize dtype; l: ld;"
+                       "f: routed_scale")
+
+
+class ResidualShape(C.Structure):
+    _fields_ = _fields("l: rows; i: dim kind x_dtype f_dtype gate_seq; f: residual_scale eps next_eps")
+
+
+class GradDesc(C.Structure):
+    _fields_ = _fields("p: grad out; l: elems; p: count; i: unit dtype out_dtype; f: weight")
 
 
 class LayerDesc(C.Structure):
@@ -204,6 +217,19 @@ _PROTOTYPES = {
     "moc_bank_adamw_step": (C.c_int, [P, P, P, C.c_int64, C.c_int32, C.c_int32, P, P, C.c_int32, P, C.c_float,
                                       C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int64, P, P,
                                       C.c_size_t, P, P]),
+    "moc_bank_adamw_step_scaled": (C.c_int, [P, P, P, C.c_int64, C.c_int32, C.c_int32, P, P, C.c_int32, P, C.c_float, P,
+                                             C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int64, P, P,
+                                             C.c_size_t, P, P]),
+    "moc_grad_clip_workspace_bytes": (C.c_int64, [C.c_int32]),
+    "moc_grad_clip": (C.c_int, [P, C.c_int32, C.c_double, C.c_double, P, P, C.c_int64, P]),
+    "moc_select_fwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
+    "moc_select_bwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
+    "moc_balance_bias_step": (C.c_int, [P, P, C.c_int32, C.c_int32, C.c_float, P]),
+    "moc_gated_residual_fwd": (C.c_int, [C.POINTER(ResidualShape)] + [P] * 11),
+    "moc_gated_residual_bwd_scratch_bytes": (C.c_int64, [C.POINTER(ResidualShape), C.c_int32]),
+    "moc_gated_residual_bwd": (C.c_int, [C.POINTER(ResidualShape)] + [P] * 18),
+    "moc_quantize_rows": (C.c_int, [P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, P, P, P]),
+    "moc_decode_attn_cache": (C.c_int, [C.POINTER(DecodeShape), P, P, P, C.c_int32, C.c_int64, P, P, P, P, P, P, P]),
     "moc_rows_sqnorm": (C.c_int, [P, P, C.c_int32, C.c_int32, P, P, C.c_size_t, P]),
     "moc_row_dot": (C.c_int, [P, P, C.c_int32, P, C.c_int64, C.c_int32, P]),
     "moc_col_sum": (C.c_int, [P, P, C.c_int64, C.c_int32, P]),

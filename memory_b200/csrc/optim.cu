@@ -39,8 +39,9 @@ template <typename I>
 __global__ void __launch_bounds__(256)
 bank_adamw_kernel(float4* __restrict__ param, float4* __restrict__ exp_avg, float4* __restrict__ exp_avg_sq,
                   const float4* __restrict__ grad_rows, const int* __restrict__ slot_of,
-                  uint2* __restrict__ shadow, I total4, I dim4, I T, AdamW h) {
+                  uint2* __restrict__ shadow, I total4, I dim4, I T, AdamW h, const float* __restrict__ device_scale) {
   const I stride = static_cast<I>(gridDim.x) * 256;
+  if (device_scale != nullptr) h.grad_scale *= *device_scale;
   const float decay = 1.f - h.lr * h.weight_decay, w1 = 1.f - h.beta1, w2 = 1.f - h.beta2;
   for (I first = static_cast<I>(blockIdx.x) * 256 + threadIdx.x; first < total4; first += kAdamAhead * stride) {
     float4 p[kAdamAhead], m[kAdamAhead], v[kAdamAhead], g[kAdamAhead];
@@ -119,7 +120,17 @@ extern "C" int moc_bank_adamw_step(float* param, float* exp_avg, float* exp_avg_
                                    int32_t T, const int32_t* uniq, const int32_t* num_unique, int32_t max_unique,
                                    const float* grad_rows, float grad_scale, float lr, float beta1, float beta2,
                                    float eps, float weight_decay, int64_t step, void* shadow_bf16, void* workspace,
-                                   size_t workspace_bytes, int32_t* status, void* stream_) {
+                                   size_t workspace_bytes, int32_t* status, void* stream) {
+  return moc_bank_adamw_step_scaled(param, exp_avg, exp_avg_sq, bank_rows, dim, T, uniq, num_unique, max_unique, grad_rows, grad_scale,
+                                    nullptr, lr, beta1, beta2, eps, weight_decay, step, shadow_bf16, workspace, workspace_bytes, status,
+                                    stream);
+}
+
+extern "C" int moc_bank_adamw_step_scaled(float* param, float* exp_avg, float* exp_avg_sq, int64_t bank_rows, int32_t dim,
+                                          int32_t T, const int32_t* uniq, const int32_t* num_unique, int32_t max_unique,
+                                          const float* grad_rows, float grad_scale, const float* d_grad_scale, float lr,
+                                          float beta1, float beta2, float eps, float weight_decay, int64_t step, void* shadow_bf16,
+                                          void* workspace, size_t workspace_bytes, int32_t* status, void* stream_) {
   MOC_REQUIRE(param && exp_avg && exp_avg_sq && uniq && num_unique && grad_rows && workspace && status, "NULL buffer");
   MOC_REQUIRE(bank_rows > 0 && dim > 0 && T > 0 && bank_rows % T == 0, "bank rows must be whole chapters");
   MOC_REQUIRE(dim % 4 == 0, "row width must be a multiple of 4");
@@ -149,7 +160,7 @@ extern "C" int moc_bank_adamw_step(float* param, float* exp_avg, float* exp_avg_
     bank_adamw_kernel<I><<<static_cast<int>(blocks), 256, 0, stream>>>(
         reinterpret_cast<float4*>(param), reinterpret_cast<float4*>(exp_avg), reinterpret_cast<float4*>(exp_avg_sq),
         reinterpret_cast<const float4*>(grad_rows), slot_of, static_cast<uint2*>(shadow_bf16), static_cast<I>(total4),
-        static_cast<I>(dim / 4), static_cast<I>(T), h);
+        static_cast<I>(dim / 4), static_cast<I>(T), h, d_grad_scale);
   };
   // (the last step of a thread may reach past the end by up to kAdamAhead strides)
   if (total4 + 2LL * kAdamAhead * blocks * 256 < (1LL << 31)) run(uint32_t{0}); else run(int64_t{0});

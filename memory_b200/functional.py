@@ -14,7 +14,7 @@ Three differentiable pieces mirror the reference's sequence-level memory layer
 from __future__ import annotations
 
 import os
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -927,3 +927,255 @@ def token_routed_attention_joint(h, shared_memory, routed_memory, token_chapter_
     if comb is None:
         comb = q.new_zeros(1, rows, d)
     return linear(comb, wo, cd).view(b, l, -1).to(h.dtype)
+
+
+# --------------------------------------------------------------------------------------------
+# selection from logits
+# --------------------------------------------------------------------------------------------
+class ChapterSelection(NamedTuple):
+    """What :func:`select_chapters` returns: for every row the chosen ids (int64) and weights, the joint list with the shared
+    chapters in front (int32 ids and weights, as ``memory_layer`` and the decoder take them), and how many rows chose each
+    chapter (int32 [C])."""
+    indices: torch.Tensor
+    weights: torch.Tensor
+    combined_indices: torch.Tensor
+    combined_weights: torch.Tensor
+    load: torch.Tensor
+
+
+class _Select(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, s):
+        ctx.set_materialize_grads(False)
+        idx, w, cidx, cw, stats, load = ops.select_fwd(logits, bias, s)
+        ctx.s = s
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, idx, w, cw, stats)
+        ctx.mark_non_differentiable(idx, cidx, load)
+        return idx, w, cidx, cw, load
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _idx, g_w, _cidx, g_cw, _load):
+        if g_w is None and g_cw is None:
+            return None, None, None
+        logits, idx, w, cw, stats = ctx.saved_tensors
+        g_w = None if g_w is None else ops._contig(g_w.float())
+        g_cw = None if g_cw is None else ops._contig(g_cw.float())
+        return ops.select_bwd(logits, ctx.s, idx, w, cw, stats, g_w, g_cw), None, None
+
+
+_MOST_SELECTED, _MOST_ROUTED, _MOST_GROUPS = 128, 16384, 64
+
+
+def _select_shape(rows: int, chapters: int, top_k: int, score: str, num_shared: int, routed_scale: float, num_groups: int,
+                  top_groups: Optional[int], group_score: str, renormalize: bool):
+    """The descriptor of a selection, its sizes and names checked (top_k as the router has it: at most what there is)."""
+    if score not in ops.SCORES:
+        raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
+    if num_shared < 0 or num_shared >= chapters:
+        raise ValueError(f"num_shared ({num_shared}) must leave a chapter of {chapters} to choose from")
+    n = chapters - num_shared
+    if n > _MOST_ROUTED:
+        raise ValueError(f"at most {_MOST_ROUTED} chapters to choose from, got {n}")
+    if num_groups < 1 or num_groups > _MOST_GROUPS or n % num_groups != 0:
+        raise ValueError(f"num_groups ({num_groups}) must divide the {n} chapters to choose from and be at most {_MOST_GROUPS}")
+    keep = num_groups if top_groups is None else int(top_groups)
+    if keep < 1 or keep > num_groups:
+        raise ValueError(f"top_groups must be in 1..{num_groups}, got {keep}")
+    if top_k <= 0:
+        raise ValueError(f"top_k must be > 0, got {top_k}")
+    k = min(int(top_k), n)
+    if k > _MOST_SELECTED or k > keep * (n // num_groups):
+        raise ValueError(f"top_k ({k}) must be at most {_MOST_SELECTED} and the {keep * (n // num_groups)} chapters of {keep} groups")
+    return L.SelectShape(rows, chapters, k, num_shared, ops.SCORES[score], num_groups, keep, int(group_score == "top2"),
+                         int(bool(renormalize)), 0, 0, float(routed_scale))
+
+
+def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax", balance_bias: Optional[torch.Tensor] = None,
+                    num_shared: int = 0, routed_scale: float = 1.0, num_groups: int = 1, top_groups: Optional[int] = None,
+                    group_score: str = "max", renormalize: bool = True) -> ChapterSelection:
+    """Top-k chapters of every row of ``logits`` [..., C] (fp32 or bf16), by rules beyond the reference router's.
+
+    The first ``num_shared`` chapters are not chosen from; the others score ``softmax`` or ``sigmoid`` of their logits.
+    ``balance_bias`` [C] fp32 is added to the scores in the selection alone (no gradient; :func:`memory_b200.ops.balance_bias_step`
+    moves it by ``load``).  With ``num_groups`` runs of equal size only the ``top_groups`` best stay, by their largest score or the
+    sum of their ``top2``.  Order: score with bias descending, id ascending, as exact arithmetic has it.  Weights are the scores
+    (without bias), divided by their sum with ``renormalize``; the joint list puts the shared chapters in front at weight 1, scales
+    the others by ``routed_scale`` and divides by the sum.
+
+    A logit at or below -3.3895e38 (the lowest bfloat16; -inf too) masks its chapter: it comes after all others, lowest id first, with
+    weight 0, so a row that is masked as a whole gets the first ids and zero weights.  A NaN makes its row's weights NaN (softmax)
+    or its own (sigmoid) and comes first.  Differentiable in ``logits`` through both weights."""
+    if logits.dim() < 2:
+        raise ValueError(f"logits must be [..., num_chapters], got shape {tuple(logits.shape)}")
+    c = logits.shape[-1]
+    lead = logits.shape[:-1]
+    rows = logits.numel() // max(c, 1)
+    s = _select_shape(rows, c, int(top_k), score, int(num_shared), routed_scale, int(num_groups), top_groups, group_score, renormalize)
+    L.require_cuda(logits, balance_bias)
+    if balance_bias is not None:
+        _check_numel("balance_bias", balance_bias, c)
+        if balance_bias.device != logits.device:
+            raise ValueError("balance_bias must be on the device of the logits")
+        balance_bias = ops._contig(balance_bias.detach().float())
+    z = logits if logits.dim() == 2 else logits.reshape(-1, c)
+    if z.stride(1) != 1 or z.stride(0) < c:
+        z = z.contiguous()
+    s.dtype, s.ld = L.dtype_code(z.dtype), max(c, z.stride(0))
+    if rows == 0:
+        dev, joint = z.device, s.num_shared + s.top_k
+        flat = (z.new_empty(0, s.top_k, dtype=torch.int64), z.new_empty(0, s.top_k, dtype=torch.float32),
+                z.new_empty(0, joint, dtype=torch.int32), z.new_empty(0, joint, dtype=torch.float32),
+                torch.zeros(c, dtype=torch.int32, device=dev))
+    else:
+        flat = _Select.apply(z, balance_bias, s)
+    if logits.dim() == 2:
+        return ChapterSelection(*flat)
+    return ChapterSelection(*[t.view(*lead, t.shape[-1]) for t in flat[:4]], flat[4])
+
+
+class _RouterLogits(torch.autograd.Function):
+    """Logits of a router: of every token (``pos_weight`` None), or of the states pooled with one coefficient per position
+    (the mean, or ChapterRouter's rolling windows).  fp32, bias included."""
+
+    @staticmethod
+    def forward(ctx, h, weight, bias, pos_weight):
+        _check_width("router weight", weight, h.shape[2])
+        _check_numel("router bias", bias, weight.shape[0])
+        L.require_cuda(h, weight, bias, pos_weight)
+        b, l, d = h.shape
+        w = ops._contig(weight.detach().float())
+        if pos_weight is not None:
+            x = ops.pool_weighted_fwd(h, pos_weight)
+        else:
+            x = ops._contig(h.reshape(b * l, d))
+        c = w.shape[0]
+        split = x.dtype == torch.bfloat16 and d % 8 == 0 and x.shape[0] * c * d >= _SPLIT_ROUTER_MIN_WORK
+        if x.dtype == torch.bfloat16 and not split:
+            x = ops.cast(x, torch.float32)
+        logits = ops.gemm_split(x, w, tag="router_logits") if split else ops.gemm(x, w, tag="router_logits")
+        if bias is not None:
+            logits = ops.sum_terms(logits, c, 1, bias.detach().float())
+        ctx.cfg = (b, l, d), h.dtype, split, bias is not None
+        ctx.save_for_backward(x, w, pos_weight)
+        return logits
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, w, pos_weight = ctx.saved_tensors
+        (b, l, d), dtype, split, has_bias = ctx.cfg
+        g = ops._contig(g.float())
+        d_h = d_w = d_b = None
+        if ctx.needs_input_grad[2] and has_bias:
+            d_b = ops.col_sum(g)
+        if split and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
+            # the tensor cores take rows of whole 16 bytes: chapters and tokens in multiples of 8
+            gc, gr = -w.shape[0] % 8, -x.shape[0] % 8
+            g = torch.nn.functional.pad(g, (0, gc, 0, gr)) if gc or gr else g
+            w = torch.nn.functional.pad(w, (0, 0, 0, gc)) if gc else w
+            x = torch.nn.functional.pad(x, (0, 0, 0, gr)) if gr else x
+            if ctx.needs_input_grad[0]:
+                d_h = ops.gemm_split(g, w, b_kmajor=False, tag="router_dh")[:b * l]
+            if ctx.needs_input_grad[1]:
+                d_w = ops.gemm_split(g, x, a_kmajor=False, b_kmajor=False, tag="router_dw")[:g.shape[1] - gc]
+        else:
+            if ctx.needs_input_grad[0]:
+                d_h = ops.gemm(g, w, b_kmajor=False, tag="router_dh")
+            if ctx.needs_input_grad[1]:
+                d_w = ops.gemm(g, x, a_kmajor=False, b_kmajor=False, tag="router_dw")
+        if d_h is not None:
+            d_h = (ops.pool_weighted_bwd(d_h, pos_weight, (b, l, d), dtype) if pos_weight is not None
+                   else d_h.reshape(b, l, d).to(dtype))
+        return d_h, d_w, d_b, None
+
+
+def router_logits(h: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                  pos_weight: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fp32 logits [B * L, C] of the tokens of ``h`` [B, L, d], or [B, C] of the states pooled with ``pos_weight`` [L]."""
+    if h.dim() != 3:
+        raise ValueError(f"hidden_states must be 3D (B, T, D), got shape {tuple(h.shape)}")
+    return _RouterLogits.apply(h, weight, bias, pos_weight)
+
+
+# --------------------------------------------------------------------------------------------
+# a block's output merged into the residual stream
+# --------------------------------------------------------------------------------------------
+class _GatedResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, weight, bias, gate, next_weight, next_bias, s):
+        ctx.set_materialize_grads(False)
+        params = weight, bias, gate, next_weight, next_bias
+        x, f = ops._contig(x), ops._contig(f)
+        p32 = [None if t is None else ops._contig(t.detach().float()) for t in params]
+        train = any(ctx.needs_input_grad)
+        y, n, stats = ops.gated_residual_fwd(s, x, f, *p32, train)
+        if train:
+            ctx.save_for_backward(x, f, *p32, stats)
+            ctx.s, ctx.dtypes = s, [None if t is None else t.dtype for t in params]
+        return y, n
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_y, d_n):
+        if d_y is None and d_n is None:
+            return (None,) * 8
+        x, f, weight, bias, gate, next_weight, next_bias, stats = ctx.saved_tensors
+        d_y = None if d_y is None else ops._contig(d_y.to(x.dtype))
+        d_n = None if d_n is None else ops._contig(d_n.to(f.dtype))
+        d_x, d_f, *d_params = ops.gated_residual_bwd(ctx.s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n,
+                                                     ctx.needs_input_grad[0], bias is not None, next_bias is not None)
+        if d_n is None:
+            d_params[3] = d_params[4] = None           # the next norm was not used: no gradient, not a zero one
+        d_params = [None if t is None or not need else t.to(dt)
+                    for t, dt, need in zip(d_params, ctx.dtypes, ctx.needs_input_grad[2:7])]
+        return d_x, d_f if ctx.needs_input_grad[1] else None, *d_params, None
+
+
+def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                        norm_type: str = "rms", eps: float = 1e-6, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+                        next_weight: Optional[torch.Tensor] = None, next_bias: Optional[torch.Tensor] = None,
+                        next_eps: Optional[float] = None):
+    """``y = residual_scale * x + gate * norm(branch)`` and, with ``next_weight``, ``(y, norm(y))`` with the next block's weights,
+    in one pass each way.
+
+    ``x`` (the residual stream) and ``branch`` (a block's output) are [B, L, d] (or [rows, d]), fp32 or bf16 each; y has the
+    type of ``x``, the next norm's result that of ``branch`` and is taken of y before y is rounded.  ``norm_type`` is ``rms`` (no
+    biases) or ``layernorm``.  ``gate``: None, [d], or [B, d] with one row per sequence (as adaptive norms have it).  Sums,
+    statistics and parameter gradients are fp32.  d is at most 8192."""
+    if x.dim() not in (2, 3) or x.shape != branch.shape:
+        raise ValueError(f"x and branch must share a shape [B, L, d] or [rows, d], got {tuple(x.shape)} and {tuple(branch.shape)}")
+    if norm_type not in ("rms", "layernorm"):
+        raise ValueError(f"norm_type must be 'rms' or 'layernorm', got {norm_type!r}")
+    d = x.shape[-1]
+    if not 1 <= d <= 8192:
+        raise ValueError(f"the width must be in 1..8192, got {d}")
+    if norm_type == "rms" and (bias is not None or next_bias is not None):
+        raise ValueError("an RMSNorm has no bias")
+    if next_bias is not None and next_weight is None:
+        raise ValueError("next_bias needs next_weight")
+    params = {"weight": weight, "bias": bias, "next_weight": next_weight, "next_bias": next_bias}
+    for name, t in params.items():
+        if t is not None and (t.dim() != 1 or t.shape[0] != d):
+            raise ValueError(f"{name} must have {d} elements, got shape {tuple(t.shape)}")
+    gate_seq = 0
+    if gate is not None and gate.dim() == 2 and x.dim() == 3 and tuple(gate.shape) == (x.shape[0], d):
+        gate_seq = x.shape[1]
+    elif gate is not None and tuple(gate.shape) != (d,):
+        raise ValueError(f"gate must be [d] or, beside [B, L, d], [B, d]; got shape {tuple(gate.shape)} for {tuple(x.shape)}")
+    L.require_cuda(x, branch, gate, *params.values())
+    if any(t is not None and t.device != x.device for t in (branch, gate, *params.values())):
+        raise ValueError("all tensors must be on the device of x")
+    rows = x.numel() // d
+    s = L.ResidualShape(rows, d, L.NORM_CODES[norm_type], L.dtype_code(x.dtype), L.dtype_code(branch.dtype), gate_seq,
+                        float(residual_scale), float(eps), float(eps if next_eps is None else next_eps))
+    if rows == 0:
+        y = x * residual_scale + 0.0 * branch.to(x.dtype)          # (nothing to compute; a graph that gives zero gradients)
+        return (y, 0.0 * branch) if next_weight is not None else y
+    if gate_seq and x.shape[0] > 65534:
+        raise ValueError("at most 65,534 sequences with a gate of their own")
+    y, n = _GatedResidual.apply(x, branch, weight, bias, gate, next_weight, next_bias, s)
+    return (y, n) if next_weight is not None else y

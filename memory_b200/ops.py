@@ -4,6 +4,7 @@ Every function requires CUDA tensors; nothing here computes on the host.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Dict, Optional, Tuple
 
@@ -15,6 +16,14 @@ from . import _lib as L
 
 def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else (t if t.is_contiguous() else t.contiguous())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch where it is not: a stream belongs to its device."""
+    return _HERE if torch._C._cuda_getDevice() == L.device_index(device) else torch.cuda.device(device)
 
 
 # Kernel-launch accounting and optional per-call CUDA-event timing (used by the benchmark).  A kernel that leaves at once because the
@@ -279,6 +288,57 @@ def agree_probe(device, late_warps: int, poll_limit: int):
 
 
 # --------------------------------------------------------------------------------------------
+# selection from logits
+# --------------------------------------------------------------------------------------------
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+@_instrument("select_fwd", 1)
+def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s):
+    """``moc_select_fwd`` on logits [rows, C] (fp32 or bf16, unit column stride); ``s``: the filled ``SelectShape``.  Returns (idx
+    int64, weights, joint idx int32, joint weights, row stats, load)."""
+    dev, rows, k, joint = logits.device, s.rows, s.top_k, s.num_shared + s.top_k
+    # one allocation for the fp32 outputs and the two int32 lists (fp32 row stats first: they want 16 bytes)
+    idx = torch.empty(rows, k, dtype=torch.int64, device=dev)
+    f = torch.empty(rows * (4 + k + joint), dtype=torch.float32, device=dev)
+    i = torch.empty(rows * joint + s.num_chapters, dtype=torch.int32, device=dev)
+    stats, weights, comb_w = f[:rows * 4].view(rows, 4), f[rows * 4:rows * (4 + k)].view(rows, k), f[rows * (4 + k):].view(rows, joint)
+    comb_idx, load = i[:rows * joint].view(rows, joint), i[rows * joint:]
+    with _on(dev):
+        rc = L.lib().moc_select_fwd(C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(),
+                                    comb_idx.data_ptr(), comb_w.data_ptr(), stats.data_ptr(), load.data_ptr(), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "moc_select_fwd")
+    return idx, weights, comb_idx, comb_w, stats, load
+
+
+@_instrument("select_bwd", 1)
+def select_bwd(logits: torch.Tensor, s, idx, weights, comb_w, stats, g_weights, g_comb) -> torch.Tensor:
+    """Gradient of the logits [rows, C] (dense, their type) from those of the weights and the joint weights (either may be None)."""
+    dev = logits.device
+    d = torch.empty(s.rows, s.num_chapters, dtype=logits.dtype, device=dev)
+    with _on(dev):
+        rc = L.lib().moc_select_bwd(C.byref(s), logits.data_ptr(), idx.data_ptr(), weights.data_ptr(), comb_w.data_ptr(),
+                                    stats.data_ptr(), L.ptr(g_weights), L.ptr(g_comb), d.data_ptr(), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "moc_select_bwd")
+    return d
+
+
+@_instrument("balance_bias_step", 1)
+def balance_bias_step(bias: torch.Tensor, load: torch.Tensor, num_shared: int, rate: float) -> None:
+    """bias[c] += rate * sign(mean load - load[c]) in place over the chapters behind the shared ones."""
+    L.require_cuda(bias, load)
+    if bias.dtype != torch.float32 or bias.dim() != 1 or not bias.is_contiguous():
+        raise TypeError("the balance bias must be a contiguous fp32 vector")
+    if load.dtype != torch.int32 or load.shape != bias.shape or load.device != bias.device or not load.is_contiguous():
+        raise ValueError("load must be int32 counts shaped like the bias, on its device")
+    with _on(bias.device):
+        L.check(L.lib().moc_balance_bias_step(L.ptr(bias), L.ptr(load), bias.numel(), int(num_shared), float(rate),
+                                              L.stream_ptr(bias.device)), "moc_balance_bias_step")
+
+
+# --------------------------------------------------------------------------------------------
 # gather
 # --------------------------------------------------------------------------------------------
 @_instrument("gather_rows_fwd", 1)
@@ -497,9 +557,13 @@ def bank_adamw_step(param: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torc
                     num_unique: torch.Tensor, grad_rows: torch.Tensor, tokens_per_chapter: int, *, lr: float,
                     betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, step: int = 1,
                     grad_scale: float = 1.0, shadow: Optional[torch.Tensor] = None,
-                    workspace: Optional[torch.Tensor] = None) -> None:
-    """In-place AdamW update of every bank row from a compact gradient (see ``moc_bank_adamw_step``)."""
-    L.require_cuda(param, exp_avg, exp_avg_sq, uniq, num_unique, grad_rows, shadow)
+                    workspace: Optional[torch.Tensor] = None, device_scale: Optional[torch.Tensor] = None) -> None:
+    """In-place AdamW update of every bank row from a compact gradient (see ``moc_bank_adamw_step``).  ``device_scale``: one
+    fp32 number on the device that multiplies the gradient beside ``grad_scale``."""
+    L.require_cuda(param, exp_avg, exp_avg_sq, uniq, num_unique, grad_rows, shadow, device_scale)
+    if device_scale is not None and (device_scale.dtype != torch.float32 or device_scale.numel() != 1
+                                     or device_scale.device != param.device):
+        raise TypeError("a gradient scale on the device must be one fp32 number beside the parameter")
     for t in (param, exp_avg, exp_avg_sq, grad_rows):
         if t.dtype != torch.float32 or not t.is_contiguous():
             raise TypeError("parameter, moments and gradient rows must be contiguous fp32 tensors")
@@ -511,12 +575,42 @@ def bank_adamw_step(param: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torc
     need = lib.moc_bank_adamw_workspace_bytes(c)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=param.device)
-    rc = lib.moc_bank_adamw_step(L.ptr(param), L.ptr(exp_avg), L.ptr(exp_avg_sq), rows, d, int(tokens_per_chapter),
-                                 L.ptr(uniq), L.ptr(num_unique), uniq.numel(), L.ptr(grad_rows), float(grad_scale),
-                                 float(lr), float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
-                                 int(step), L.ptr(shadow), L.ptr(workspace), workspace.numel(),
-                                 L.ptr(L.status_word(param.device)), L.stream_ptr(param.device))
+    rc = lib.moc_bank_adamw_step_scaled(L.ptr(param), L.ptr(exp_avg), L.ptr(exp_avg_sq), rows, d, int(tokens_per_chapter),
+                                        L.ptr(uniq), L.ptr(num_unique), uniq.numel(), L.ptr(grad_rows), float(grad_scale),
+                                        L.ptr(device_scale), float(lr), float(betas[0]), float(betas[1]), float(eps),
+                                        float(weight_decay), int(step), L.ptr(shadow), L.ptr(workspace), workspace.numel(),
+                                        L.ptr(L.status_word(param.device)), L.stream_ptr(param.device))
     L.check(rc, "moc_bank_adamw_step")
+
+
+_GRAD_DTYPES = {torch.float32: L.MOC_F32, torch.bfloat16: L.MOC_BF16, torch.float16: L.MOC_F16}
+
+
+def _grad_clip_launches(entries, *a, **k):
+    return 2 * (1 if len(entries) <= 64 else -(-len(entries) // 680))
+
+
+@_instrument("grad_clip", _grad_clip_launches)
+def grad_clip(entries, max_norm: float, eps: float, device: torch.device) -> torch.Tensor:
+    """``moc_grad_clip``: ``entries`` are (gradient, output or None, count or None, unit, weight) with dense tensors on
+    ``device``.  Returns [2] fp32 = (norm, coefficient)."""
+    n = len(entries)
+    table = (L.GradDesc * n)()
+    codes = _GRAD_DTYPES
+    for d, (g, out, count, unit, weight) in zip(table, entries):
+        d.grad, d.elems, d.dtype, d.unit, d.weight = g.data_ptr(), g.numel(), codes[g.dtype], unit, weight
+        if out is not None:
+            d.out, d.out_dtype = out.data_ptr(), codes[out.dtype]
+        if count is not None:
+            d.count = count.data_ptr()
+    lib = L.lib()
+    result = torch.empty(2, dtype=torch.float32, device=device)
+    ws = torch.empty(lib.moc_grad_clip_workspace_bytes(n), dtype=torch.uint8, device=device)
+    with _on(device):
+        rc = lib.moc_grad_clip(table, n, float(max_norm), float(eps), result.data_ptr(), ws.data_ptr(), ws.numel(),
+                               L.stream_ptr(device))
+    L.check(rc, "moc_grad_clip")
+    return result
 
 
 @_instrument("rows_sqnorm", 2)
@@ -1208,8 +1302,105 @@ def norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, stats: tor
 
 
 # --------------------------------------------------------------------------------------------
+# a block's output merged into the residual stream
+# --------------------------------------------------------------------------------------------
+@_instrument("gated_residual_fwd", 1)
+def gated_residual_fwd(s, x, f, weight, bias, gate, next_weight, next_bias, want_stats: bool):
+    """``moc_gated_residual_fwd`` on dense x and f; returns (y like x, n like f or None, stats or None)."""
+    dev, p = x.device, L.ptr
+    y = torch.empty_like(x)
+    n = torch.empty_like(f) if next_weight is not None else None
+    stats = torch.empty(s.rows, 4, dtype=torch.float32, device=dev) if want_stats else None
+    with _on(dev):
+        rc = L.lib().moc_gated_residual_fwd(C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight),
+                                            p(next_bias), y.data_ptr(), p(n), p(stats), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "moc_gated_residual_fwd")
+    return y, n, stats
+
+
+@_instrument("gated_residual_bwd", 2)
+def gated_residual_bwd(s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n, want_dx: bool, want_bias: bool,
+                       want_next_bias: bool):
+    """Gradients of :func:`gated_residual_fwd`: (d_x or None, d_f, d_weight, d_bias, d_gate, d_next_weight, d_next_bias)."""
+    dev, p, lib = x.device, L.ptr, L.lib()
+    d_x = torch.empty_like(x) if want_dx else None
+    d_f = torch.empty_like(f)
+
+    def vector(like, want=True):
+        return torch.empty_like(like) if like is not None and want else None
+    d_w, d_gate = vector(weight), vector(gate)
+    d_b, d_nw = vector(weight, want_bias), vector(next_weight)
+    d_nb = vector(next_weight, want_next_bias)
+    with _on(dev):
+        scratch = torch.empty(lib.moc_gated_residual_bwd_scratch_bytes(C.byref(s), int(gate is not None)), dtype=torch.uint8, device=dev)
+        rc = lib.moc_gated_residual_bwd(C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight),
+                                        stats.data_ptr(), p(d_y), p(d_n), p(d_x), d_f.data_ptr(), p(d_w), p(d_b), p(d_gate), p(d_nw),
+                                        p(d_nb), scratch.data_ptr(), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "moc_gated_residual_bwd")
+    return d_x, d_f, d_w, d_b, d_gate, d_nw, d_nb
+
+
+# --------------------------------------------------------------------------------------------
 # decode-time attention over cached projected bank rows
 # --------------------------------------------------------------------------------------------
+def check_cache(kv_bank: torch.Tensor, kv_scale: Optional[torch.Tensor], scale_rows: int, tokens_per_chapter: int,
+                num_kv_heads: int) -> None:
+    """Refuses a K/V cache whose parts contradict each other."""
+    if kv_scale is None:
+        if kv_bank.dtype != torch.bfloat16:
+            raise TypeError("decode attention runs on a bf16 K/V cache, or on e4m3 values with their scales")
+        return
+    if kv_bank.dim() != 2 or tokens_per_chapter <= 0 or kv_bank.shape[0] % tokens_per_chapter != 0:
+        raise ValueError("kv_bank must be [rows, 2 * num_kv_heads * head_dim] with whole chapters of rows")
+    if kv_bank.dtype != torch.float8_e4m3fn or kv_scale.dtype != torch.float32:
+        raise TypeError("an 8-bit K/V cache is e4m3 values with fp32 scales")
+    if scale_rows <= 0 or tokens_per_chapter % scale_rows != 0:
+        raise ValueError(f"a chapter of {tokens_per_chapter} rows must be whole blocks of scale_rows ({scale_rows})")
+    if tuple(kv_scale.shape) != (kv_bank.shape[0] // scale_rows, 2 * num_kv_heads) or not kv_scale.is_contiguous():
+        raise ValueError("kv_scale must be a dense [rows / scale_rows, 2 * num_kv_heads]")
+    if kv_scale.device != kv_bank.device:
+        raise ValueError("kv_scale and kv_bank must be on one device")
+
+
+@_instrument("quantize_rows", 1)
+def quantize_rows(rows: torch.Tensor, scale_rows: int, head_dim: int, values: torch.Tensor, scales: torch.Tensor) -> None:
+    """bf16 ``rows`` [n, heads * head_dim] -> ``values`` (e4m3, same shape) and ``scales`` fp32 [n / scale_rows, heads]
+    (``moc_quantize_rows``); both are dense."""
+    L.require_cuda(rows, values, scales)
+    if rows.dtype != torch.bfloat16 or values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError("the 8-bit cache is made from bf16 rows: e4m3 values and fp32 scales")
+    heads = rows.shape[1] // head_dim
+    if (values.shape != rows.shape or tuple(scales.shape) != (rows.shape[0] // scale_rows, heads) or rows.shape[0] % scale_rows != 0
+            or not (values.is_contiguous() and scales.is_contiguous())):
+        raise ValueError("values must be dense and shaped like the rows, scales [rows / scale_rows, heads]")
+    rows = _contig(rows)
+    with _on(rows.device):
+        rc = L.lib().moc_quantize_rows(rows.data_ptr(), rows.shape[0], heads, int(head_dim), int(scale_rows), values.data_ptr(),
+                                       scales.data_ptr(), L.stream_ptr(rows.device))
+    L.check(rc, "moc_quantize_rows")
+
+
+@_instrument("decode_attn_cache", 1)
+def decode_attn_cache(q, kv_bank, kv_scale, scale_rows: int, idx, weights, counts, num_heads: int, num_kv_heads: int,
+                      tokens_per_chapter: int, scale: float, want_lse: bool):
+    """``moc_decode_attn_cache``: q [B, n_q, H*64] bf16 over a bf16 cache (``kv_scale`` None) or an 8-bit one.  Returns (out, lse or
+    None)."""
+    b, n_q, hd = q.shape
+    dev = q.device
+    s = L.DecodeShape(b, n_q, num_heads, num_kv_heads, hd // num_heads, idx.shape[1], tokens_per_chapter, scale)
+    out = torch.empty_like(q)
+    lse = torch.empty(b, n_q, num_heads, dtype=torch.float32, device=dev) if want_lse else None
+    with _on(dev):
+        rc = L.lib().moc_decode_attn_cache(C.byref(s), q.data_ptr(), kv_bank.data_ptr(), L.ptr(kv_scale), scale_rows, kv_bank.shape[0],
+                                           idx.data_ptr(), weights.data_ptr(), L.ptr(counts), out.data_ptr(), L.ptr(lse),
+                                           L.ptr(L.status_word(dev)), L.stream_ptr(dev))
+    if rc:
+        L.check(rc, "moc_decode_attn_cache")
+    return out, lse
+
+
 @_instrument("decode_attn", 1)
 def decode_attn(q: torch.Tensor, kv_bank: torch.Tensor, comb_idx: torch.Tensor, comb_w: torch.Tensor,
                 num_heads: int, num_kv_heads: int, tokens_per_chapter: int, scale: float, want_lse: bool = False):
@@ -1270,10 +1461,12 @@ _DECODE_PLANS_MAX = 32
 def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: torch.Tensor,
                 router_b: Optional[torch.Tensor], wq: torch.Tensor, wo: torch.Tensor, kv_bank: torch.Tensor, *,
                 num_heads: int, num_kv_heads: int, tokens_per_chapter: int, top_k: int, num_shared: int,
-                routed_scale: float, scale: float, plans: Optional[dict] = None):
+                routed_scale: float, scale: float, plans: Optional[dict] = None, kv_scale: Optional[torch.Tensor] = None,
+                scale_rows: int = 0):
     """One decoding step (``moc_decode_step``): out [B, n_q, d] in the dtype of ``hidden``, then indices int64, weights,
     combined indices int32 and combined weights of the router.  ``plans``: a dict the caller keeps; descriptors of calls
-    that agree in shapes, types and weights (by address) are filled once."""
+    that agree in shapes, types and weights (by address) are filled once.  ``kv_scale`` [rows / scale_rows, 2 * num_kv_heads]: the
+    scales of a cache held in 8 bits."""
     w = _contig(router_w.float())
     bias = None if router_b is None else _contig(router_b.float())
     h, states = _contig(hidden), _contig(routing_states)
@@ -1283,15 +1476,16 @@ def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: to
     # everything the descriptor holds or a check looked at; the per-step buffers are filled in below
     key = (h.shape, states.shape, w.shape, wq.shape, wo.shape, kv_bank.shape, h.dtype, states.dtype, wq.dtype, wo.dtype,
            kv_bank.dtype, dev, w.data_ptr(), p(bias), None if bias is None else bias.shape, wq.data_ptr(),
-           wo.data_ptr(), kv_bank.data_ptr(), num_heads, num_kv_heads, tokens_per_chapter, top_k, num_shared, routed_scale,
-           scale, stream)
+           wo.data_ptr(), kv_bank.data_ptr(), p(kv_scale), None if kv_scale is None else kv_scale.shape, scale_rows, num_heads,
+           num_kv_heads, tokens_per_chapter, top_k, num_shared, routed_scale, scale, stream)
     plan = None if plans is None else plans.get(key)
     if plan is None:
         L.require_cuda(h, states, w, bias, wq, wo, kv_bank)
         if states.dim() != 3:
             raise ValueError(f"hidden_states must be 3D (B, T, D), got shape {tuple(states.shape)}")
-        if not wq.dtype == wo.dtype == kv_bank.dtype == torch.bfloat16:
-            raise TypeError("decoding runs on bf16 projections and a bf16 K/V cache")
+        check_cache(kv_bank, kv_scale, scale_rows, tokens_per_chapter, num_kv_heads)
+        if not wq.dtype == wo.dtype == torch.bfloat16:
+            raise TypeError("decoding runs on bf16 projections")
         if bias is not None and bias.numel() != w.shape[0]:
             raise ValueError(f"the router's bias must have {w.shape[0]} elements, got {bias.numel()}")
         b, n_q, d = h.shape
@@ -1313,7 +1507,7 @@ def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: to
             L.RouterShape(b, window, rd, c, top_k, num_shared, routed_scale, L.dtype_code(states.dtype)),
             L.DecodeShape(b, n_q, num_heads, num_kv_heads, head_dim, num_shared + k, tokens_per_chapter, scale),
             L.dtype_code(h.dtype), wo.shape[0], kv_bank.shape[0], None, None, p(w), p(bias), p(wq), p(wo), p(kv_bank), None,
-            None, None, None, None, None, p(L.status_word(dev)), stream, _side_stream(L.device_index(dev), stream), d)
+            None, None, None, None, None, p(L.status_word(dev)), stream, _side_stream(L.device_index(dev), stream), d, 0, p(kv_scale), scale_rows)
         plan = bytes(s), _size("moc_decode_step_arena_bytes", s), (b, k), (b, num_shared + k), (b, n_q, wo.shape[0])
         if plans is not None:
             if len(plans) >= _DECODE_PLANS_MAX:
@@ -1334,7 +1528,8 @@ def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: to
           else _timed("decode_step", lambda: L.lib().moc_decode_step(C.byref(s))))
     if rc:
         L.check(rc, "moc_decode_step")
-    _report(s.launches, lambda: ("router_fwd:" + _TAG_OF_CODE[s.router.h_dtype], "gemm:bf16", "decode_attn:bf16", "gemm:bf16"))
+    _report(s.launches, lambda: ("router_fwd:" + _TAG_OF_CODE[s.router.h_dtype], "gemm:bf16",
+                                 "decode_attn:bf16" if kv_scale is None else "decode_attn:e4m3", "gemm:bf16"))
     return out, idx, weights, comb_idx, comb_w
 
 

@@ -4,14 +4,16 @@ The reference hands the bank to ``torch.optim.AdamW`` as its own parameter group
 372-378) and feeds it the dense 262,208 x 768 gradient of ``torch.gather``'s backward.  ``SparseBankAdamW`` applies
 the identical update -- every row, bias-corrected moments, decoupled weight decay -- straight from a
 ``SparseBankGrad`` (chapter ids + rows), in one kernel pass, and can refresh the bf16 working copy of the bank in
-the same pass.
+the same pass.  ``clip_grad_norm_`` is the clipping in front of it (training/trainer.py:876-880), over dense gradients and
+compact ones, without a host round trip.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Iterable, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
+from . import _lib as L
 from . import ops
 from .functional import SparseBankGrad
 
@@ -20,7 +22,7 @@ class SparseBankAdamW:
     """AdamW for one bank parameter ([rows, d] fp32) driven by compact gradients.
 
     ``step(grad)`` takes the ``SparseBankGrad`` a backward pass (or ``GradReducer``) filled; its ``scale`` and the
-    optional ``grad_scale`` (e.g. a clipping coefficient) multiply the gradient.  ``state_dict`` / ``load_state_dict``
+    optional ``grad_scale`` (a number, or the coefficient ``clip_grad_norm_`` left on the device) multiply the gradient.  ``state_dict`` / ``load_state_dict``
     use torch.optim.AdamW's per-parameter keys (``step``, ``exp_avg``, ``exp_avg_sq``), so optimizer state moves
     between the two."""
 
@@ -41,13 +43,16 @@ class SparseBankAdamW:
         self._ws = None
 
     @torch.no_grad()
-    def step(self, grad: SparseBankGrad, grad_scale: float = 1.0, lr: Optional[float] = None) -> None:
+    def step(self, grad: SparseBankGrad, grad_scale: Union[float, torch.Tensor] = 1.0, lr: Optional[float] = None) -> None:
         if len(grad.entries) != 1:
             raise NotImplementedError(
                 "one compact entry per step: sum several layers' entries first (ops.bank_grad_merge)")
         uniq, num_unique, rows, t = grad.entries[0]
         if t != self.t:
             raise ValueError("gradient rows were produced with a different chapter size")
+        on_device = torch.is_tensor(grad_scale) and grad_scale.is_cuda
+        if on_device and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.device != self.param.device):
+            raise TypeError("a gradient scale on the device must be one fp32 number beside the parameter")
         self.step_count += 1
         if self._ws is None:
             self._ws = torch.empty(4 * (self.param.shape[0] // self.t), dtype=torch.uint8, device=self.param.device)
@@ -55,7 +60,8 @@ class SparseBankAdamW:
                             rows if rows.dtype == torch.float32 else rows.float(), self.t,
                             lr=self.lr if lr is None else lr, betas=self.betas, eps=self.eps,
                             weight_decay=self.weight_decay, step=self.step_count,
-                            grad_scale=float(grad.scale) * float(grad_scale), shadow=self.shadow, workspace=self._ws)
+                            grad_scale=float(grad.scale) * (1.0 if on_device else float(grad_scale)), shadow=self.shadow,
+                            workspace=self._ws, device_scale=grad_scale if on_device else None)
 
     def grad_sqnorm(self, grad: SparseBankGrad) -> torch.Tensor:
         """Squared L2 norm of the (scaled) bank gradient as a [1] tensor: the bank's term of a global clip norm."""
@@ -69,3 +75,88 @@ class SparseBankAdamW:
         self.step_count = int(state["step"])
         self.exp_avg.copy_(state["exp_avg"])
         self.exp_avg_sq.copy_(state["exp_avg_sq"])
+
+
+class GradClip(NamedTuple):
+    """Result of :func:`clip_grad_norm_`, both 0-d fp32 on the device: the global norm before clipping, and the factor
+    min(1, max_norm / (norm + eps)) that the gradients were multiplied by (pass it to ``SparseBankAdamW.step`` as
+    ``grad_scale`` for the bank)."""
+    total_norm: torch.Tensor
+    coefficient: torch.Tensor
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *,
+                    bank_grads: Sequence[SparseBankGrad] = (), out: Optional[Sequence[torch.Tensor]] = None,
+                    eps: float = 1e-6) -> GradClip:
+    """Clips gradients by their global norm in two kernel launches, without a host synchronisation.
+
+    ``parameters``: leaves with a gradient (their ``.grad`` is clipped; those without one are passed over), or gradient tensors
+    themselves, fp32, bf16 or fp16 in any mix, all on one device.  ``bank_grads``: compact bank gradients (at most one entry
+    each, with their ``scale``) that count in the norm; their rows are left as they are -- give the coefficient to the optimizer
+    step.  ``out``: one tensor per gradient (same shape, any of the three types) that receives the clipped values instead of the gradients.
+
+    As with ``torch.nn.utils.clip_grad_norm_`` a norm that is NaN makes every gradient NaN and an infinite one gives the coefficient 0.
+    Squares are summed in 64 bits.  A tensor listed twice counts once; tensors that overlap otherwise are refused."""
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    listed = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad if isinstance(p, torch.nn.Parameter) or (p.requires_grad and p.is_leaf) else p for p in listed]
+    if out is None:
+        pairs = [(g, g) for g in grads if g is not None]
+    else:
+        out = list(out)
+        if len(out) != len(grads):
+            raise ValueError(f"out must have one tensor per gradient: {len(out)} vs {len(grads)}")
+        pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
+    device = pairs[0][0].device if pairs else None
+    entries, copies, spans, seen = [], [], [], set()
+    for g, o in pairs:
+        if g.is_sparse or not g.is_cuda or g.device != device:
+            raise ValueError("gradients must be dense CUDA tensors on one device")
+        if g.dtype not in ops._GRAD_DTYPES or o.dtype not in ops._GRAD_DTYPES:
+            raise TypeError(f"gradients must be float32, bfloat16 or float16, got {g.dtype} and {o.dtype}")
+        if o is not g and (o.shape != g.shape or o.device != device):
+            raise ValueError("out must match the gradients in shape and device")
+        n, key = g.numel(), (g.data_ptr(), g.shape, g.stride())
+        if key in seen and n and o is not g:
+            raise ValueError("a gradient is listed twice with an out of its own")
+        if n == 0 or key in seen:
+            continue
+        seen.add(key)
+        src = g if g.is_contiguous() else g.contiguous()
+        dst = src if o is g else o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=device)
+        if dst is not o:
+            copies.append((o, dst))
+        entries.append((src, dst, None, 0, 1.0))
+        spans.append((src.data_ptr(), n * src.element_size()))
+        if dst is not src:
+            spans.append((dst.data_ptr(), n * dst.element_size()))
+    _refuse_overlaps(spans)
+    for sink in bank_grads:
+        if len(sink.entries) > 1:
+            raise NotImplementedError("one compact entry per bank: sum several layers' entries first (ops.bank_grad_merge)")
+        for _, count, rows, t in sink.entries:
+            device = rows.device if device is None else device
+            if rows.device != device or count.device != device:
+                raise ValueError("gradients must be dense CUDA tensors on one device")
+            L.require_cuda(rows, count)
+            entries.append((ops._contig(rows), None, count, t * rows.shape[1], float(sink.scale)))
+    if device is None:
+        raise ValueError("no gradients to clip")
+    result = ops.grad_clip(entries, max_norm, eps, device)
+    for o, dst in copies:
+        o.copy_(dst)
+    norm, coefficient = result.unbind()
+    return GradClip(norm, coefficient)
+
+
+def _refuse_overlaps(spans: list) -> None:
+    """``spans``: (first byte, bytes) of the tensors that are read (and clipped in place) and of separate outputs."""
+    end = 0
+    for first, size in sorted(spans):
+        if first < end:
+            raise ValueError("gradients (and out) must not overlap")
+        end = first + size

@@ -17,9 +17,16 @@ class ChapterRouter(nn.Module):
     (weight N(0, 0.02), zero bias), ``.top_k`` and ``.routing_strategy`` may be changed by the
     caller between calls, ``forward`` returns ``(indices int64, weights, losses)``.
     Selection order is (weight descending, chapter id ascending).
+
+    Beyond the reference: ``score="sigmoid"``, ``balance_bias=True`` (a buffer that :meth:`update_balance` moves towards equal
+    load; it counts in the selection alone), ``num_groups`` / ``top_groups`` / ``group_score`` (group-limited selection over the chapters
+    behind the excluded prefix) and ``renormalize=False`` select by :func:`memory_b200.select_chapters`.  Such a router returns no loss terms (an empty
+    dict): the bias takes the place of the balance loss.  ``last_load`` holds the latest call's count of rows per chapter.
     """
 
-    def __init__(self, hidden_dim: int, num_chapters: int, top_k: int = 1, routing_strategy: str = "sequence"):
+    def __init__(self, hidden_dim: int, num_chapters: int, top_k: int = 1, routing_strategy: str = "sequence", *,
+                 score: str = "softmax", balance_bias: bool = False, num_groups: int = 1, top_groups: Optional[int] = None,
+                 group_score: str = "max", renormalize: bool = True):
         super().__init__()
         if num_chapters <= 0:
             raise ValueError(f"num_chapters must be > 0, got {num_chapters}")
@@ -34,6 +41,35 @@ class ChapterRouter(nn.Module):
         self.router = nn.Linear(hidden_dim, num_chapters, bias=True)
         nn.init.normal_(self.router.weight, mean=0.0, std=0.02)
         nn.init.zeros_(self.router.bias)
+        if score not in ("softmax", "sigmoid"):
+            raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
+        if group_score not in ("max", "top2"):
+            raise ValueError(f"group_score must be 'max' or 'top2', got {group_score!r}")
+        if num_groups < 1 or not 1 <= (num_groups if top_groups is None else top_groups) <= num_groups:
+            raise ValueError(f"top_groups must be in 1..num_groups, got {top_groups} of {num_groups}")
+        self.selection = {"score": score, "num_groups": num_groups, "top_groups": top_groups, "group_score": group_score,
+                          "renormalize": renormalize}
+        self.by_logits = (score, renormalize) != ("softmax", True) or balance_bias or top_groups not in (None, num_groups)
+        self.last_load: Optional[torch.Tensor] = None
+        self.register_buffer("balance_bias", torch.zeros(num_chapters) if balance_bias else None)
+
+    def select(self, logits: torch.Tensor, num_shared: int, routed_scale: float = 1.0) -> F_moc.ChapterSelection:
+        """This router's selection from logits [rows, num_chapters]."""
+        got = F_moc.select_chapters(logits, self.top_k, balance_bias=self.balance_bias, num_shared=num_shared,
+                                    routed_scale=routed_scale, **self.selection)
+        self.last_load = got.load
+        return got
+
+    def update_balance(self, rate: float = 1e-3, load: Optional[torch.Tensor] = None, num_shared: int = 0) -> None:
+        """Moves the balance bias of every chapter behind the shared ones by ``rate`` towards the mean load: up where fewer rows
+        chose it, down where more did.  ``load`` [C] int32: the counts of a step (summed over ranks, say); the latest call's by
+        default."""
+        if self.balance_bias is None:
+            raise ValueError("this router has no balance bias")
+        load = self.last_load if load is None else load
+        if load is None:
+            raise ValueError("no load yet: route first, or pass the counts")
+        F_moc.ops.balance_bias_step(self.balance_bias, load, num_shared, rate)
 
     def forward(self, hidden_states: torch.Tensor, return_losses: bool = True, exclude_prefix_chapters: int = 0,
                 rolling_window_size: Optional[int] = None
@@ -53,9 +89,19 @@ class ChapterRouter(nn.Module):
         if exclude_prefix_chapters < 0 or exclude_prefix_chapters > self.num_chapters:
             raise ValueError(
                 f"exclude_prefix_chapters must be in [0, {self.num_chapters}], got {exclude_prefix_chapters}")
+        if self.by_logits:
+            got = self.select(self._pooled_logits(hidden_states, pos_weight), exclude_prefix_chapters)
+            return got.indices, got.weights, {}
         idx, w, _, _, losses = F_moc.route(hidden_states, self.router.weight, self.router.bias, self.top_k,
                                            exclude_prefix_chapters, 1.0, return_losses, pos_weight=pos_weight)
         return idx, w, losses
+
+    def _pooled_logits(self, hidden_states: torch.Tensor, pos_weight: Optional[torch.Tensor]) -> torch.Tensor:
+        if hidden_states.dim() != 3:
+            raise ValueError(f"hidden_states must be 3D (B, T, D), got shape {tuple(hidden_states.shape)}")
+        if pos_weight is None:          # the mean is the window that spans the sequence: one coefficient, 1 / L
+            pos_weight = torch.full((hidden_states.shape[1],), 1.0 / max(1, hidden_states.shape[1]), device=hidden_states.device)
+        return F_moc.router_logits(hidden_states, self.router.weight, self.router.bias, pos_weight)
 
     def _rolling_coefficients(self, seq: int, window: Optional[int], device) -> torch.Tensor:
         key = (int(seq), None if window is None else int(window), str(device))
@@ -77,6 +123,10 @@ class ChapterRouter(nn.Module):
         if exclude_prefix_chapters < 0 or exclude_prefix_chapters > self.num_chapters:
             raise ValueError(
                 f"exclude_prefix_chapters must be in [0, {self.num_chapters}], got {exclude_prefix_chapters}")
+        if self.by_logits:
+            b, l, _ = hidden_states.shape
+            got = self.select(F_moc.router_logits(hidden_states, self.router.weight, self.router.bias), exclude_prefix_chapters)
+            return got.indices.view(b, l, -1), got.weights.view(b, l, -1), {}
         return F_moc.route_tokens(hidden_states, self.router.weight, self.router.bias, self.top_k,
                                   exclude_prefix_chapters, return_losses)
 
@@ -84,6 +134,9 @@ class ChapterRouter(nn.Module):
                           routed_scaling_factor: float, return_losses: bool = True):
         """Router plus the model-side shared-prefix step (model.py:356-391) in one launch sequence.
         Returns (indices, weights, combined_indices int32, combined_weights, losses)."""
+        if self.by_logits:
+            got = self.select(self._pooled_logits(hidden_states, None), num_shared_chapters, routed_scaling_factor)
+            return got.indices, got.weights, got.combined_indices, got.combined_weights, {}
         return F_moc.route(hidden_states, self.router.weight, self.router.bias, self.top_k,
                            num_shared_chapters, routed_scaling_factor, return_losses)
 
