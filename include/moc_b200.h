@@ -186,7 +186,7 @@ int moc_token_route_bwd(const moc_token_route_desc* s, const float* g_weights, c
  * order of exact arithmetic.  weights = s of the chosen, divided by max(their sum, 1e-12) with renormalize.  A logit at or below
  * -3.3895e38 (the lowest finite bfloat16; -inf too) is masked: chosen after all others, lowest id first, with weight 0.
  * idx [rows, top_k] int64, weights [rows, top_k]; joint list as in moc_router_fwd: comb_idx / comb_w [rows, num_shared + top_k];
- * row_stats [rows, 4] (16-byte aligned) goes to the backward pass; load [num_chapters] int32 (NULL: not wanted) = rows that chose
+ * row_stats [rows, 4] (16-byte aligned; NULL: no backward pass) goes to the backward pass; load [num_chapters] int32 (NULL: not wanted) = rows that chose
  * each chapter.  Limits: 16384 chapters to choose from, top_k 128, 64 groups of equal size, top_k <= chapters of top_groups groups. */
 #define MOC_SCORE_SOFTMAX 0
 #define MOC_SCORE_SIGMOID 1
@@ -665,20 +665,16 @@ int moc_bank_adamw_step_scaled(float* param, float* exp_avg, float* exp_avg_sq, 
                                void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 /* Global gradient norm over many tensors and the clipped tensors (the reference: torch.nn.utils.clip_grad_norm_ over every
  * parameter, training/trainer.py:876-880):  norm = sqrt(sum_i weight_i^2 sum g_i^2),  coefficient = min(1, max_norm / (norm + eps)),
- * out_i = coefficient g_i (NaN stays NaN).  result [2] fp32 (device) = {norm, coefficient}.  `grads` is a host array; a tensor
- * without `out` counts in the norm alone, `out` equal to `grad` is clipped in place.  Tensors must not overlap.  The number of
- * launches is two for up to 680 tensors.  workspace: moc_grad_clip_workspace_bytes(count), of this call alone. */
-typedef struct {
-  const void* grad;        /* elems elements of `dtype` (MOC_F32, MOC_BF16 or MOC_F16), aligned to their type */
-  void* out;               /* as many of out_dtype, or NULL */
-  int64_t elems;
-  const int32_t* count;    /* device: the first *count blocks of `unit` elements exist (a compact bank gradient); NULL: all */
-  int32_t unit, dtype, out_dtype;
-  float weight;            /* factor of the gradient in the norm (1 / world of a sum over ranks) */
-} moc_grad_desc;
+ * out_i = coefficient g_i (NaN stays NaN).  result [2] fp32 (device) = {norm, coefficient}.  The lists are host arrays; the first
+ * `dense` of the `count` tensors have an `out` (equal to the gradient: clipped in place; NULL: it counts in the norm alone), the
+ * others are compact bank gradients of which the first *counts[j] blocks of units[j] elements exist, with the factor weights[j] in
+ * the norm (1 / world of a sum over ranks).  Types: MOC_F32, MOC_BF16 or MOC_F16, each tensor aligned to its own.  Memory that is
+ * written must not overlap anything else in the lists (refused).  Two launches for up to 680 tensors.  workspace:
+ * moc_grad_clip_workspace_bytes(count), 8-byte aligned, of this call alone. */
 int64_t moc_grad_clip_workspace_bytes(int32_t count);
-int moc_grad_clip(const moc_grad_desc* grads, int32_t count, double max_norm, double eps, float* result, void* workspace,
-                  int64_t workspace_bytes, void* stream);
+int moc_grad_clip(int32_t count, int32_t dense, const void* const* grads, const int64_t* elems, const uint8_t* dtypes, void* const* out,
+                  const uint8_t* out_dtypes, const int32_t* const* counts, const int32_t* units, const float* weights, double max_norm,
+                  double eps, float* result, void* workspace, int64_t workspace_bytes, void* stream);
 /* out[0] = sum of squares of the first num_unique*T rows of a compact gradient: the bank's share of the global
  * gradient norm that the reference clips by (training/trainer.py:876-880).  workspace: 592 floats. */
 int moc_rows_sqnorm(const float* rows, const int32_t* num_unique, int32_t tokens_per_chapter, int32_t dim,

@@ -101,9 +101,6 @@ class ResidualShape(C.Structure):
     _fields_ = _fields("l: rows; i: dim kind x_dtype f_dtype gate_seq; f: residual_scale eps next_eps")
 
 
-class GradDesc(C.Structure):
-    _fields_ = _fields("p: grad out; l: elems; p: count; i: unit dtype out_dtype; f: weight")
-
 
 class LayerDesc(C.Structure):
     _fields_ = _fields(
@@ -221,7 +218,7 @@ _PROTOTYPES = {
                                              C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int64, P, P,
                                              C.c_size_t, P, P]),
     "moc_grad_clip_workspace_bytes": (C.c_int64, [C.c_int32]),
-    "moc_grad_clip": (C.c_int, [P, C.c_int32, C.c_double, C.c_double, P, P, C.c_int64, P]),
+    "moc_grad_clip": (C.c_int, [C.c_int32, C.c_int32] + [P] * 8 + [C.c_double, C.c_double, P, P, C.c_int64, P]),
     "moc_select_fwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
     "moc_select_bwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
     "moc_balance_bias_step": (C.c_int, [P, P, C.c_int32, C.c_int32, C.c_float, P]),

@@ -9,6 +9,8 @@
 // the range above 1.8e19 and below 1e-19, and the conversion and the product hide behind HBM, which bounds both passes.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "moc_common.cuh"
 
 namespace moc {
@@ -198,23 +200,42 @@ grad_clip_kernel(const __grid_constant__ ClipTable<N> t, const double* __restric
   }
 }
 
+// The tensors of a call.
+struct GradList {
+  int32_t count, dense;
+  const void* const* grads;
+  const int64_t* elems;
+  const uint8_t* dtypes;
+  void* const* out;
+  const uint8_t* out_dtypes;
+  const int32_t* const* counts;
+  const int32_t* units;
+  const float* weights;
+};
+int bytes_of(int dtype) { return dtype == MOC_F32 ? 4 : 2; }
+
 // go(table, CTAs, CTAs of the launches before) for the tensors in runs of as many as a table holds, once at least
 template <int N, typename Go>
-int each_table(const moc_grad_desc* g, int32_t count, bool write, Go go) {
+int each_table(const GradList& g, bool write, Go go) {
   static thread_local ClipTable<N> t;              // (32 KB: not on the stack of a caller's thread)
   int32_t i = 0;
   int before = 0;
+  const int32_t end = write ? g.dense : g.count;
   do {
     t.entries = 0;
     long long chunks = 0;
-    for (; i < count && t.entries < N; ++i) {
-      if (g[i].elems == 0 || (write && g[i].out == nullptr)) continue;
+    for (; i < end && t.entries < N; ++i) {
+      const bool dense = i < g.dense;
+      if (g.elems[i] == 0 || (write && g.out[i] == nullptr)) continue;
       ClipEntry& e = t.e[t.entries++];
-      e.src = g[i].grad; e.dst = g[i].out; e.n = g[i].elems; e.count = g[i].count; e.unit = g[i].unit;
-      e.weight = g[i].weight; e.dtypes = g[i].dtype | g[i].out_dtype << 8;
+      e.src = g.grads[i]; e.n = g.elems[i];
+      e.dst = dense ? g.out[i] : nullptr;
+      e.dtypes = g.dtypes[i] | (dense ? g.out_dtypes[i] << 8 : 0);
+      e.count = dense ? nullptr : g.counts[i - g.dense];
+      e.unit = dense ? 0 : g.units[i - g.dense];
+      e.weight = dense ? 1.f : g.weights[i - g.dense];
       e.chunk0 = static_cast<int>(chunks);
-      const int size = g[i].dtype == MOC_F32 ? 4 : 2;
-      const long long shift = static_cast<long long>((reinterpret_cast<uintptr_t>(g[i].grad) & 15) / size);
+      const long long shift = static_cast<long long>((reinterpret_cast<uintptr_t>(g.grads[i]) & 15) / bytes_of(g.dtypes[i]));
       chunks += (e.n + shift + kClipChunk - 1) / kClipChunk;
       MOC_REQUIRE(chunks < (1ll << 30), "too many gradient elements in one call");
     }
@@ -223,25 +244,56 @@ int each_table(const moc_grad_desc* g, int32_t count, bool write, Go go) {
     const int rc = go(t, blocks, before);
     if (rc != MOC_OK) return rc;
     before += blocks;
-  } while (i < count);
+  } while (i < end);
   return MOC_OK;
 }
 
 template <int N>
-int grad_clip(const moc_grad_desc* g, int32_t count, double max_norm, double eps, float* result, double* partial, cudaStream_t stream) {
+int grad_clip(const GradList& g, double max_norm, double eps, float* result, double* partial, cudaStream_t stream) {
   int partials = 0;
-  int rc = each_table<N>(g, count, false, [&](const ClipTable<N>& t, int blocks, int before) {
+  int rc = each_table<N>(g, false, [&](const ClipTable<N>& t, int blocks, int before) {
     grad_sqnorm_kernel<N><<<blocks, kClipThreads, 0, stream>>>(t, partial + before);
     MOC_CUDA_OK(cudaGetLastError());
     partials = before + blocks;
     return MOC_OK;
   });
   if (rc != MOC_OK) return rc;
-  return each_table<N>(g, count, true, [&](const ClipTable<N>& t, int blocks, int before) {
+  return each_table<N>(g, true, [&](const ClipTable<N>& t, int blocks, int before) {
     grad_clip_kernel<N><<<blocks, kClipThreads, 0, stream>>>(t, partial, partials, max_norm, eps, before == 0 ? result : nullptr);
     MOC_CUDA_OK(cudaGetLastError());
     return MOC_OK;
   });
+}
+
+// Memory that is written may be read as the same gradient (clipped in place) and by nothing else.
+struct Span {
+  uintptr_t first, end;
+  bool written;
+};
+int check_overlaps(const GradList& g) {
+  static thread_local Span spans[2 * 4096];
+  int n = 0;
+  const int most = static_cast<int>(sizeof(spans) / sizeof(spans[0]));
+  for (int32_t i = 0; i < g.count; ++i) {
+    if (g.elems[i] == 0) continue;
+    MOC_REQUIRE(n + 2 <= most, "at most 4096 tensors in one call");
+    const uintptr_t p = reinterpret_cast<uintptr_t>(g.grads[i]);
+    void* o = i < g.dense ? g.out[i] : nullptr;
+    spans[n++] = Span{p, p + static_cast<uintptr_t>(g.elems[i]) * bytes_of(g.dtypes[i]), o == g.grads[i]};
+    if (o != nullptr && o != g.grads[i]) {
+      const uintptr_t q = reinterpret_cast<uintptr_t>(o);
+      spans[n++] = Span{q, q + static_cast<uintptr_t>(g.elems[i]) * bytes_of(g.out_dtypes[i]), true};
+    }
+  }
+  std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.first < b.first; });
+  // (the furthest end so far, of everything and of what is written)
+  uintptr_t end = 0, end_written = 0;
+  for (int i = 0; i < n; ++i) {
+    MOC_REQUIRE(spans[i].first >= (spans[i].written ? end : end_written), "gradients (and out) must not overlap");
+    end = std::max(end, spans[i].end);
+    if (spans[i].written) end_written = std::max(end_written, spans[i].end);
+  }
+  return MOC_OK;
 }
 
 }  // namespace
@@ -255,23 +307,30 @@ extern "C" int64_t moc_grad_clip_workspace_bytes(int32_t count) {
   return (count / per + 1) * kClipBlocks * static_cast<int64_t>(sizeof(double));
 }
 
-extern "C" int moc_grad_clip(const moc_grad_desc* grads, int32_t count, double max_norm, double eps, float* result, void* workspace,
+extern "C" int moc_grad_clip(int32_t count, int32_t dense, const void* const* grads, const int64_t* elems, const uint8_t* dtypes,
+                             void* const* out, const uint8_t* out_dtypes, const int32_t* const* counts, const int32_t* units,
+                             const float* weights, double max_norm, double eps, float* result, void* workspace,
                              int64_t workspace_bytes, void* stream) {
-  MOC_REQUIRE(count >= 0 && (grads != nullptr || count == 0) && result && workspace, "NULL gradient-clipping argument");
+  MOC_REQUIRE(count >= 0 && dense >= 0 && dense <= count && result && workspace, "NULL gradient-clipping argument");
+  MOC_REQUIRE((grads && elems && dtypes) || count == 0, "NULL gradient list");
+  MOC_REQUIRE((out && out_dtypes) || dense == 0, "NULL list of outputs");
+  MOC_REQUIRE((counts && units && weights) || dense == count, "NULL list of counts");
   MOC_REQUIRE(max_norm >= 0.0 && eps >= 0.0, "max_norm and eps must not be negative");
   MOC_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7) == 0 && workspace_bytes >= moc_grad_clip_workspace_bytes(count),
               "gradient-clipping workspace too small");
   for (int32_t i = 0; i < count; ++i) {
-    const moc_grad_desc& g = grads[i];
-    MOC_REQUIRE(g.elems >= 0 && (g.elems == 0 || g.grad), "NULL gradient");
-    for (int dt : {g.dtype, g.out_dtype}) MOC_REQUIRE(dt == MOC_F32 || dt == MOC_BF16 || dt == MOC_F16, "unknown gradient dtype");
-    MOC_REQUIRE((reinterpret_cast<uintptr_t>(g.grad) & (g.dtype == MOC_F32 ? 3 : 1)) == 0 &&
-                (reinterpret_cast<uintptr_t>(g.out) & (g.out_dtype == MOC_F32 ? 3 : 1)) == 0, "gradients must be aligned to their type");
-    MOC_REQUIRE(g.count == nullptr || (g.unit > 0 && g.out == nullptr), "counted rows need a unit and are not written");
-    MOC_REQUIRE(g.out != g.grad || g.out_dtype == g.dtype, "a gradient clipped in place keeps its type");
+    MOC_REQUIRE(elems[i] >= 0 && (elems[i] == 0 || grads[i]), "NULL gradient");
+    MOC_REQUIRE(dtypes[i] <= MOC_F16 && (i >= dense || out_dtypes[i] <= MOC_F16), "unknown gradient dtype");
+    MOC_REQUIRE(reinterpret_cast<uintptr_t>(grads[i]) % bytes_of(dtypes[i]) == 0 &&
+                (i >= dense || reinterpret_cast<uintptr_t>(out[i]) % bytes_of(out_dtypes[i]) == 0), "gradients must be aligned to their type");
+    MOC_REQUIRE(i >= dense || out[i] != grads[i] || out_dtypes[i] == dtypes[i], "a gradient clipped in place keeps its type");
+    MOC_REQUIRE(i < dense || (units[i - dense] > 0 && counts[i - dense]), "compact rows need a unit and a count");
   }
+  const GradList g{count, dense, grads, elems, dtypes, out, out_dtypes, counts, units, weights};
+  const int rc = check_overlaps(g);
+  if (rc != MOC_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
-  return count <= kFewEntries ? grad_clip<kFewEntries>(grads, count, max_norm, eps, result, partial, st)
-                              : grad_clip<kMostEntries>(grads, count, max_norm, eps, result, partial, st);
+  return count <= kFewEntries ? grad_clip<kFewEntries>(g, max_norm, eps, result, partial, st)
+                              : grad_clip<kMostEntries>(g, max_norm, eps, result, partial, st);
 }

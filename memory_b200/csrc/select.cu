@@ -9,19 +9,20 @@
 // of candidates is filled up with the lowest ids left, weight 0.  The bias counts in the selection alone.
 //
 // The order is that of exact arithmetic.  With a bias, or sums of two, fp32 keys carry errors of the exponential and the
-// quotient; neighbours in the order that are closer than those errors allow (one row in some hundreds) send the row through
-// the same selection in 64 bits.  Bare logits need no arithmetic and are always sure.
+// quotient; where neighbours in the order are closer than those errors allow (a row in some hundreds), the few candidates
+// concerned are ranked again by 64-bit keys.  Rows that this does not settle (groups that close, NaN, fewer candidates than
+// places) run through the same selection in 64 bits as a whole.  Bare logits need no arithmetic and are always sure.
 //
-// Bound by HBM for many rows (4 bytes a logit read), by latency for a few.  Up to 512 candidates and k <= 32 a warp has a
-// row in registers and picks one after the other (two warp reductions each); beyond that a CTA has the row, and the k + 1
-// largest lie among the values above a bound that one warp finds from the threads' own maxima.
+// Bound by HBM for many rows (4 bytes a logit read), by latency for a few.  Up to 512 candidates and k < 32 a warp has a
+// row in registers, beyond that a CTA.  Either way the k + 1 largest lie among the values above a bound that at least k + 1 of
+// the threads' own maxima reach, found by bisection; what lies above it is ranked.
 #include "moc_common.cuh"
 
 namespace moc {
 namespace {
 
 constexpr float kMaskedLogit = -3.3895313892515355e38f;      // lowest finite bfloat16
-constexpr int kMostK = 128, kWarpMostK = 32, kWarpMostN = 512, kMostN = 16384, kMostGroups = 64;
+constexpr int kMostK = 128, kWarpMostK = 31, kWarpMostN = 512, kMostN = 16384, kMostGroups = 64;
 constexpr int kSelCand = 512;
 constexpr int kWarpRows = 4;                 // rows (warps) of a CTA
 // Keys order like the numbers (larger first), with what may not be chosen below: distinct, the lowest id on top.
@@ -38,7 +39,9 @@ struct SelectParams {
   int* load;                      // [C] or NULL
   long long ld;
   int rows, N, S, k, groups, keep, per;
+  FastDiv per_group;
   int sigmoid, top2, renorm;
+  int clear_load;                 // the launch is one CTA, which sets the counts to zero itself
   float rho;
 };
 
@@ -64,7 +67,6 @@ template <typename K> struct KeyOf;
 template <> struct KeyOf<float> { using type = uint32_t; };
 template <> struct KeyOf<double> { using type = uint64_t; };
 
-__device__ __forceinline__ uint32_t warp_most(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint64_t warp_most(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) { const uint64_t t = __shfl_xor_sync(0xffffffffu, v, o); v = t > v ? t : v; }
@@ -94,15 +96,24 @@ __device__ __forceinline__ typename KeyOf<K>::type candidate_key(const SelectPar
 }
 template <typename U> __device__ __forceinline__ bool chosen_from(U key) { return key > static_cast<U>(kFiller); }
 
-// How far fp32 keys can be off: the score's exponential (2 ulp), sums and quotient, against the largest score; the bias's addition.
-// Two of them are told apart beyond twice that.
-__device__ __forceinline__ float key_error(const SelectParams& p, float v, float total) {
-  return (p.sigmoid ? 1e-6f : 4e-6f / total) + 2.5e-7f * fabsf(v);
+// Fast keys of the first pass (softmax: `e` = exp(z - m) and 1 / total): -inf for what may not be chosen, NaN stays.
+__device__ __forceinline__ float fast_sigmoid(float z) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
 }
-__device__ __forceinline__ bool apart(const SelectParams& p, uint32_t above, uint32_t below, float total) {
-  if (!chosen_from(below) || !chosen_from(above)) return true;
-  const float a = of_key(above), b = of_key(below);
-  return a - b > key_error(p, a, total) + key_error(p, b, total);      // (NaN and infinities: not apart)
+
+// How far fast keys can be off.  Sigmoid: the exponential is off by 2 + 1.2 |z| ulp, which the slope s (1 - s) <= 1/4 brings
+// below 4e-8, the sum and the reciprocal by another 3 ulp of at most 1: 2.5e-7.  Softmax: 2 ulp of the exponential, |z - m| 2^-24 e^-|z - m| of its
+// argument, 2e-6 of the sum (terms off by up to 25 ulp each), all against the largest score 1 / total.  The bias's addition: half
+// an ulp of the key.  A sum of two keys adds theirs.
+__device__ __forceinline__ float key_error(const SelectParams& p, float v, float inv_total) {
+  return (p.sigmoid ? 3e-7f : 3e-6f * inv_total) + 6.1e-8f * fabsf(v);
+}
+// whether a > b for certain (NaN: no)
+__device__ __forceinline__ bool apart(const SelectParams& p, float a, float b, float inv_total) {
+  return a - b > key_error(p, a, inv_total) + key_error(p, b, inv_total);
 }
 
 // the two largest keys of a group
@@ -115,154 +126,171 @@ template <typename U> __device__ __forceinline__ U group_value(const SelectParam
   return p.top2 && chosen_from(t.a) && chosen_from(t.b) ? to_key(of_key(t.a) + of_key(t.b)) : t.a;
 }
 
-// One row's lists, by one warp; pick(j): candidate of the j-th place and whether it may be chosen at all.
-template <typename LT, typename Pick>
-__device__ __forceinline__ void write_row(const SelectParams& p, long long row, const LT* z, float m, float total, Pick pick) {
+// One row's lists, by one warp; pick(j, ok, z): candidate of the j-th place, whether it may be chosen at all, and its logit.
+template <int EACH, typename Pick>
+__device__ __forceinline__ void write_row(const SelectParams& p, long long row, float m, float total, Pick pick) {
   const int lane = threadIdx.x & 31;
-  constexpr int kEach = kMostK / 32;
-  int id[kEach];
-  float w[kEach], mass = 0.f;
+  int id[EACH];
+  float w[EACH], mass = 0.f;
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
+  for (int q = 0; q < EACH; ++q) {
     const int j = lane + 32 * q;
     id[q] = 0;
     w[q] = 0.f;
     if (j < p.k) {
       bool ok;
-      id[q] = pick(j, ok);
-      if (ok) w[q] = score_of<float>(p, logit_of(z, id[q]), m, total);
+      float z;
+      id[q] = pick(j, ok, z);
+      if (ok) w[q] = score_of<float>(p, z, m, total);
       mass += w[q];
+      if (p.load != nullptr) atomicAdd(p.load + p.S + id[q], 1);
     }
   }
   mass = warp_total(mass);
-  const float over = max_nan(mass, 1e-12f);
+  const float over = 1.f / max_nan(mass, 1e-12f);
   float sum = 0.f;
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
+  for (int q = 0; q < EACH; ++q) {
     const int j = lane + 32 * q;
     if (j >= p.k) break;
-    if (p.renorm) w[q] = w[q] / over;
+    if (p.renorm) w[q] *= over;
     sum += p.rho * w[q];
     p.idx[row * p.k + j] = id[q] + p.S;
     p.weights[row * p.k + j] = w[q];
-    if (p.load != nullptr) atomicAdd(p.load + p.S + id[q], 1);
   }
   sum = static_cast<float>(p.S) + warp_total(sum);
-  const float joint = max_nan(sum, 1e-12f);
+  const float joint = 1.f / max_nan(sum, 1e-12f);
   int* ci = p.comb_idx + row * (p.S + p.k);
   float* cw = p.comb_w + row * (p.S + p.k);
-  for (int j = lane; j < p.S; j += 32) { ci[j] = j; cw[j] = 1.f / joint; }
+  for (int j = lane; j < p.S; j += 32) { ci[j] = j; cw[j] = joint; }
 #pragma unroll
-  for (int q = 0; q < kEach; ++q) {
+  for (int q = 0; q < EACH; ++q) {
     const int j = lane + 32 * q;
     if (j >= p.k) break;
     ci[p.S + j] = id[q] + p.S;
-    cw[p.S + j] = p.S > 0 ? p.rho * w[q] / joint : w[q];
+    cw[p.S + j] = p.S > 0 ? p.rho * w[q] * joint : w[q];
   }
-  if (lane == 0) reinterpret_cast<float4*>(p.row_stats)[row] = make_float4(m, total, mass, sum);
+  if (lane == 0 && p.row_stats != nullptr) reinterpret_cast<float4*>(p.row_stats)[row] = make_float4(m, total, mass, sum);
+}
+
+// 64-bit sum of the exponentials of a row, by `threads` threads of which this is `t`; their parts are still to be added
+template <typename LT> __device__ __noinline__ double total64(const LT* z, int n, float m, int t, int threads) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int c = t; c < n; c += threads) {
+    const float v = logit_of(z, c);
+    if (!masked(v)) sum += exp(static_cast<double>(v) - static_cast<double>(m));
+  }
+  return sum;
+}
+template <typename LT> __device__ __noinline__ uint64_t key64(const SelectParams& p, const LT* z, int c, float m, double total, bool group) {
+  return candidate_key<double>(p, logit_of(z, c), c, m, total, group);
 }
 
 // ---- a warp a row ----------------------------------------------------------------------------
-// Lane j keeps the j-th pick.  Returns false where fp32 cannot tell neighbours apart.
-template <typename K, int NV>
-__device__ __forceinline__ bool choose_warp(const SelectParams& p, const float (&z)[NV], float m, K total, uint64_t* shared_keys,
-                                            int& pick, bool& ok) {
-  using U = typename KeyOf<K>::type;
-  constexpr bool kRough = sizeof(K) == 4;
+// The whole selection by 64-bit keys: lane j keeps the j-th pick.  `keys`: 64-bit words of this warp, N + N / 32.
+template <typename LT>
+__device__ __noinline__ void choose_warp64(const SelectParams& p, const LT* z, float m, uint64_t* keys, int& pick, bool& ok) {
   const int lane = threadIdx.x & 31;
-  U key[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = lane + 32 * i;
-    key[i] = c < p.N ? candidate_key<K>(p, z[i], c, m, total, false) : U(0);
-  }
+  double total = 1.0;
+  if (!p.sigmoid) total = warp_total(total64(z, p.N, m, lane, 32));
+  unsigned long long kept = ~0ull;
   if (p.keep < p.groups) {
-    U* sk = reinterpret_cast<U*>(shared_keys);           // candidate c at c + c / 32: groups of 32 columns start in different banks
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
-      if (c < p.N) sk[c + (c >> 5)] = p.bias == nullptr && p.top2 ? candidate_key<K>(p, z[i], c, m, total, true) : key[i];
-    }
+    for (int c = lane; c < p.N; c += 32) keys[c] = key64(p, z, c, m, total, true);
     __syncwarp();
-    // groups in rounds of 32; a group has as many lanes as fit
-    unsigned long long kept = 0;
-    U value[2];
+    uint64_t value[2] = {0, 0};
     int rank[2] = {0, 0};
-    const int lanes = p.groups > 16 ? 1 : p.groups > 8 ? 2 : p.groups > 4 ? 4 : p.groups > 2 ? 8 : 16;
-    const int sub = lane & (lanes - 1), rounds = (p.groups * lanes + 31) / 32;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int g = (lane + 32 * r) / lanes;
-      Best2<U> t{U(0), U(0)};
-      if (r < rounds) {
-        if (g < p.groups)
-          for (int c = g * p.per + sub; c < (g + 1) * p.per; c += lanes) take(t, sk[c + (c >> 5)]);
-        for (int o = lanes >> 1; o > 0; o >>= 1) {
-          const U a = __shfl_xor_sync(0xffffffffu, t.a, o), b = __shfl_xor_sync(0xffffffffu, t.b, o);
-          take(t, a);
-          take(t, b);
-        }
-      }
-      value[r] = r < rounds && g < p.groups ? group_value(p, t) : U(0);
+      const int g = lane + 32 * r;
+      if (g >= p.groups) continue;
+      Best2<uint64_t> t{0, 0};
+      for (int c = g * p.per; c < (g + 1) * p.per; ++c) take(t, keys[c]);
+      value[r] = group_value(p, t);
     }
     for (int g = 0; g < p.groups; ++g) {
-      const U other = __shfl_sync(0xffffffffu, value[(g * lanes) >> 5 & 1], (g * lanes) & 31);
+      const uint64_t other = __shfl_sync(0xffffffffu, value[g >> 5], g & 31);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int mine = (lane + 32 * r) / lanes;
-        rank[r] += other > value[r] || (other == value[r] && g < mine);
-      }
+      for (int r = 0; r < 2; ++r) rank[r] += other > value[r] || (other == value[r] && g < lane + 32 * r);
     }
-    U least = ~U(0), most = 0;           // of those that stay and of those that go
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int g = (lane + 32 * r) / lanes;
-      if (r >= rounds || g >= p.groups) continue;
-      if (rank[r] < p.keep) { kept |= 1ull << g; least = min(least, value[r]); }
-      else most = max(most, value[r]);
-    }
-    kept = static_cast<unsigned long long>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(kept >> 32))) << 32 |
-           __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(kept));
-    if constexpr (kRough) {
-      least = __reduce_min_sync(0xffffffffu, least);
-      most = __reduce_max_sync(0xffffffffu, most);
-      if ((p.bias != nullptr || p.top2) && !apart(p, least, most, total)) return false;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
-      if (c < p.N && !(kept >> (c / p.per) & 1)) key[i] = static_cast<U>(kFiller - c);
-    }
+    const uint32_t lo = __ballot_sync(0xffffffffu, lane < p.groups && rank[0] < p.keep);
+    const uint32_t hi = __ballot_sync(0xffffffffu, lane + 32 < p.groups && rank[1] < p.keep);
+    kept = static_cast<unsigned long long>(hi) << 32 | lo;
   }
-  U best = 0;
+  __syncwarp();
+  for (int c = lane; c < p.N; c += 32)
+    keys[c] = kept >> div_of(c, p.per_group) & 1 ? key64(p, z, c, m, total, false) : static_cast<uint64_t>(kFiller - c);
+  __syncwarp();
+  uint64_t best = 0;
   int at = 0;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
-  const bool check = kRough && p.bias != nullptr;
-  const int steps = check && p.k < p.N ? p.k + 1 : p.k;
-  U before = 0;
-  bool sure = true;
-  for (int t = 0; t < steps; ++t) {
-    const U top = warp_most(best);
+  for (int c = lane; c < p.N; c += 32)
+    if (keys[c] > best) { best = keys[c]; at = c; }
+  for (int t = 0; t < p.k; ++t) {
+    const uint64_t top = warp_most(best);
     const int id = static_cast<int>(__reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at) : 0xFFFFFFFFu));
     if (lane == t) { pick = id; ok = chosen_from(top); }
-    if constexpr (kRough) {
-      if (check && t > 0 && !apart(p, before, top, total)) { sure = false; break; }
-    }
-    before = top;
-    if (best == top && at == id) {
+    if (best == top && at == id) {              // (only this lane's own columns)
+      keys[id] = 0;
       best = 0;
-      at = 0;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (lane + 32 * i == id) key[i] = 0;
-        if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
-      }
+      for (int c = lane; c < p.N; c += 32)
+        if (keys[c] > best) { best = keys[c]; at = c; }
     }
   }
-  return sure;
+}
+
+// The groups that stay (bit g), from keys in shared memory (candidate c at c + c / 32), by R groups a lane (2: of more than 32) or
+// 1 / lanes of one; false: fp32 cannot tell.
+template <int R>
+__device__ __forceinline__ bool choose_groups_warp(const SelectParams& p, const float* sk, float inv_total, unsigned long long& kept) {
+  const int lane = threadIdx.x & 31;
+  const int shift = R > 1 || p.groups > 16 ? 0 : p.groups > 8 ? 1 : p.groups > 4 ? 2 : p.groups > 2 ? 3 : 4;     // log2 of a group's lanes
+  const int lanes = 1 << shift, sub = lane & (lanes - 1);
+  float value[R];
+  int rank[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int g = (lane >> shift) + 32 * r;
+    float a = -INFINITY, b = -INFINITY;
+    if (g < p.groups)
+      for (int c = g * p.per + sub; c < (g + 1) * p.per; c += lanes) {
+        const float v = sk[c + (c >> 5)];
+        b = fmaxf(b, fminf(a, v));
+        a = fmaxf(a, v);
+      }
+    for (int o = lanes >> 1; o > 0; o >>= 1) {
+      const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+      a = fmaxf(a, oa);
+    }
+    value[r] = p.top2 && b > -INFINITY ? a + b : a;
+    rank[r] = 0;
+  }
+  for (int g = 0; g < p.groups; ++g) {
+    const float other = __shfl_sync(0xffffffffu, R > 1 && g >= 32 ? value[R - 1] : value[0], (g << shift) & 31);
+#pragma unroll
+    for (int r = 0; r < R; ++r) rank[r] += other > value[r] || (other == value[r] && g < (lane >> shift) + 32 * r);
+  }
+  float least = INFINITY, most = -INFINITY;            // of those that stay, of those that go
+  uint32_t mask[2] = {0, 0};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int g = (lane >> shift) + 32 * r;
+    if (g >= p.groups) continue;
+    if (rank[r] < p.keep) {
+      mask[r] |= 1u << (g & 31);
+      least = fminf(least, value[r]);
+    } else {
+      most = fmaxf(most, value[r]);
+    }
+  }
+  kept = __reduce_or_sync(0xffffffffu, mask[0]);
+  if constexpr (R > 1) kept |= static_cast<unsigned long long>(__reduce_or_sync(0xffffffffu, mask[1])) << 32;
+  if (p.bias == nullptr && !p.top2) return true;
+  least = of_key(__reduce_min_sync(0xffffffffu, to_key(least)));
+  most = of_key(__reduce_max_sync(0xffffffffu, to_key(most)));
+  // (two keys each; groups without a candidate are all behind those with one, in the order of their ids)
+  return least - most > 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total)) || (least == -INFINITY && most == -INFINITY);
 }
 
 template <typename LT, int NV>
@@ -271,41 +299,187 @@ select_warp_kernel(const SelectParams p) {
   __shared__ uint64_t keys[kWarpRows][NV * 33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * kWarpRows + warp;
+  if (p.clear_load) {
+    for (int c = threadIdx.x; c < p.S + p.N; c += 32 * kWarpRows) p.load[c] = 0;
+    __syncthreads();
+  }
   if (row >= p.rows) return;
   const LT* zr = static_cast<const LT*>(p.logits) + row * p.ld + p.S;
-  float z[NV];
+  float z[NV], v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) z[i] = lane + 32 * i < p.N ? logit_of(zr, lane + 32 * i) : -INFINITY;
-  float m = 0.f, total = 1.f;
-  if (!p.sigmoid) {
+  if (p.bias != nullptr) {
+    const float* b = p.bias + p.S;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = lane + 32 * i < p.N ? b[lane + 32 * i] : 0.f;
+  }
+  float m = 0.f, total = 1.f, inv_total = 1.f;
+  const bool judged = p.keep < p.groups && p.top2 && p.bias == nullptr;      // groups by scores, picks by logits
+  float* sk = reinterpret_cast<float*>(keys[warp]);
+  if (p.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float sc = p.bias != nullptr || judged ? fast_sigmoid(z[i]) : 0.f;
+      if (judged) sk[lane + 33 * i] = masked(z[i]) ? -INFINITY : sc;
+      v[i] = masked(z[i]) ? -INFINITY : p.bias != nullptr ? sc + v[i] : z[i];
+    }
+  } else {
     m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; ++i) m = fmaxf(m, z[i]);
-    m = warp_max(m);
+    m = of_key(__reduce_max_sync(0xffffffffu, to_key(m)));
+    float e[NV];
     total = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) total += masked(z[i]) ? 0.f : expf(z[i] - m);
+    for (int i = 0; i < NV; ++i) { e[i] = masked(z[i]) ? 0.f : expf(z[i] - m); total += e[i]; }
     total = warp_total(total);
     if (total == 0.f) total = 1.f;                  // (every logit masked)
+    inv_total = 1.f / total;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (judged) sk[lane + 33 * i] = masked(z[i]) ? -INFINITY : e[i] * inv_total;
+      v[i] = masked(z[i]) ? -INFINITY : p.bias != nullptr ? e[i] * inv_total + v[i] : z[i];
+    }
   }
+  bool sure = true;
+  if (p.keep < p.groups) {
+    if (!judged) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) sk[lane + 33 * i] = v[i];
+    }
+    __syncwarp();
+    unsigned long long kept;
+    if (p.groups <= 32) {
+      sure = choose_groups_warp<1>(p, sk, inv_total, kept);
+      const uint32_t k32 = static_cast<uint32_t>(kept);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (!(k32 >> (div_of(lane + 32 * i, p.per_group) & 31) & 1)) v[i] += -INFINITY;        // (NaN stays)
+    } else {
+      sure = choose_groups_warp<2>(p, sk, inv_total, kept);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (!(kept >> (div_of(lane + 32 * i, p.per_group) & 63) & 1)) v[i] += -INFINITY;
+    }
+    __syncwarp();
+  }
+  // lane j keeps the j-th pick
   int pick = 0;
   bool ok = false;
-  if (!choose_warp<float, NV>(p, z, m, total, keys[warp], pick, ok)) {
-    double t64 = 1.0;
-    if (!p.sigmoid) {
-      t64 = 0.0;
-#pragma unroll 1
-      for (int c = lane; c < p.N; c += 32) {
-        const float v = logit_of(zr, c);
-        if (!masked(v)) t64 += exp(static_cast<double>(v) - static_cast<double>(m));
+  float chosen = 0.f;              // its logit
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) best = max_nan(best, v[i]);
+  const uint32_t mine = to_key(best), none = 0x007FFFFFu;          // (the key of -inf)
+  uint32_t hi = __reduce_max_sync(0xffffffffu, mine);
+  const int some = __popc(__ballot_sync(0xffffffffu, mine > none));
+  const int need = min(p.k + 1, p.N);
+  if (some == 0) {                                           // nothing to choose from: the lowest ids
+    pick = lane;
+  } else if (hi == 0xFFFFFFFFu || some < need) {             // NaN, or candidates in too few lanes
+    sure = false;
+  } else if (sure) {
+    // count(lanes >= lo) >= need, count(> hi) == 0
+    uint32_t lo = __reduce_min_sync(0xffffffffu, mine > none ? mine : 0xFFFFFFFFu);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      const int n = __popc(__ballot_sync(0xffffffffu, mine >= mid));
+      if (n >= need) {
+        lo = mid;
+        if (n <= need + 2) break;
+      } else {
+        hi = mid - 1;
       }
-      t64 = warp_total(t64);
     }
-    choose_warp<double, NV>(p, z, m, t64, keys[warp], pick, ok);
+    hi = 0xFF7FFFFFu;                                        // (the largest finite number's key)
+    float edge;
+    int n;
+    while (true) {
+      edge = of_key(lo);
+      if (p.bias != nullptr) edge -= 2.f * key_error(p, edge, inv_total);        // what may yet turn out to reach the bound
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) count += v[i] >= edge;
+      n = __reduce_add_sync(0xffffffffu, count);
+      if (n <= 32) break;
+      // too many for a candidate a lane: a higher bound that at least `need` values reach
+      int above = 0;
+      uint32_t mid = lo;
+      while (lo < hi) {
+        mid = lo + (hi - lo + 1) / 2;
+        const float bound = of_key(mid);
+        count = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) count += v[i] >= bound;
+        above = __reduce_add_sync(0xffffffffu, count);
+        if (above >= need) break;
+        hi = mid - 1;
+      }
+      if (lo >= hi) break;
+      lo = mid;
+    }
+    sure = n <= 32 && n >= need && edge < INFINITY;          // (equal keys, or infinite ones)
+    if (sure) {
+      // a candidate a lane: id and key through shared memory
+      uint32_t* out = reinterpret_cast<uint32_t*>(keys[warp]);
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const bool in = v[i] >= edge;
+        const uint32_t votes = __ballot_sync(0xffffffffu, in);
+        if (in) {
+          const int pos = at + __popc(votes & ((1u << lane) - 1u));
+          out[pos] = lane + 32 * i;
+          out[32 + pos] = __float_as_uint(v[i]);
+          out[64 + pos] = __float_as_uint(z[i]);
+        }
+        at += __popc(votes);
+      }
+      __syncwarp();
+      const int id = lane < n ? static_cast<int>(out[lane]) : 0x7FFFFFFF;
+      const float key = lane < n ? __uint_as_float(out[32 + lane]) : -INFINITY, logit = lane < n ? __uint_as_float(out[64 + lane]) : 0.f;
+      int rank = 0;
+      bool close = false;
+      // (candidates came in the order of their ids within a slot only)
+      for (int j = 0; j < n; ++j) {
+        const float other = __shfl_sync(0xffffffffu, key, j);
+        const int oid = __shfl_sync(0xffffffffu, id, j);
+        rank += other > key || (other == key && oid < id);
+        if (p.bias != nullptr) close |= j != lane && lane < n && !apart(p, fmaxf(other, key), fminf(other, key), inv_total);
+      }
+      if (__any_sync(0xffffffffu, close)) {
+        // again by 64-bit keys: all other candidates are certainly behind the first k of these
+        double t64 = 1.0;
+        if (!p.sigmoid) t64 = warp_total(total64(zr, p.N, m, lane, 32));
+        const uint64_t wide = lane < n ? key64(p, zr, id, m, t64, false) : 0;
+        rank = 0;
+        for (int j = 0; j < n; ++j) {
+          const uint64_t other = __shfl_sync(0xffffffffu, wide, j);
+          const int oid = __shfl_sync(0xffffffffu, id, j);
+          rank += other > wide || (other == wide && oid < id);
+        }
+      }
+      __syncwarp();
+      if (lane < n) {
+        out[rank] = id;
+        out[32 + rank] = __float_as_uint(logit);
+      }
+      __syncwarp();
+      if (lane < n) {
+        pick = out[lane];
+        chosen = __uint_as_float(out[32 + lane]);
+        ok = true;
+      }
+    }
   }
-  const unsigned live = __ballot_sync(0xffffffffu, ok);
-  write_row(p, row, zr, m, total, [&](int j, bool& good) {      // (k <= 32: place j is this lane's)
-    good = live >> (j & 31) & 1;
+  if (!sure) {
+    ok = false;
+    choose_warp64(p, zr, m, keys[warp], pick, ok);
+    chosen = lane < p.k ? logit_of(zr, pick) : 0.f;
+  }
+  write_row<1>(p, row, m, total, [&](int, bool& good, float& logit) {      // (k <= 32: place j is this lane's)
+    good = ok;
+    logit = chosen;
     return pick;
   });
 }
@@ -327,21 +501,20 @@ struct CtaShared {
   unsigned long long kept;
   double red[32];
   uint64_t most[32];
-  int count, unsure;
-  uint32_t edge;
+  int count, unsure, close;
+  float edge;
 };
 
-// Which groups stay; keys of all candidates in shared memory.  false: fp32 cannot tell.
-template <typename K, int TH>
-__device__ __forceinline__ bool choose_groups(const SelectParams& p, CtaShared& s, const typename KeyOf<K>::type* keys, float total) {
-  using U = typename KeyOf<K>::type;
+// The groups that stay, from 64-bit keys of all candidates in shared memory.
+template <int TH>
+__device__ __noinline__ void choose_groups64(const SelectParams& p, CtaShared& s, const uint64_t* keys) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int g = warp; g < p.groups; g += TH / 32) {
-    Best2<U> t{U(0), U(0)};
+    Best2<uint64_t> t{0, 0};
     for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32) take(t, keys[c]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      const U a = __shfl_xor_sync(0xffffffffu, t.a, o), b = __shfl_xor_sync(0xffffffffu, t.b, o);
+      const uint64_t a = __shfl_xor_sync(0xffffffffu, t.a, o), b = __shfl_xor_sync(0xffffffffu, t.b, o);
       take(t, a);
       take(t, b);
     }
@@ -349,36 +522,79 @@ __device__ __forceinline__ bool choose_groups(const SelectParams& p, CtaShared& 
   }
   __syncthreads();
   if (warp == 0) {
-    unsigned long long kept = 0;
-    U least = ~U(0), most = 0;
+    uint32_t lo = 0, hi = 0;
     for (int g = lane; g < p.groups; g += 32) {
-      const U mine = static_cast<U>(s.group[g]);
+      const uint64_t mine = s.group[g];
       int rank = 0;
-      for (int o = 0; o < p.groups; ++o) {
-        const U other = static_cast<U>(s.group[o]);
-        rank += other > mine || (other == mine && o < g);
-      }
-      if (rank < p.keep) { kept |= 1ull << g; least = min(least, mine); }
-      else most = max(most, mine);
+      for (int o = 0; o < p.groups; ++o) rank += s.group[o] > mine || (s.group[o] == mine && o < g);
+      if (rank < p.keep) { if (g < 32) lo |= 1u << g; else hi |= 1u << (g - 32); }
     }
-    kept = static_cast<unsigned long long>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(kept >> 32))) << 32 |
-           __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(kept));
-    bool sure = true;
-    if constexpr (sizeof(K) == 4) {
-      least = __reduce_min_sync(0xffffffffu, least);
-      most = __reduce_max_sync(0xffffffffu, most);
-      sure = !(p.bias != nullptr || p.top2) || apart(p, least, most, total);
-    }
-    if (lane == 0) { s.kept = kept; s.unsure = !sure; }
+    lo = __reduce_or_sync(0xffffffffu, lo);
+    hi = __reduce_or_sync(0xffffffffu, hi);
+    if (lane == 0) s.kept = static_cast<unsigned long long>(hi) << 32 | lo;
   }
   __syncthreads();
-  return !s.unsure;
+}
+// The same from fp32 keys; s.unsure where they cannot tell.
+template <int TH>
+__device__ __forceinline__ void choose_groups(const SelectParams& p, CtaShared& s, const float* keys, float inv_total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* values = reinterpret_cast<float*>(s.group);
+  for (int g = warp; g < p.groups; g += TH / 32) {
+    float a = -INFINITY, b = -INFINITY;
+#pragma unroll 4
+    for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32) {
+      const float v = keys[c];
+      b = fmaxf(b, fminf(a, v));
+      a = fmaxf(a, v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+      b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+      a = fmaxf(a, oa);
+    }
+    if (lane == 0) values[g] = p.top2 && b > -INFINITY ? a + b : a;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    float least = INFINITY, most = -INFINITY;
+    for (int g = lane; g < p.groups; g += 32) {
+      const float mine = values[g];
+      int rank = 0;
+      for (int o = 0; o < p.groups; ++o) rank += values[o] > mine || (values[o] == mine && o < g);
+      values[kMostGroups + g] = rank < p.keep ? 0.f : -INFINITY;
+      if (rank < p.keep) least = fminf(least, mine);
+      else most = fmaxf(most, mine);
+    }
+    least = of_key(__reduce_min_sync(0xffffffffu, to_key(least)));
+    most = of_key(__reduce_max_sync(0xffffffffu, to_key(most)));
+    const bool sure = (p.bias == nullptr && !p.top2) || (least == -INFINITY && most == -INFINITY) ||
+                      least - most > 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total));
+    if (lane == 0 && !sure) s.unsure = 1;
+  }
+  __syncthreads();
 }
 
-// The picks one after the other from 64-bit keys in shared memory: any row, at the cost of two barriers a pick.
-template <int TH>
-__device__ __forceinline__ void choose_slowly(const SelectParams& p, CtaShared& s, uint64_t* keys) {
+// The whole selection by 64-bit keys in shared memory: any row, at the cost of two barriers a pick.
+template <typename LT, int TH>
+__device__ __noinline__ void choose_cta64(const SelectParams& p, CtaShared& s, uint64_t* keys, const LT* zr, float m) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double total = 1.0;
+  if (!p.sigmoid) total = cta_total<double, TH>(total64(zr, p.N, m, threadIdx.x, TH), s.red);
+  __syncthreads();
+  unsigned long long kept = ~0ull;
+  if (p.keep < p.groups) {
+#pragma unroll 1
+    for (int c = threadIdx.x; c < p.N; c += TH) keys[c] = key64(p, zr, c, m, total, true);
+    __syncthreads();
+    choose_groups64<TH>(p, s, keys);
+    kept = s.kept;
+  }
+#pragma unroll 1
+  for (int c = threadIdx.x; c < p.N; c += TH)
+    keys[c] = kept >> (div_of(c, p.per_group) & 63) & 1 ? key64(p, zr, c, m, total, false) : static_cast<uint64_t>(kFiller - c);
+  // (a thread reads and clears its own columns alone)
   uint64_t best = 0;
   int at = 0;
   for (int c = threadIdx.x; c < p.N; c += TH)
@@ -407,85 +623,112 @@ __device__ __forceinline__ void choose_slowly(const SelectParams& p, CtaShared& 
 }
 
 template <typename LT, int NV, int TH>
-__global__ void __launch_bounds__(TH)
+__global__ void __launch_bounds__(TH, TH == 256 ? 5 : 1)
 select_cta_kernel(const SelectParams p) {
-  extern __shared__ uint64_t keys[];       // [N]: 64-bit keys of an unsure row, or 32-bit keys for the groups
+  extern __shared__ uint64_t keys[];       // [N]: 64-bit keys of an unsure row, or fp32 keys for the groups
   __shared__ CtaShared s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.x;
+  if (p.clear_load)                        // (many barriers before the first count)
+    for (int c = threadIdx.x; c < p.S + p.N; c += TH) p.load[c] = 0;
   const LT* zr = static_cast<const LT*>(p.logits) + row * p.ld + p.S;
-  float z[NV];
+  const bool biased = p.bias != nullptr, grouped = p.keep < p.groups, judged = grouped && p.top2 && !biased;
+  const float* b = biased ? p.bias + p.S : nullptr;
+  float* sk = reinterpret_cast<float*>(keys);
+  float v[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) z[i] = threadIdx.x + TH * i < p.N ? logit_of(zr, threadIdx.x + TH * i) : -INFINITY;
-  float m = 0.f, total = 1.f;
-  if (!p.sigmoid) {
-    m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) m = fmaxf(m, z[i]);
-    m = warp_max(m);
-    float* red = reinterpret_cast<float*>(s.most);
-    if (lane == 0) red[warp] = m;
-    __syncthreads();
-    m = warp_max(red[lane < TH / 32 ? lane : 0]);
-    total = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) total += masked(z[i]) ? 0.f : expf(z[i] - m);
-    total = cta_total<float, TH>(total, reinterpret_cast<float*>(s.red));
-    if (total == 0.f) total = 1.f;
-  }
-  const bool exact = p.bias == nullptr;
-  bool sure = true;
-  uint32_t key[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = threadIdx.x + TH * i;
-    key[i] = c < p.N ? candidate_key<float>(p, z[i], c, m, total, false) : 0u;
-  }
-  if (p.keep < p.groups) {
-    uint32_t* k32 = reinterpret_cast<uint32_t*>(keys);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = threadIdx.x + TH * i;
-      if (c < p.N) k32[c] = exact && p.top2 ? candidate_key<float>(p, z[i], c, m, total, true) : key[i];
-    }
-    __syncthreads();
-    sure = choose_groups<float, TH>(p, s, k32, total);
-    const unsigned long long kept = s.kept;
-    if (sure) {
+  for (int i = 0; i < NV; ++i) v[i] = threadIdx.x + TH * i < p.N ? logit_of(zr, threadIdx.x + TH * i) : -INFINITY;
+  if (threadIdx.x == 0) { s.count = 0; s.unsure = 0; s.close = 0; }
+  float m = 0.f, total = 1.f, inv_total = 1.f;
+  if (p.sigmoid) {
+    if (biased || judged) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = threadIdx.x + TH * i;
-        if (c < p.N && !(kept >> (c / p.per) & 1)) key[i] = kFiller - c;
+        const float sc = masked(v[i]) ? -INFINITY : fast_sigmoid(v[i]);
+        if (judged && c < p.N) sk[c] = sc;
+        if (biased && c < p.N) v[i] = sc + b[c];
       }
     }
-  }
-  if (sure) {
-    // A bound that at least k + 1 of the threads' own maxima reach (all of them where there are no more candidates), and few more.
-    uint32_t* tops = reinterpret_cast<uint32_t*>(s.cand);          // [TH] <= kSelCand * 2
-    uint32_t top = 0;
+  } else {
+    m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) top = max(top, key[i]);
-    tops[threadIdx.x] = top;
-    if (threadIdx.x == 0) { s.count = 0; s.unsure = 0; }
+    for (int i = 0; i < NV; ++i) m = fmaxf(m, v[i]);
+    m = of_key(__reduce_max_sync(0xffffffffu, to_key(m)));
+    float* red = reinterpret_cast<float*>(s.most);
+    if (lane == 0) red[warp] = m;
     __syncthreads();
-    const int need = min(p.k + 1, min(p.N, TH));
-    if (warp == 0) {
-      uint32_t v[TH / 32];
-      uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    m = of_key(__reduce_max_sync(0xffffffffu, to_key(red[lane < TH / 32 ? lane : 0])));
+    total = 0.f;
+    if (biased || judged) {                    // the exponentials become the keys
+      float e[NV];
 #pragma unroll
-      for (int i = 0; i < TH / 32; ++i) {
-        v[i] = tops[lane + 32 * i];
-        hi = max(hi, v[i]);
-        lo = min(lo, v[i]);
+      for (int i = 0; i < NV; ++i) { e[i] = masked(v[i]) ? 0.f : expf(v[i] - m); total += e[i]; }
+      total = cta_total<float, TH>(total, reinterpret_cast<float*>(s.red));
+      if (total == 0.f) total = 1.f;
+      inv_total = 1.f / total;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = threadIdx.x + TH * i;
+        const float sc = masked(v[i]) ? -INFINITY : e[i] * inv_total;
+        if (judged && c < p.N) sk[c] = sc;
+        if (biased && c < p.N) v[i] = sc + b[c];
       }
-      hi = __reduce_max_sync(0xffffffffu, hi);
-      lo = __reduce_min_sync(0xffffffffu, lo);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) total += masked(v[i]) ? 0.f : expf(v[i] - m);
+      total = cta_total<float, TH>(total, reinterpret_cast<float*>(s.red));
+      if (total == 0.f) total = 1.f;
+      inv_total = 1.f / total;
+    }
+  }
+  if (!biased) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = masked(v[i]) ? -INFINITY : v[i];
+  }
+  if (grouped) {
+    if (!judged) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (threadIdx.x + TH * i < p.N) sk[threadIdx.x + TH * i] = v[i];
+    }
+    __syncthreads();
+    choose_groups<TH>(p, s, sk, inv_total);
+    const float* off = reinterpret_cast<const float*>(s.group) + kMostGroups;          // 0 where the group stays, else -inf
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] += off[min(div_of(threadIdx.x + TH * i, p.per_group), kMostGroups - 1)];     // (NaN stays)
+  }
+  // A bound that at least k + 1 of the threads' own maxima reach, and few more.
+  float* tops = reinterpret_cast<float*>(s.cand);          // [TH] <= kSelCand * 2
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) top = max_nan(top, v[i]);
+  tops[threadIdx.x] = top;
+  __syncthreads();
+  const int need = min(p.k + 1, p.N);
+  if (warp == 0) {
+    uint32_t key[TH / 32], lo = 0xFFFFFFFFu, hi = 0;
+    constexpr uint32_t kNone = 0x007FFFFFu;                // of -inf
+    int some = 0;
+#pragma unroll
+    for (int i = 0; i < TH / 32; ++i) {
+      key[i] = to_key(tops[lane + 32 * i]);
+      hi = max(hi, key[i]);
+      if (key[i] > kNone) { ++some; lo = min(lo, key[i]); }
+    }
+    some = __reduce_add_sync(0xffffffffu, some);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    // NaN, or candidates in too few threads, unless there is none at all: not for this bound
+    if (hi == 0xFFFFFFFFu || (some < need && some > 0)) {
+      if (lane == 0) s.unsure = 1;
+    } else if (some > 0) {
       // count(>= lo) >= need, count(> hi) == 0
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < TH / 32; ++i) n += v[i] >= mid;
+        for (int i = 0; i < TH / 32; ++i) n += key[i] >= mid;
         n = __reduce_add_sync(0xffffffffu, n);
         if (n >= need) {
           lo = mid;
@@ -494,20 +737,26 @@ select_cta_kernel(const SelectParams p) {
           hi = mid - 1;
         }
       }
-      if (lo == 0) lo = 1;                                    // (threads without a candidate)
-      if (!exact && chosen_from(lo)) {                        // what may yet turn out to reach the bound
-        const float e = of_key(lo);
-        lo = min(lo, to_key(e - 2.f * key_error(p, e, total)));
-      }
-      if (lane == 0) s.edge = lo;
     }
-    __syncthreads();
-    const uint32_t edge = s.edge;
+    // (with a bias: what may yet turn out to reach the bound)
+    const float e = some > 0 ? of_key(lo) : INFINITY;
+    if (lane == 0) {
+      s.edge = biased && some > 0 ? e - 2.f * key_error(p, e, inv_total) : e;
+      if (some > 0 && !(s.edge < INFINITY)) s.unsure = 1;          // (more infinite keys than places)
+    }
+    if (some == 0)
+      for (int j = lane; j < p.k; j += 32) s.place[j] = ~j;        // nothing to choose from: the lowest ids
+  }
+  __syncthreads();
+  const float edge = s.edge;
+  bool sure = !s.unsure;
+  if (sure && edge < INFINITY) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (key[i] >= edge) {
+      if (v[i] >= edge) {
         const int pos = atomicAdd(&s.count, 1);
-        if (pos < kSelCand) s.cand[pos] = static_cast<unsigned long long>(key[i]) << 32 | ~static_cast<uint32_t>(threadIdx.x + TH * i);
+        if (pos < kSelCand)
+          s.cand[pos] = static_cast<unsigned long long>(to_key(v[i])) << 32 | ~static_cast<uint32_t>(threadIdx.x + TH * i);
       }
     }
     __syncthreads();
@@ -518,51 +767,45 @@ select_cta_kernel(const SelectParams p) {
         const unsigned long long mine = s.cand[t];
         unsigned long long next = 0;                // the largest below it
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) {
           const unsigned long long o = s.cand[j];
           rank += o > mine;
-          if (o < mine && o > next) next = o;
+          if (biased && o < mine && o > next) next = o;
         }
         if (rank < p.k) {
-          const uint32_t k32 = static_cast<uint32_t>(mine >> 32);
-          const int id = static_cast<int>(~static_cast<uint32_t>(mine));
-          s.place[rank] = chosen_from(k32) ? id : ~id;
-          if (!exact && next != 0 && !apart(p, k32, static_cast<uint32_t>(next >> 32), total)) s.unsure = 1;
+          s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
+          if (next != 0 && !apart(p, of_key(static_cast<uint32_t>(mine >> 32)), of_key(static_cast<uint32_t>(next >> 32)), inv_total))
+            s.close = 1;
         }
       }
       __syncthreads();
-      sure = !s.unsure;
+      if (s.close) {                                // the candidates again by 64-bit keys
+        double t64 = 1.0;
+        if (!p.sigmoid) t64 = cta_total<double, TH>(total64(zr, p.N, m, threadIdx.x, TH), s.red);
+        for (int t = threadIdx.x; t < n; t += TH) keys[t] = key64(p, zr, static_cast<int>(~static_cast<uint32_t>(s.cand[t])), m, t64, false);
+        __syncthreads();
+        for (int t = threadIdx.x; t < n; t += TH) {
+          const uint64_t mine = keys[t];
+          const uint32_t id = ~static_cast<uint32_t>(s.cand[t]);
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += keys[j] > mine || (keys[j] == mine && ~static_cast<uint32_t>(s.cand[j]) < id);
+          if (rank < p.k) s.place[rank] = static_cast<int>(id);
+        }
+        __syncthreads();
+      }
     }
   }
   if (!sure) {                       // (the same for every thread)
-    double t64 = 1.0;
-    if (!p.sigmoid) {
-      t64 = 0.0;
-#pragma unroll 1
-      for (int c = threadIdx.x; c < p.N; c += TH) {
-        const float v = logit_of(zr, c);
-        if (!masked(v)) t64 += exp(static_cast<double>(v) - static_cast<double>(m));
-      }
-      t64 = cta_total<double, TH>(t64, s.red);
-    }
     __syncthreads();
-#pragma unroll 1
-    for (int pass = p.keep < p.groups ? 0 : 1; pass < 2; ++pass) {
-#pragma unroll 1
-      for (int c = threadIdx.x; c < p.N; c += TH) {
-        const bool out = pass == 1 && p.keep < p.groups && !(s.kept >> (c / p.per) & 1);
-        keys[c] = out ? kFiller - c : candidate_key<double>(p, logit_of(zr, c), c, m, t64, pass == 0);
-      }
-      __syncthreads();
-      if (pass == 0) choose_groups<double, TH>(p, s, keys, total);
-    }
-    choose_slowly<TH>(p, s, keys);
+    choose_cta64<LT, TH>(p, s, keys, zr, m);
   }
   if (warp == 0) {
-    write_row(p, row, zr, m, total, [&](int j, bool& good) {
-      const int v = s.place[j];
-      good = v >= 0;
-      return v >= 0 ? v : ~v;
+    write_row<kMostK / 32>(p, row, m, total, [&](int j, bool& good, float& logit) {
+      const int at = s.place[j], id = at >= 0 ? at : ~at;
+      good = at >= 0;
+      logit = logit_of(zr, id);
+      return id;
     });
   }
 }
@@ -692,7 +935,7 @@ template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream
     const bool big = p.N > 4096;
     auto kern = p.N <= 1024 ? select_cta_kernel<LT, 4, 256> : p.N <= 2048 ? select_cta_kernel<LT, 8, 256>
                 : !big ? select_cta_kernel<LT, 16, 256> : p.N <= 8192 ? select_cta_kernel<LT, 8, 1024> : select_cta_kernel<LT, 16, 1024>;
-    MOC_CUDA_OK(allow_shared(kern, static_cast<size_t>(p.N) * 8, kMostN * 8));
+    if (p.N > 4096) MOC_CUDA_OK(allow_shared(kern, static_cast<size_t>(p.N) * 8, kMostN * 8));      // (48 KB need no leave)
     kern<<<p.rows, big ? 1024 : 256, static_cast<size_t>(p.N) * 8, stream>>>(p);
   }
   MOC_CUDA_OK(cudaGetLastError());
@@ -715,7 +958,7 @@ extern "C" int moc_select_fwd(const moc_select_shape* s, const void* logits, con
                               int32_t* comb_idx, float* comb_w, float* row_stats, int32_t* load, void* stream_) {
   const int rc = check(s);
   if (rc != MOC_OK) return rc;
-  MOC_REQUIRE(logits && idx && weights && comb_idx && comb_w && row_stats, "NULL selection buffer");
+  MOC_REQUIRE(logits && idx && weights && comb_idx && comb_w, "NULL selection buffer");
   MOC_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 15) == 0, "row_stats must be 16-byte aligned");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   SelectParams p{};
@@ -723,8 +966,11 @@ extern "C" int moc_select_fwd(const moc_select_shape* s, const void* logits, con
   p.comb_idx = comb_idx; p.comb_w = comb_w; p.row_stats = row_stats; p.load = load; p.ld = s->ld;
   p.rows = s->rows; p.N = s->num_chapters - s->num_shared; p.S = s->num_shared; p.k = s->top_k;
   p.groups = s->num_groups; p.keep = s->top_groups; p.per = p.N / p.groups;
+  p.per_group = fast_div(p.per);
   p.sigmoid = s->score == MOC_SCORE_SIGMOID; p.top2 = s->group_top2 != 0; p.renorm = s->renormalize != 0; p.rho = s->routed_scale;
-  if (load != nullptr) MOC_CUDA_OK(cudaMemsetAsync(load, 0, static_cast<size_t>(s->num_chapters) * sizeof(int32_t), stream));
+  const bool warps = p.N <= kWarpMostN && p.k <= kWarpMostK;
+  p.clear_load = load != nullptr && p.rows <= (warps ? kWarpRows : 1);
+  if (load != nullptr && !p.clear_load) MOC_CUDA_OK(cudaMemsetAsync(load, 0, static_cast<size_t>(s->num_chapters) * sizeof(int32_t), stream));
   return s->dtype == MOC_F32 ? select_fwd<float>(p, stream) : select_fwd<__nv_bfloat16>(p, stream);
 }
 

@@ -14,9 +14,11 @@ Three differentiable pieces mirror the reference's sequence-level memory layer
 from __future__ import annotations
 
 import os
+from functools import lru_cache
 from typing import Dict, NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import ops
@@ -943,14 +945,20 @@ class ChapterSelection(NamedTuple):
     load: torch.Tensor
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether autograd has to see a call on these tensors (forward-mode gradients included, which it then refuses)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class _Select(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, s):
         ctx.set_materialize_grads(False)
-        idx, w, cidx, cw, stats, load = ops.select_fwd(logits, bias, s)
+        idx, w, cidx, cw, load, stats = ops.select_fwd(logits, bias, s, True)
         ctx.s = s
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, idx, w, cw, stats)
+        ctx.save_for_backward(logits, idx, w, cw, stats)
         ctx.mark_non_differentiable(idx, cidx, load)
         return idx, w, cidx, cw, load
 
@@ -968,9 +976,11 @@ class _Select(torch.autograd.Function):
 _MOST_SELECTED, _MOST_ROUTED, _MOST_GROUPS = 128, 16384, 64
 
 
-def _select_shape(rows: int, chapters: int, top_k: int, score: str, num_shared: int, routed_scale: float, num_groups: int,
-                  top_groups: Optional[int], group_score: str, renormalize: bool):
-    """The descriptor of a selection, its sizes and names checked (top_k as the router has it: at most what there is)."""
+@lru_cache(maxsize=256)
+def _select_image(chapters: int, top_k: int, score: str, num_shared: int, routed_scale: float, num_groups: int,
+                  top_groups: Optional[int], group_score: str, renormalize: bool) -> bytes:
+    """The descriptor of a selection but for its rows, its sizes and names checked (top_k as the router has it: at most what there
+    is)."""
     if score not in ops.SCORES:
         raise ValueError(f"score must be 'softmax' or 'sigmoid', got {score!r}")
     if group_score not in ("max", "top2"):
@@ -990,8 +1000,8 @@ def _select_shape(rows: int, chapters: int, top_k: int, score: str, num_shared: 
     k = min(int(top_k), n)
     if k > _MOST_SELECTED or k > keep * (n // num_groups):
         raise ValueError(f"top_k ({k}) must be at most {_MOST_SELECTED} and the {keep * (n // num_groups)} chapters of {keep} groups")
-    return L.SelectShape(rows, chapters, k, num_shared, ops.SCORES[score], num_groups, keep, int(group_score == "top2"),
-                         int(bool(renormalize)), 0, 0, float(routed_scale))
+    return bytes(L.SelectShape(0, chapters, k, num_shared, ops.SCORES[score], num_groups, keep, int(group_score == "top2"),
+                               int(bool(renormalize)), 0, 0, float(routed_scale)))
 
 
 def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax", balance_bias: Optional[torch.Tensor] = None,
@@ -1012,28 +1022,31 @@ def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     if logits.dim() < 2:
         raise ValueError(f"logits must be [..., num_chapters], got shape {tuple(logits.shape)}")
     c = logits.shape[-1]
-    lead = logits.shape[:-1]
-    rows = logits.numel() // max(c, 1)
-    s = _select_shape(rows, c, int(top_k), score, int(num_shared), routed_scale, int(num_groups), top_groups, group_score, renormalize)
+    s = L.SelectShape.from_buffer_copy(_select_image(c, top_k, score, num_shared, routed_scale, num_groups, top_groups, group_score,
+                                                     renormalize))
     L.require_cuda(logits, balance_bias)
     if balance_bias is not None:
         _check_numel("balance_bias", balance_bias, c)
         if balance_bias.device != logits.device:
             raise ValueError("balance_bias must be on the device of the logits")
-        balance_bias = ops._contig(balance_bias.detach().float())
+        if balance_bias.dtype != torch.float32 or not balance_bias.is_contiguous():
+            balance_bias = balance_bias.detach().float().contiguous()
     z = logits if logits.dim() == 2 else logits.reshape(-1, c)
     if z.stride(1) != 1 or z.stride(0) < c:
         z = z.contiguous()
-    s.dtype, s.ld = L.dtype_code(z.dtype), max(c, z.stride(0))
-    if rows == 0:
-        dev, joint = z.device, s.num_shared + s.top_k
+    s.rows, s.dtype, s.ld = z.shape[0], L.dtype_code(z.dtype), max(c, z.stride(0))
+    if s.rows == 0:
+        joint = s.num_shared + s.top_k
         flat = (z.new_empty(0, s.top_k, dtype=torch.int64), z.new_empty(0, s.top_k, dtype=torch.float32),
                 z.new_empty(0, joint, dtype=torch.int32), z.new_empty(0, joint, dtype=torch.float32),
-                torch.zeros(c, dtype=torch.int32, device=dev))
-    else:
+                torch.zeros(c, dtype=torch.int32, device=z.device))
+    elif _differentiated(z):
         flat = _Select.apply(z, balance_bias, s)
+    else:
+        flat = ops.select_fwd(z, balance_bias, s, False)[:5]
     if logits.dim() == 2:
         return ChapterSelection(*flat)
+    lead = logits.shape[:-1]
     return ChapterSelection(*[t.view(*lead, t.shape[-1]) for t in flat[:4]], flat[4])
 
 
@@ -1104,18 +1117,21 @@ def router_logits(h: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 # --------------------------------------------------------------------------------------------
 # a block's output merged into the residual stream
 # --------------------------------------------------------------------------------------------
+def _dense_f32(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
+
+
 class _GatedResidual(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, weight, bias, gate, next_weight, next_bias, s):
         ctx.set_materialize_grads(False)
         params = weight, bias, gate, next_weight, next_bias
-        x, f = ops._contig(x), ops._contig(f)
-        p32 = [None if t is None else ops._contig(t.detach().float()) for t in params]
-        train = any(ctx.needs_input_grad)
-        y, n, stats = ops.gated_residual_fwd(s, x, f, *p32, train)
-        if train:
-            ctx.save_for_backward(x, f, *p32, stats)
-            ctx.s, ctx.dtypes = s, [None if t is None else t.dtype for t in params]
+        x, f, p32 = ops._contig(x), ops._contig(f), [_dense_f32(t) for t in params]
+        y, n, stats = ops.gated_residual_fwd(s, x, f, *p32, True)
+        ctx.save_for_backward(x, f, *p32, stats)
+        ctx.s, ctx.dtypes = s, [None if t is None else t.dtype for t in params]
         return y, n
 
     @staticmethod
@@ -1126,13 +1142,14 @@ class _GatedResidual(torch.autograd.Function):
         x, f, weight, bias, gate, next_weight, next_bias, stats = ctx.saved_tensors
         d_y = None if d_y is None else ops._contig(d_y.to(x.dtype))
         d_n = None if d_n is None else ops._contig(d_n.to(f.dtype))
-        d_x, d_f, *d_params = ops.gated_residual_bwd(ctx.s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n,
-                                                     ctx.needs_input_grad[0], bias is not None, next_bias is not None)
+        need = ctx.needs_input_grad
+        d_x, d_f, *d_params = ops.gated_residual_bwd(ctx.s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n, need[0],
+                                                     bias is not None, next_bias is not None)
         if d_n is None:
             d_params[3] = d_params[4] = None           # the next norm was not used: no gradient, not a zero one
-        d_params = [None if t is None or not need else t.to(dt)
-                    for t, dt, need in zip(d_params, ctx.dtypes, ctx.needs_input_grad[2:7])]
-        return d_x, d_f if ctx.needs_input_grad[1] else None, *d_params, None
+        d_params = [None if t is None or not want else t if dt == torch.float32 else t.to(dt)
+                    for t, dt, want in zip(d_params, ctx.dtypes, need[2:7])]
+        return d_x, d_f if need[1] else None, *d_params, None
 
 
 def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -1146,36 +1163,43 @@ def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: torch.Ten
     type of ``x``, the next norm's result that of ``branch`` and is taken of y before y is rounded.  ``norm_type`` is ``rms`` (no
     biases) or ``layernorm``.  ``gate``: None, [d], or [B, d] with one row per sequence (as adaptive norms have it).  Sums,
     statistics and parameter gradients are fp32.  d is at most 8192."""
-    if x.dim() not in (2, 3) or x.shape != branch.shape:
-        raise ValueError(f"x and branch must share a shape [B, L, d] or [rows, d], got {tuple(x.shape)} and {tuple(branch.shape)}")
+    shape = x.shape
+    if len(shape) not in (2, 3) or shape != branch.shape:
+        raise ValueError(f"x and branch must share a shape [B, L, d] or [rows, d], got {tuple(shape)} and {tuple(branch.shape)}")
     if norm_type not in ("rms", "layernorm"):
         raise ValueError(f"norm_type must be 'rms' or 'layernorm', got {norm_type!r}")
-    d = x.shape[-1]
+    d = shape[-1]
     if not 1 <= d <= 8192:
         raise ValueError(f"the width must be in 1..8192, got {d}")
     if norm_type == "rms" and (bias is not None or next_bias is not None):
         raise ValueError("an RMSNorm has no bias")
     if next_bias is not None and next_weight is None:
         raise ValueError("next_bias needs next_weight")
-    params = {"weight": weight, "bias": bias, "next_weight": next_weight, "next_bias": next_bias}
-    for name, t in params.items():
-        if t is not None and (t.dim() != 1 or t.shape[0] != d):
+    params = weight, bias, next_weight, next_bias
+    for name, t in zip(("weight", "bias", "next_weight", "next_bias"), params):
+        if t is not None and t.shape != (d,):
             raise ValueError(f"{name} must have {d} elements, got shape {tuple(t.shape)}")
     gate_seq = 0
-    if gate is not None and gate.dim() == 2 and x.dim() == 3 and tuple(gate.shape) == (x.shape[0], d):
-        gate_seq = x.shape[1]
-    elif gate is not None and tuple(gate.shape) != (d,):
-        raise ValueError(f"gate must be [d] or, beside [B, L, d], [B, d]; got shape {tuple(gate.shape)} for {tuple(x.shape)}")
-    L.require_cuda(x, branch, gate, *params.values())
-    if any(t is not None and t.device != x.device for t in (branch, gate, *params.values())):
-        raise ValueError("all tensors must be on the device of x")
+    if gate is not None and gate.shape != (d,):
+        if len(shape) != 3 or gate.shape != (shape[0], d):
+            raise ValueError(f"gate must be [d] or, beside [B, L, d], [B, d]; got shape {tuple(gate.shape)} for {tuple(shape)}")
+        gate_seq = shape[1]
+    device = x.device
+    for t in (x, branch, gate, *params):
+        if t is not None and (t.device != device or not t.is_cuda):
+            L.require_cuda(x, branch, gate, *params)
+            raise ValueError("all tensors must be on the device of x")
     rows = x.numel() // d
     s = L.ResidualShape(rows, d, L.NORM_CODES[norm_type], L.dtype_code(x.dtype), L.dtype_code(branch.dtype), gate_seq,
-                        float(residual_scale), float(eps), float(eps if next_eps is None else next_eps))
+                        residual_scale, eps, eps if next_eps is None else next_eps)
     if rows == 0:
         y = x * residual_scale + 0.0 * branch.to(x.dtype)          # (nothing to compute; a graph that gives zero gradients)
         return (y, 0.0 * branch) if next_weight is not None else y
-    if gate_seq and x.shape[0] > 65534:
+    if gate_seq and shape[0] > 65534:
         raise ValueError("at most 65,534 sequences with a gate of their own")
-    y, n = _GatedResidual.apply(x, branch, weight, bias, gate, next_weight, next_bias, s)
+    if _differentiated(x, branch, gate, *params):
+        y, n = _GatedResidual.apply(x, branch, weight, bias, gate, next_weight, next_bias, s)
+    else:
+        y, n, _ = ops.gated_residual_fwd(s, ops._contig(x), ops._contig(branch), _dense_f32(weight), _dense_f32(bias), _dense_f32(gate),
+                                         _dense_f32(next_weight), _dense_f32(next_bias), False)
     return (y, n) if next_weight is not None else y

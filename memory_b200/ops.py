@@ -293,35 +293,38 @@ def agree_probe(device, late_warps: int, poll_limit: int):
 SCORES = {"softmax": 0, "sigmoid": 1}
 
 
-@_instrument("select_fwd", 1)
-def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s):
+def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, want_stats: bool):
     """``moc_select_fwd`` on logits [rows, C] (fp32 or bf16, unit column stride); ``s``: the filled ``SelectShape``.  Returns (idx
-    int64, weights, joint idx int32, joint weights, row stats, load)."""
+    int64, weights, joint idx int32, joint weights, load, row stats or None)."""
     dev, rows, k, joint = logits.device, s.rows, s.top_k, s.num_shared + s.top_k
-    # one allocation for the fp32 outputs and the two int32 lists (fp32 row stats first: they want 16 bytes)
-    idx = torch.empty(rows, k, dtype=torch.int64, device=dev)
-    f = torch.empty(rows * (4 + k + joint), dtype=torch.float32, device=dev)
-    i = torch.empty(rows * joint + s.num_chapters, dtype=torch.int32, device=dev)
-    stats, weights, comb_w = f[:rows * 4].view(rows, 4), f[rows * 4:rows * (4 + k)].view(rows, k), f[rows * (4 + k):].view(rows, joint)
-    comb_idx, load = i[:rows * joint].view(rows, joint), i[rows * joint:]
+    f32, i32 = torch.float32, torch.int32
+    idx = torch.empty((rows, k), dtype=torch.int64, device=dev)
+    weights = torch.empty((rows, k), dtype=f32, device=dev)
+    comb_idx = torch.empty((rows, joint), dtype=i32, device=dev)
+    comb_w = torch.empty((rows, joint), dtype=f32, device=dev)
+    load = torch.empty(s.num_chapters, dtype=i32, device=dev)
+    stats = torch.empty((rows, 4), dtype=f32, device=dev) if want_stats else None
     with _on(dev):
-        rc = L.lib().moc_select_fwd(C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(),
-                                    comb_idx.data_ptr(), comb_w.data_ptr(), stats.data_ptr(), load.data_ptr(), L.stream_ptr(dev))
+        args = (C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(),
+                comb_w.data_ptr(), L.ptr(stats), load.data_ptr(), L.stream_ptr(dev))
+        rc = L.lib().moc_select_fwd(*args) if TIMER is None else _timed("select_fwd", lambda: L.lib().moc_select_fwd(*args))
     if rc:
         L.check(rc, "moc_select_fwd")
-    return idx, weights, comb_idx, comb_w, stats, load
+    _report(1, lambda: ("select_fwd:" + _DTYPE_TAG[logits.dtype],))
+    return idx, weights, comb_idx, comb_w, load, stats
 
 
-@_instrument("select_bwd", 1)
 def select_bwd(logits: torch.Tensor, s, idx, weights, comb_w, stats, g_weights, g_comb) -> torch.Tensor:
     """Gradient of the logits [rows, C] (dense, their type) from those of the weights and the joint weights (either may be None)."""
     dev = logits.device
-    d = torch.empty(s.rows, s.num_chapters, dtype=logits.dtype, device=dev)
+    d = torch.empty((s.rows, s.num_chapters), dtype=logits.dtype, device=dev)
     with _on(dev):
-        rc = L.lib().moc_select_bwd(C.byref(s), logits.data_ptr(), idx.data_ptr(), weights.data_ptr(), comb_w.data_ptr(),
-                                    stats.data_ptr(), L.ptr(g_weights), L.ptr(g_comb), d.data_ptr(), L.stream_ptr(dev))
+        args = (C.byref(s), logits.data_ptr(), idx.data_ptr(), weights.data_ptr(), comb_w.data_ptr(), stats.data_ptr(),
+                L.ptr(g_weights), L.ptr(g_comb), d.data_ptr(), L.stream_ptr(dev))
+        rc = L.lib().moc_select_bwd(*args) if TIMER is None else _timed("select_bwd", lambda: L.lib().moc_select_bwd(*args))
     if rc:
         L.check(rc, "moc_select_bwd")
+    _report(1, lambda: ("select_bwd:" + _DTYPE_TAG[logits.dtype],))
     return d
 
 
@@ -586,30 +589,30 @@ def bank_adamw_step(param: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torc
 _GRAD_DTYPES = {torch.float32: L.MOC_F32, torch.bfloat16: L.MOC_BF16, torch.float16: L.MOC_F16}
 
 
-def _grad_clip_launches(entries, *a, **k):
-    return 2 * (1 if len(entries) <= 64 else -(-len(entries) // 680))
-
-
-@_instrument("grad_clip", _grad_clip_launches)
-def grad_clip(entries, max_norm: float, eps: float, device: torch.device) -> torch.Tensor:
-    """``moc_grad_clip``: ``entries`` are (gradient, output or None, count or None, unit, weight) with dense tensors on
-    ``device``.  Returns [2] fp32 = (norm, coefficient)."""
-    n = len(entries)
-    table = (L.GradDesc * n)()
-    codes = _GRAD_DTYPES
-    for d, (g, out, count, unit, weight) in zip(table, entries):
-        d.grad, d.elems, d.dtype, d.unit, d.weight = g.data_ptr(), g.numel(), codes[g.dtype], unit, weight
-        if out is not None:
-            d.out, d.out_dtype = out.data_ptr(), codes[out.dtype]
-        if count is not None:
-            d.count = count.data_ptr()
-    lib = L.lib()
+def grad_clip(grads, out, banks, max_norm: float, eps: float, device: torch.device) -> torch.Tensor:
+    """``moc_grad_clip`` on dense, contiguous ``grads`` and the tensors ``out`` that receive them clipped (or the gradients
+    themselves), and on compact rows ``banks``: (rows, count, elements of a unit, weight), which count in the norm alone.  Returns
+    [2] fp32 = (norm, coefficient)."""
+    n, m = len(grads), len(banks)
+    codes, lib = _GRAD_DTYPES, L.lib()
+    total = n + m
+    # one column of the table per list comprehension: a third of the time of a loop over the tensors
+    ptrs = [g.data_ptr() for g in grads] + [b[0].data_ptr() for b in banks]
+    sizes = [g.numel() for g in grads] + [b[0].numel() for b in banks]
+    types = [codes[g.dtype] for g in grads] + [codes[b[0].dtype] for b in banks]
+    same = out is grads
+    outs = ptrs[:n] if same else [o.data_ptr() for o in out]
+    out_types = types[:n] if same else [codes[o.dtype] for o in out]
     result = torch.empty(2, dtype=torch.float32, device=device)
-    ws = torch.empty(lib.moc_grad_clip_workspace_bytes(n), dtype=torch.uint8, device=device)
+    ws = torch.empty(lib.moc_grad_clip_workspace_bytes(total), dtype=torch.uint8, device=device)
     with _on(device):
-        rc = lib.moc_grad_clip(table, n, float(max_norm), float(eps), result.data_ptr(), ws.data_ptr(), ws.numel(),
-                               L.stream_ptr(device))
+        args = (total, n, (C.c_void_p * total)(*ptrs), (C.c_int64 * total)(*sizes), (C.c_uint8 * total)(*types),
+                (C.c_void_p * n)(*outs), (C.c_uint8 * n)(*out_types), (C.c_void_p * m)(*[b[1].data_ptr() for b in banks]),
+                (C.c_int32 * m)(*[b[2] for b in banks]), (C.c_float * m)(*[b[3] for b in banks]), float(max_norm), float(eps),
+                result.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(device))
+        rc = lib.moc_grad_clip(*args) if TIMER is None else _timed("grad_clip", lambda: lib.moc_grad_clip(*args))
     L.check(rc, "moc_grad_clip")
+    _report(2 * (1 if total <= 64 else -(-total // 680)), lambda: ("grad_clip:-",))
     return result
 
 
@@ -1304,41 +1307,43 @@ def norm_bwd(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, stats: tor
 # --------------------------------------------------------------------------------------------
 # a block's output merged into the residual stream
 # --------------------------------------------------------------------------------------------
-@_instrument("gated_residual_fwd", 1)
 def gated_residual_fwd(s, x, f, weight, bias, gate, next_weight, next_bias, want_stats: bool):
     """``moc_gated_residual_fwd`` on dense x and f; returns (y like x, n like f or None, stats or None)."""
     dev, p = x.device, L.ptr
     y = torch.empty_like(x)
     n = torch.empty_like(f) if next_weight is not None else None
-    stats = torch.empty(s.rows, 4, dtype=torch.float32, device=dev) if want_stats else None
+    stats = torch.empty((s.rows, 4), dtype=torch.float32, device=dev) if want_stats else None
     with _on(dev):
-        rc = L.lib().moc_gated_residual_fwd(C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight),
-                                            p(next_bias), y.data_ptr(), p(n), p(stats), L.stream_ptr(dev))
+        args = (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), p(next_bias), y.data_ptr(),
+                p(n), p(stats), L.stream_ptr(dev))
+        rc = (L.lib().moc_gated_residual_fwd(*args) if TIMER is None
+              else _timed("gated_residual_fwd", lambda: L.lib().moc_gated_residual_fwd(*args)))
     if rc:
         L.check(rc, "moc_gated_residual_fwd")
+    _report(1, lambda: ("gated_residual_fwd:" + _DTYPE_TAG[x.dtype],))
     return y, n, stats
 
 
-@_instrument("gated_residual_bwd", 2)
 def gated_residual_bwd(s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n, want_dx: bool, want_bias: bool,
                        want_next_bias: bool):
     """Gradients of :func:`gated_residual_fwd`: (d_x or None, d_f, d_weight, d_bias, d_gate, d_next_weight, d_next_bias)."""
     dev, p, lib = x.device, L.ptr, L.lib()
     d_x = torch.empty_like(x) if want_dx else None
     d_f = torch.empty_like(f)
-
-    def vector(like, want=True):
-        return torch.empty_like(like) if like is not None and want else None
-    d_w, d_gate = vector(weight), vector(gate)
-    d_b, d_nw = vector(weight, want_bias), vector(next_weight)
-    d_nb = vector(next_weight, want_next_bias)
+    d_w, d_gate = torch.empty_like(weight), None if gate is None else torch.empty_like(gate)
+    d_b = torch.empty_like(weight) if want_bias else None
+    d_nw = None if next_weight is None else torch.empty_like(weight)
+    d_nb = torch.empty_like(weight) if want_next_bias else None
     with _on(dev):
         scratch = torch.empty(lib.moc_gated_residual_bwd_scratch_bytes(C.byref(s), int(gate is not None)), dtype=torch.uint8, device=dev)
-        rc = lib.moc_gated_residual_bwd(C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight),
-                                        stats.data_ptr(), p(d_y), p(d_n), p(d_x), d_f.data_ptr(), p(d_w), p(d_b), p(d_gate), p(d_nw),
-                                        p(d_nb), scratch.data_ptr(), L.stream_ptr(dev))
+        args = (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), stats.data_ptr(), p(d_y),
+                p(d_n), p(d_x), d_f.data_ptr(), d_w.data_ptr(), p(d_b), p(d_gate), p(d_nw), p(d_nb), scratch.data_ptr(),
+                L.stream_ptr(dev))
+        rc = (lib.moc_gated_residual_bwd(*args) if TIMER is None
+              else _timed("gated_residual_bwd", lambda: lib.moc_gated_residual_bwd(*args)))
     if rc:
         L.check(rc, "moc_gated_residual_bwd")
+    _report(2, lambda: ("gated_residual_bwd:" + _DTYPE_TAG[x.dtype],))
     return d_x, d_f, d_w, d_b, d_gate, d_nw, d_nb
 
 
@@ -1382,7 +1387,6 @@ def quantize_rows(rows: torch.Tensor, scale_rows: int, head_dim: int, values: to
     L.check(rc, "moc_quantize_rows")
 
 
-@_instrument("decode_attn_cache", 1)
 def decode_attn_cache(q, kv_bank, kv_scale, scale_rows: int, idx, weights, counts, num_heads: int, num_kv_heads: int,
                       tokens_per_chapter: int, scale: float, want_lse: bool):
     """``moc_decode_attn_cache``: q [B, n_q, H*64] bf16 over a bf16 cache (``kv_scale`` None) or an 8-bit one.  Returns (out, lse or
@@ -1391,13 +1395,15 @@ def decode_attn_cache(q, kv_bank, kv_scale, scale_rows: int, idx, weights, count
     dev = q.device
     s = L.DecodeShape(b, n_q, num_heads, num_kv_heads, hd // num_heads, idx.shape[1], tokens_per_chapter, scale)
     out = torch.empty_like(q)
-    lse = torch.empty(b, n_q, num_heads, dtype=torch.float32, device=dev) if want_lse else None
+    lse = torch.empty((b, n_q, num_heads), dtype=torch.float32, device=dev) if want_lse else None
     with _on(dev):
-        rc = L.lib().moc_decode_attn_cache(C.byref(s), q.data_ptr(), kv_bank.data_ptr(), L.ptr(kv_scale), scale_rows, kv_bank.shape[0],
-                                           idx.data_ptr(), weights.data_ptr(), L.ptr(counts), out.data_ptr(), L.ptr(lse),
-                                           L.ptr(L.status_word(dev)), L.stream_ptr(dev))
+        args = (C.byref(s), q.data_ptr(), kv_bank.data_ptr(), L.ptr(kv_scale), scale_rows, kv_bank.shape[0], idx.data_ptr(),
+                weights.data_ptr(), L.ptr(counts), out.data_ptr(), L.ptr(lse), L.status_word(dev).data_ptr(), L.stream_ptr(dev))
+        rc = (L.lib().moc_decode_attn_cache(*args) if TIMER is None
+              else _timed("decode_attn", lambda: L.lib().moc_decode_attn_cache(*args)))
     if rc:
         L.check(rc, "moc_decode_attn_cache")
+    _report(1, lambda: ("decode_attn:bf16" if kv_scale is None else "decode_attn:e4m3",))
     return out, lse
 
 

@@ -102,61 +102,59 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    listed = [parameters] if torch.is_tensor(parameters) else list(parameters)
-    grads = [p.grad if isinstance(p, torch.nn.Parameter) or (p.requires_grad and p.is_leaf) else p for p in listed]
-    if out is None:
-        pairs = [(g, g) for g in grads if g is not None]
-    else:
-        out = list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"out must have one tensor per gradient: {len(out)} vs {len(grads)}")
-        pairs = [(g, o) for g, o in zip(grads, out) if g is not None]
-    device = pairs[0][0].device if pairs else None
-    entries, copies, spans, seen = [], [], [], set()
-    for g, o in pairs:
-        if g.is_sparse or not g.is_cuda or g.device != device:
-            raise ValueError("gradients must be dense CUDA tensors on one device")
-        if g.dtype not in ops._GRAD_DTYPES or o.dtype not in ops._GRAD_DTYPES:
-            raise TypeError(f"gradients must be float32, bfloat16 or float16, got {g.dtype} and {o.dtype}")
-        if o is not g and (o.shape != g.shape or o.device != device):
-            raise ValueError("out must match the gradients in shape and device")
-        n, key = g.numel(), (g.data_ptr(), g.shape, g.stride())
-        if key in seen and n and o is not g:
-            raise ValueError("a gradient is listed twice with an out of its own")
-        if n == 0 or key in seen:
-            continue
-        seen.add(key)
-        src = g if g.is_contiguous() else g.contiguous()
-        dst = src if o is g else o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=device)
-        if dst is not o:
-            copies.append((o, dst))
-        entries.append((src, dst, None, 0, 1.0))
-        spans.append((src.data_ptr(), n * src.element_size()))
-        if dst is not src:
-            spans.append((dst.data_ptr(), n * dst.element_size()))
-    _refuse_overlaps(spans)
+    grads = [_gradient(p) for p in ((parameters,) if torch.is_tensor(parameters) else parameters)]
+    outs = grads if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError(f"out must have one tensor per gradient: {len(outs)} vs {len(grads)}")
+    if any(g is None for g in grads):
+        outs = [o for g, o in zip(grads, outs) if g is not None]
+        grads = outs if out is None else [g for g in grads if g is not None]
+    known, banks = ops._GRAD_DTYPES, []
     for sink in bank_grads:
         if len(sink.entries) > 1:
             raise NotImplementedError("one compact entry per bank: sum several layers' entries first (ops.bank_grad_merge)")
         for _, count, rows, t in sink.entries:
-            device = rows.device if device is None else device
-            if rows.device != device or count.device != device:
-                raise ValueError("gradients must be dense CUDA tensors on one device")
-            L.require_cuda(rows, count)
-            entries.append((ops._contig(rows), None, count, t * rows.shape[1], float(sink.scale)))
-    if device is None:
+            banks.append((ops._contig(rows), count, t * rows.shape[1], float(sink.scale)))
+    if not grads and not banks:
         raise ValueError("no gradients to clip")
-    result = ops.grad_clip(entries, max_norm, eps, device)
-    for o, dst in copies:
-        o.copy_(dst)
-    norm, coefficient = result.unbind()
-    return GradClip(norm, coefficient)
+    device = grads[0].device if grads else banks[0][0].device
+    tensors = [*grads, *(b[0] for b in banks), *(b[1] for b in banks)] + ([] if outs is grads else outs)
+    if device.type != "cuda" or any(t.device != device or t.layout is not torch.strided for t in tensors):
+        raise ValueError("gradients must be dense CUDA tensors on one device")
+    if any(t.dtype not in known for t in (*grads, *outs, *(b[0] for b in banks))):
+        raise TypeError("gradients must be float32, bfloat16 or float16")
+    if outs is not grads and any(o.shape != g.shape for g, o in zip(grads, outs)):
+        raise ValueError("out must match the gradients in shape")
+    copies: list = []
+    if len({(g.data_ptr(), g.shape) for g in grads}) < len(grads) or not all(t.is_contiguous() for t in (*grads, *outs)):
+        grads, outs, copies = _distinct_and_dense(grads, outs)
+    result = ops.grad_clip(grads, outs, banks, max_norm, eps, device)
+    for o, dense in copies:
+        o.copy_(dense)
+    return GradClip(*result.unbind())
 
 
-def _refuse_overlaps(spans: list) -> None:
-    """``spans``: (first byte, bytes) of the tensors that are read (and clipped in place) and of separate outputs."""
-    end = 0
-    for first, size in sorted(spans):
-        if first < end:
-            raise ValueError("gradients (and out) must not overlap")
-        end = first + size
+def _gradient(p: torch.Tensor) -> Optional[torch.Tensor]:
+    if type(p) is torch.Tensor and not p.requires_grad:
+        return p
+    return p.grad if isinstance(p, torch.nn.Parameter) or p.is_leaf else p.detach()
+
+
+def _distinct_and_dense(grads: list, outs: list):
+    """The same lists without a gradient's second mention, with dense copies in the place of other layouts: (gradients, outputs,
+    (tensor, dense copy) pairs to copy back)."""
+    in_place, seen, src, dst, copies = outs is grads, set(), [], [], []
+    for g, o in zip(grads, outs):
+        key = (g.data_ptr(), g.shape, g.stride(), g.dtype)
+        if g.numel() == 0:
+            continue
+        if key in seen:
+            if in_place:
+                continue
+            raise ValueError("a gradient is listed twice with an out of its own")
+        seen.add(key)
+        src.append(g.contiguous())
+        dst.append(src[-1] if in_place else o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device))
+        if dst[-1] is not o:
+            copies.append((o, dst[-1]))
+    return src, src if in_place else dst, copies

@@ -222,13 +222,15 @@ def test_c_entry_refuses_without_a_gpu():
     assert lib.moc_grad_clip_workspace_bytes(-1) == -1
     assert lib.moc_grad_clip_workspace_bytes(0) > 0 and lib.moc_grad_clip_workspace_bytes(681) > lib.moc_grad_clip_workspace_bytes(680) - 1
     p = 4096
-    size = lib.moc_grad_clip_workspace_bytes(1)
-    good = dict(grad=p, out=p, elems=4, count=None, unit=0, dtype=0, out_dtype=0, weight=1.0)
-    for change in (dict(grad=None), dict(elems=-1), dict(dtype=7), dict(grad=p + 2, out=None), dict(count=p), dict(out_dtype=1),
-                   dict(count=p, out=None, unit=0)):
-        d = L.GradDesc(**dict(good, **change))
-        assert lib.moc_grad_clip(C.byref(d), 1, 1.0, 1e-6, p, p, size, None) == -1
-    d = L.GradDesc(**good)
-    assert lib.moc_grad_clip(C.byref(d), 1, -1.0, 1e-6, p, p, size, None) == -1
-    assert lib.moc_grad_clip(C.byref(d), 1, 1.0, 1e-6, p, p, size - 1, None) == -1
-    assert lib.moc_grad_clip(C.byref(d), 1, 1.0, 1e-6, None, p, size, None) == -1
+    size = lib.moc_grad_clip_workspace_bytes(2)
+
+    def call(count=2, dense=1, grads=(p, p), elems=(4, 8), dtypes=(0, 0), out=(p + 64,), out_dtypes=(0,), counts=(p,), units=(4,), max_norm=1.0,
+             result=p, ws=size):
+        ptrs, sizes, types = C.c_void_p * 2, C.c_int64 * 2, C.c_uint8 * 2
+        return lib.moc_grad_clip(count, dense, ptrs(*grads), sizes(*elems), types(*dtypes), ptrs(*out), types(*out_dtypes), ptrs(*counts),
+                                 (C.c_int32 * 2)(*units), (C.c_float * 2)(1.0), max_norm, 1e-6, result, p, ws, None)
+    for change in (dict(count=-1), dict(dense=3), dict(dense=-1), dict(grads=(None, p)), dict(elems=(-1, 8)), dict(dtypes=(7, 0)), dict(dtypes=(0, 3)),
+                   dict(out_dtypes=(3,)), dict(grads=(p + 2, p)), dict(out=(p + 3,)), dict(out=(p,), out_dtypes=(1,)), dict(counts=(None,)),
+                   dict(units=(0,)), dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(result=None), dict(ws=size - 1),
+                   dict(out=(p + 8,)), dict(out=(p,))):
+        assert call(**change) == -1, change
