@@ -41,7 +41,7 @@ struct SelectParams {
   int rows, N, S, k, groups, keep, per;
   FastDiv per_group;
   int sigmoid, top2, renorm;
-  int clear_load;                 // the launch is one CTA, which sets the counts to zero itself
+  int count_here;                 // the launch is one CTA, which counts as well (`load` from zero)
   float rho;
 };
 
@@ -96,6 +96,9 @@ __device__ __forceinline__ typename KeyOf<K>::type candidate_key(const SelectPar
 }
 template <typename U> __device__ __forceinline__ bool chosen_from(U key) { return key > static_cast<U>(kFiller); }
 
+// whether candidate ia with key a comes before ib with key b
+__device__ __forceinline__ bool ahead(uint64_t a, int ia, uint64_t b, int ib) { return a > b || (a == b && ia < ib); }
+
 // Fast keys of the first pass (softmax: `e` = exp(z - m) and 1 / total): -inf for what may not be chosen, NaN stays.
 __device__ __forceinline__ float fast_sigmoid(float z) {
   float e, s;
@@ -143,7 +146,7 @@ __device__ __forceinline__ void write_row(const SelectParams& p, long long row, 
       id[q] = pick(j, ok, z);
       if (ok) w[q] = score_of<float>(p, z, m, total);
       mass += w[q];
-      if (p.load != nullptr) atomicAdd(p.load + p.S + id[q], 1);
+      if (p.count_here) atomicAdd(p.load + p.S + id[q], 1);
     }
   }
   mass = warp_total(mass);
@@ -175,74 +178,201 @@ __device__ __forceinline__ void write_row(const SelectParams& p, long long row, 
 
 // 64-bit sum of the exponentials of a row, by `threads` threads of which this is `t`; their parts are still to be added
 template <typename LT> __device__ __noinline__ double total64(const LT* z, int n, float m, int t, int threads) {
-  double sum = 0.0;
+  double sum[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 1
-  for (int c = t; c < n; c += threads) {
-    const float v = logit_of(z, c);
-    if (!masked(v)) sum += exp(static_cast<double>(v) - static_cast<double>(m));
+  for (int c = t; c < n; c += 4 * threads) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float v = c + u * threads < n ? logit_of(z, c + u * threads) : -INFINITY;
+      if (!masked(v)) sum[u] += exp(static_cast<double>(v) - static_cast<double>(m));
+    }
   }
-  return sum;
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 template <typename LT> __device__ __noinline__ uint64_t key64(const SelectParams& p, const LT* z, int c, float m, double total, bool group) {
   return candidate_key<double>(p, logit_of(z, c), c, m, total, group);
 }
 
-// ---- a warp a row ----------------------------------------------------------------------------
-// The whole selection by 64-bit keys: lane j keeps the j-th pick.  `keys`: 64-bit words of this warp, N + N / 32.
+// Candidates ranked by 64-bit keys: whether a, the next above b, is before it for certain.  Softmax keys may have been formed with
+// the fp32 sum of the exponentials, off by 2e-6 at most: it scales the difference of the scores, not that of the biases.
+__device__ __forceinline__ bool apart64(const SelectParams& p, uint64_t a, int ia, uint64_t b, int ib) {
+  if (p.sigmoid || a == b) return p.sigmoid || p.bias[p.S + ia] == p.bias[p.S + ib];
+  const double sa = of_key(a), sb = of_key(b);
+  const double da = sa - static_cast<double>(p.bias[p.S + ia]), db = sb - static_cast<double>(p.bias[p.S + ib]);
+  return sa - sb > 2.2e-6 * fabs(da - db);
+}
+// Whether fp32 values tell the groups that stay (least of them) from those that go: two keys each, or bare logits.  (Groups without a
+// candidate are behind all others, in the order of their ids.)
+__device__ __forceinline__ bool groups_apart(const SelectParams& p, float least, float most, float inv_total) {
+  return (p.bias == nullptr && !p.top2) || most == -INFINITY ||
+         least - most > 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total));
+}
+// Places of candidates (ids in the complements of the low words of `cand`) by their 64-bit keys, by `threads` threads of which this
+// is `t0`.  Returns whether this thread has met one that is not for certain before the next.
+__device__ __noinline__ bool rank_wide(const SelectParams& p, const unsigned long long* cand, const uint64_t* wide, int n, int t0, int threads,
+                                       int* place) {
+  bool unclear = false;
+  for (int t = t0; t < n; t += threads) {
+    const int id = static_cast<int>(~static_cast<uint32_t>(cand[t]));
+    const uint64_t mine = wide[t];
+    int rank = 0, nid = -1;
+    uint64_t next = 0;
+    for (int j = 0; j < n; ++j) {
+      const int oid = static_cast<int>(~static_cast<uint32_t>(cand[j]));
+      const uint64_t o = wide[j];
+      rank += ahead(o, oid, mine, id);
+      if (ahead(mine, id, o, oid) && (nid < 0 || ahead(o, oid, next, nid))) { next = o; nid = oid; }
+    }
+    if (rank < p.k) {
+      place[rank] = id;
+      unclear |= nid >= 0 && !apart64(p, mine, id, next, nid);
+    }
+  }
+  return unclear;
+}
+// The value of a group by 64-bit keys of the candidates that may be among its best, by one warp.
 template <typename LT>
-__device__ __noinline__ void choose_warp64(const SelectParams& p, const LT* z, float m, uint64_t* keys, int& pick, bool& ok) {
+__device__ __noinline__ uint64_t group_value64(const SelectParams& p, const LT* z, int g, float m, float inv_total, double total) {
+  const int lane = threadIdx.x & 31;
+  auto rough = [&](int c) {
+    const float v = logit_of(z, c);
+    if (masked(v)) return -INFINITY;
+    const float sc = p.sigmoid ? fast_sigmoid(v) : expf(v - m) * inv_total;
+    return p.bias != nullptr ? sc + p.bias[p.S + c] : p.top2 ? sc : v;
+  };
+  float a = -INFINITY, b = -INFINITY;
+  for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32) {
+    const float v = rough(c);
+    b = fmaxf(b, fminf(a, v));
+    a = fmaxf(a, v);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+    b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+    a = fmaxf(a, oa);
+  }
+  const float last = p.top2 ? b : a;
+  const float edge = last - 2.f * key_error(p, last, inv_total);
+  Best2<uint64_t> t{0, 0};
+  for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32)
+    if (rough(c) >= edge) take(t, key64(p, z, c, m, total, true));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const uint64_t ka = __shfl_xor_sync(0xffffffffu, t.a, o), kb = __shfl_xor_sync(0xffffffffu, t.b, o);
+    take(t, ka);
+    take(t, kb);
+  }
+  return group_value(p, t);
+}
+// Which groups stay, where fp32 values (of groups lane and lane + 32) close at the border between `least` and `most`: those near it
+// again in 64 bits.  The others are ahead of, or behind, all of them in any case.
+template <typename LT>
+__device__ __noinline__ unsigned long long choose_groups_near(const SelectParams& p, const LT* z, float v0, float v1, float least, float most,
+                                                              float m, float inv_total) {
+  const int lane = threadIdx.x & 31;
+  const double total = p.sigmoid ? 1.0 : warp_total(total64(z, p.N, m, lane, 32));
+  const float slack = 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total));
+  const float value[2] = {v0, v1};
+  uint64_t exact[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const bool near = lane + 32 * r < p.groups && value[r] >= most - slack && value[r] <= least + slack;
+    exact[r] = to_key(static_cast<double>(value[r]));
+    uint32_t todo = __ballot_sync(0xffffffffu, near);
+    while (todo != 0) {
+      const int g = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const uint64_t v = group_value64(p, z, g + 32 * r, m, inv_total, total);
+      if (lane == g) exact[r] = v;
+    }
+  }
+  int rank[2] = {0, 0};
+  for (int g = 0; g < p.groups; ++g) {
+    const uint64_t other = __shfl_sync(0xffffffffu, exact[g >> 5], g & 31);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) rank[r] += other > exact[r] || (other == exact[r] && g < lane + 32 * r);
+  }
+  const uint32_t lo = __ballot_sync(0xffffffffu, lane < p.groups && rank[0] < p.keep);
+  const uint32_t hi = __ballot_sync(0xffffffffu, lane + 32 < p.groups && rank[1] < p.keep);
+  return static_cast<unsigned long long>(hi) << 32 | lo;
+}
+
+// ---- a warp a row ----------------------------------------------------------------------------
+// What a warp keeps of the k best candidates seen so far, largest first.
+struct BestList {
+  uint64_t key[kMostK];
+  int id[kMostK];
+};
+
+// The whole selection by 64-bit keys, by one warp: the candidates stream by, those that are before the last place go into the list.
+template <typename LT>
+__device__ __noinline__ void choose_warp64(const SelectParams& p, const LT* z, float m, BestList& list) {
   const int lane = threadIdx.x & 31;
   double total = 1.0;
   if (!p.sigmoid) total = warp_total(total64(z, p.N, m, lane, 32));
   unsigned long long kept = ~0ull;
   if (p.keep < p.groups) {
-    __syncwarp();
-    for (int c = lane; c < p.N; c += 32) keys[c] = key64(p, z, c, m, total, true);
-    __syncwarp();
     uint64_t value[2] = {0, 0};
     int rank[2] = {0, 0};
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int g = lane + 32 * r;
-      if (g >= p.groups) continue;
+    for (int g = 0; g < p.groups; ++g) {
       Best2<uint64_t> t{0, 0};
-      for (int c = g * p.per; c < (g + 1) * p.per; ++c) take(t, keys[c]);
-      value[r] = group_value(p, t);
+      for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32) take(t, key64(p, z, c, m, total, true));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t a = __shfl_xor_sync(0xffffffffu, t.a, o), b = __shfl_xor_sync(0xffffffffu, t.b, o);
+        take(t, a);
+        take(t, b);
+      }
+      if (lane == (g & 31)) value[g >> 5] = group_value(p, t);
     }
     for (int g = 0; g < p.groups; ++g) {
       const uint64_t other = __shfl_sync(0xffffffffu, value[g >> 5], g & 31);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) rank[r] += other > value[r] || (other == value[r] && g < lane + 32 * r);
+      for (int r = 0; r < 2; ++r) rank[r] += ahead(other, g, value[r], lane + 32 * r);
     }
     const uint32_t lo = __ballot_sync(0xffffffffu, lane < p.groups && rank[0] < p.keep);
     const uint32_t hi = __ballot_sync(0xffffffffu, lane + 32 < p.groups && rank[1] < p.keep);
     kept = static_cast<unsigned long long>(hi) << 32 | lo;
   }
+  for (int j = lane; j < p.k; j += 32) { list.key[j] = 0; list.id[j] = 0x7FFFFFFF; }
   __syncwarp();
-  for (int c = lane; c < p.N; c += 32)
-    keys[c] = kept >> div_of(c, p.per_group) & 1 ? key64(p, z, c, m, total, false) : static_cast<uint64_t>(kFiller - c);
-  __syncwarp();
-  uint64_t best = 0;
-  int at = 0;
-  for (int c = lane; c < p.N; c += 32)
-    if (keys[c] > best) { best = keys[c]; at = c; }
-  for (int t = 0; t < p.k; ++t) {
-    const uint64_t top = warp_most(best);
-    const int id = static_cast<int>(__reduce_min_sync(0xffffffffu, best == top ? static_cast<uint32_t>(at) : 0xFFFFFFFFu));
-    if (lane == t) { pick = id; ok = chosen_from(top); }
-    if (best == top && at == id) {              // (only this lane's own columns)
-      keys[id] = 0;
-      best = 0;
-      for (int c = lane; c < p.N; c += 32)
-        if (keys[c] > best) { best = keys[c]; at = c; }
+  for (int c0 = 0; c0 < p.N; c0 += 32) {
+    const int c = c0 + lane;
+    uint64_t key = 0;
+    if (c < p.N) key = kept >> (div_of(c, p.per_group) & 63) & 1 ? key64(p, z, c, m, total, false) : static_cast<uint64_t>(kFiller - c);
+    uint32_t todo = __ballot_sync(0xffffffffu, ahead(key, c, list.key[p.k - 1], list.id[p.k - 1]) && c < p.N);
+    while (todo != 0) {
+      const int from = __ffs(todo) - 1, id = c0 + from;
+      todo &= todo - 1;
+      const uint64_t mine = __shfl_sync(0xffffffffu, key, from);
+      uint64_t k_new[kMostK / 32];
+      int i_new[kMostK / 32];
+#pragma unroll
+      for (int q = 0; q < kMostK / 32; ++q) {
+        const int j = lane + 32 * q;
+        k_new[q] = 0;
+        i_new[q] = 0;
+        if (j >= p.k) continue;
+        // entries behind the new one move down by one place
+        const bool here = !ahead(list.key[j], list.id[j], mine, id);
+        const bool above = j > 0 && !ahead(list.key[j - 1], list.id[j - 1], mine, id);
+        k_new[q] = above ? list.key[j - 1] : here ? mine : list.key[j];
+        i_new[q] = above ? list.id[j - 1] : here ? id : list.id[j];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < kMostK / 32; ++q)
+        if (lane + 32 * q < p.k) { list.key[lane + 32 * q] = k_new[q]; list.id[lane + 32 * q] = i_new[q]; }
+      __syncwarp();
     }
   }
 }
 
 // The groups that stay (bit g), from keys in shared memory (candidate c at c + c / 32), by R groups a lane (2: of more than 32) or
-// 1 / lanes of one; false: fp32 cannot tell.
-template <int R>
-__device__ __forceinline__ bool choose_groups_warp(const SelectParams& p, const float* sk, float inv_total, unsigned long long& kept) {
+// 1 / lanes of one.
+template <int R, typename LT>
+__device__ __forceinline__ unsigned long long choose_groups_warp(const SelectParams& p, const float* sk, const LT* z, float m, float inv_total) {
   const int lane = threadIdx.x & 31;
   const int shift = R > 1 || p.groups > 16 ? 0 : p.groups > 8 ? 1 : p.groups > 4 ? 2 : p.groups > 2 ? 3 : 4;     // log2 of a group's lanes
   const int lanes = 1 << shift, sub = lane & (lanes - 1);
@@ -284,22 +414,24 @@ __device__ __forceinline__ bool choose_groups_warp(const SelectParams& p, const 
       most = fmaxf(most, value[r]);
     }
   }
-  kept = __reduce_or_sync(0xffffffffu, mask[0]);
+  unsigned long long kept = __reduce_or_sync(0xffffffffu, mask[0]);
   if constexpr (R > 1) kept |= static_cast<unsigned long long>(__reduce_or_sync(0xffffffffu, mask[1])) << 32;
-  if (p.bias == nullptr && !p.top2) return true;
   least = of_key(__reduce_min_sync(0xffffffffu, to_key(least)));
   most = of_key(__reduce_max_sync(0xffffffffu, to_key(most)));
-  // (two keys each; groups without a candidate are all behind those with one, in the order of their ids)
-  return least - most > 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total)) || (least == -INFINITY && most == -INFINITY);
+  if (groups_apart(p, least, most, inv_total)) return kept;
+  const float v0 = __shfl_sync(0xffffffffu, value[0], (lane << shift) & 31);
+  return choose_groups_near(p, z, lane << shift < 32 || R > 1 ? v0 : -INFINITY, R > 1 ? value[R - 1] : -INFINITY, least, most, m, inv_total);
 }
 
 template <typename LT, int NV>
 __global__ void __launch_bounds__(32 * kWarpRows)
 select_warp_kernel(const SelectParams p) {
-  __shared__ uint64_t keys[kWarpRows][NV * 33];
+  // keys of the candidates for the groups, or the list of the 64-bit selection
+  constexpr int kWords = NV * 33 * 4 > static_cast<int>(sizeof(BestList)) ? NV * 33 * 4 / 8 + 1 : static_cast<int>(sizeof(BestList) / 8);
+  __shared__ uint64_t keys[kWarpRows][kWords];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * kWarpRows + warp;
-  if (p.clear_load) {
+  if (p.count_here) {
     for (int c = threadIdx.x; c < p.S + p.N; c += 32 * kWarpRows) p.load[c] = 0;
     __syncthreads();
   }
@@ -348,15 +480,13 @@ select_warp_kernel(const SelectParams p) {
       for (int i = 0; i < NV; ++i) sk[lane + 33 * i] = v[i];
     }
     __syncwarp();
-    unsigned long long kept;
     if (p.groups <= 32) {
-      sure = choose_groups_warp<1>(p, sk, inv_total, kept);
-      const uint32_t k32 = static_cast<uint32_t>(kept);
+      const uint32_t k32 = static_cast<uint32_t>(choose_groups_warp<1>(p, sk, zr, m, inv_total));
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (!(k32 >> (div_of(lane + 32 * i, p.per_group) & 31) & 1)) v[i] += -INFINITY;        // (NaN stays)
     } else {
-      sure = choose_groups_warp<2>(p, sk, inv_total, kept);
+      const unsigned long long kept = choose_groups_warp<2>(p, sk, zr, m, inv_total);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (!(kept >> (div_of(lane + 32 * i, p.per_group) & 63) & 1)) v[i] += -INFINITY;
@@ -449,14 +579,22 @@ select_warp_kernel(const SelectParams p) {
       }
       if (__any_sync(0xffffffffu, close)) {
         // again by 64-bit keys: all other candidates are certainly behind the first k of these
-        double t64 = 1.0;
-        if (!p.sigmoid) t64 = warp_total(total64(zr, p.N, m, lane, 32));
-        const uint64_t wide = lane < n ? key64(p, zr, id, m, t64, false) : 0;
-        rank = 0;
-        for (int j = 0; j < n; ++j) {
-          const uint64_t other = __shfl_sync(0xffffffffu, wide, j);
-          const int oid = __shfl_sync(0xffffffffu, id, j);
-          rank += other > wide || (other == wide && oid < id);
+        double t64 = total;
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+          const uint64_t wide = lane < n ? key64(p, zr, id, m, t64, false) : 0;
+          rank = 0;
+          uint64_t next = 0;
+          int nid = -1;
+          for (int j = 0; j < n; ++j) {
+            const uint64_t other = __shfl_sync(0xffffffffu, wide, j);
+            const int oid = __shfl_sync(0xffffffffu, id, j);
+            rank += ahead(other, oid, wide, id);
+            if (ahead(wide, id, other, oid) && (nid < 0 || ahead(other, oid, next, nid))) { next = other; nid = oid; }
+          }
+          const bool unclear = lane < n && rank < p.k && nid >= 0 && !apart64(p, wide, id, next, nid);
+          if (round > 0 || !__any_sync(0xffffffffu, unclear)) break;
+          t64 = warp_total(total64(zr, p.N, m, lane, 32));
         }
       }
       __syncwarp();
@@ -473,14 +611,300 @@ select_warp_kernel(const SelectParams p) {
     }
   }
   if (!sure) {
-    ok = false;
-    choose_warp64(p, zr, m, keys[warp], pick, ok);
+    BestList& list = *reinterpret_cast<BestList*>(keys[warp]);
+    __syncwarp();
+    choose_warp64(p, zr, m, list);
+    pick = lane < p.k ? list.id[lane] : 0;
+    ok = lane < p.k && chosen_from(list.key[lane]);
     chosen = lane < p.k ? logit_of(zr, pick) : 0.f;
   }
   write_row<1>(p, row, m, total, [&](int, bool& good, float& logit) {      // (k <= 32: place j is this lane's)
     good = ok;
     logit = chosen;
     return pick;
+  });
+}
+
+// ---- a warp a row, many rows of many candidates -----------------------------------------------
+// The row streams by (16 loads a lane in flight); what stays of it are the maxima of runs of S candidates a lane, in shared
+// memory.  A bound on those that k + 1 of them reach leaves some dozens of runs, which are read again for the candidates.  No
+// barrier, a third of the instructions of a CTA a row.
+constexpr int kStreamMostK = 64, kStreamHits = 256, kStreamCand = 256, kBatch = 16;
+constexpr int kStreamRows = 600;
+struct StreamShared {
+  union {
+    struct {
+      unsigned long long cand[kStreamCand];
+      uint64_t wide[kStreamCand];
+    };
+    BestList list;
+  };
+  int place[kMostK];
+  uint16_t hits[kStreamHits];
+};
+// (explicit operations: the same number when a run is read again)
+template <bool SIG> __device__ __forceinline__ float stream_score(float z, float m, float inv_total) {
+  return SIG ? fast_sigmoid(z) : __fmul_rn(expf(__fsub_rn(z, m)), inv_total);
+}
+template <bool SIG, bool BIAS> __device__ __forceinline__ float stream_key(float z, float b, float m, float inv_total) {
+  return masked(z) ? -INFINITY : BIAS ? __fadd_rn(stream_score<SIG>(z, m, inv_total), b) : z;
+}
+
+// SIG: sigmoid scores; BIAS: with a balance bias; GROUPS: some groups go.
+template <typename LT, int S, bool SIG, bool BIAS, bool GROUPS>
+__global__ void __launch_bounds__(32 * kWarpRows)
+select_stream_kernel(const SelectParams p, const int chunks) {
+  extern __shared__ uint32_t tops_all[];               // [kWarpRows][chunks][32] keys of the runs' maxima
+  __shared__ StreamShared shared[kWarpRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * kWarpRows + warp;
+  if (row >= p.rows) return;
+  StreamShared& s = shared[warp];
+  uint32_t* tops = tops_all + warp * chunks * 32;
+  const LT* zr = static_cast<const LT*>(p.logits) + row * p.ld + p.S;
+  const float* bias = BIAS ? p.bias + p.S : nullptr;
+  const int groups = GROUPS ? p.groups : 1, per = GROUPS ? p.per : p.N;
+  const int batches = (per + 32 * kBatch - 1) / (32 * kBatch);         // of a group
+  constexpr int kRuns = kBatch / S;                                    // of a batch
+  constexpr uint32_t kNone = 0x007FFFFFu;                              // key of -inf
+
+  float m = 0.f, total = 1.f, inv_total = 1.f;
+  if (!SIG) {                                          // maximum and sum, a lane's own until the end
+    m = -INFINITY;
+    total = 0.f;
+    for (int c0 = lane; c0 < p.N; c0 += 32 * kBatch) {
+      float z[kBatch], most = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) z[i] = c0 + 32 * i < p.N ? logit_of(zr, c0 + 32 * i) : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) most = fmaxf(most, masked(z[i]) ? -INFINITY : z[i]);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) sum += masked(z[i]) ? 0.f : expf(z[i] - most);
+      total = (m == -INFINITY ? total : total * expf(m - most)) + sum;
+      m = most;
+    }
+    const float all = of_key(__reduce_max_sync(0xffffffffu, to_key(m)));
+    total = warp_total(m == -INFINITY ? total : total * expf(m - all));        // (a lane with NaN alone keeps its NaN)
+    m = all;
+    if (total == 0.f) total = 1.f;                     // (every logit masked)
+    inv_total = 1.f / total;
+  }
+
+  bool sure = true;
+  float value[2] = {-INFINITY, -INFINITY};             // of groups lane and lane + 32
+  for (int g = 0; g < groups; ++g) {
+    float a = -INFINITY, b = -INFINITY;
+    for (int bt = 0; bt < batches; ++bt) {
+      const int c0 = bt * 32 * kBatch + lane;          // within the group
+      const LT* zg = zr + static_cast<long long>(g) * per + c0;
+      float z[kBatch], v[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) z[i] = c0 + 32 * i < per ? logit_of(zg, 32 * i) : -INFINITY;
+      if (BIAS) {
+        const float* bg = bias + g * per + c0;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) v[i] = c0 + 32 * i < per ? bg[32 * i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) v[i] = stream_key<SIG, BIAS>(z[i], BIAS ? v[i] : 0.f, m, inv_total);
+#pragma unroll
+      for (int q = 0; q < kRuns; ++q) {
+        float top = v[q * S];
+#pragma unroll
+        for (int i = 1; i < S; ++i) top = max_nan(top, v[q * S + i]);
+        tops[((g * batches + bt) * kRuns + q) * 32 + lane] = to_key(top);
+      }
+      if (GROUPS) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          float u = v[i];
+          if (!BIAS && p.top2) u = masked(z[i]) ? -INFINITY : stream_score<SIG>(z[i], m, inv_total);
+          b = fmaxf(b, fminf(a, u));
+          a = fmaxf(a, u);
+        }
+      }
+    }
+    if (GROUPS) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+        b = fmaxf(fminf(a, oa), fmaxf(b, ob));
+        a = fmaxf(a, oa);
+      }
+      if (lane == (g & 31)) value[g >> 5] = p.top2 && b > -INFINITY ? a + b : a;
+    }
+  }
+  if (GROUPS) {
+    int rank[2] = {0, 0};
+    for (int g = 0; g < groups; ++g) {
+      const float other = __shfl_sync(0xffffffffu, value[g >> 5], g & 31);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) rank[r] += other > value[r] || (other == value[r] && g < lane + 32 * r);
+    }
+    float least = INFINITY, most = -INFINITY;          // of those that stay, of those that go
+    uint32_t stays[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool real = lane + 32 * r < groups, in = real && rank[r] < p.keep;
+      stays[r] = __ballot_sync(0xffffffffu, in);
+      if (in) least = fminf(least, value[r]);
+      else if (real) most = fmaxf(most, value[r]);
+    }
+    least = of_key(__reduce_min_sync(0xffffffffu, to_key(least)));
+    most = of_key(__reduce_max_sync(0xffffffffu, to_key(most)));
+    if (!groups_apart(p, least, most, inv_total)) {
+      const unsigned long long kept = choose_groups_near(p, zr, value[0], value[1], least, most, m, inv_total);
+      stays[0] = static_cast<uint32_t>(kept);
+      stays[1] = static_cast<uint32_t>(kept >> 32);
+    }
+    for (int i = 0; i < chunks; ++i) {
+      const int g = i / (batches * kRuns);
+      // (NaN stays to be seen)
+      if (!((g < 32 ? stays[0] >> g : stays[1] >> (g - 32)) & 1) && tops[i * 32 + lane] != 0xFFFFFFFFu) tops[i * 32 + lane] = kNone;
+    }
+  }
+
+  // the bound
+  uint32_t lo = 0xFFFFFFFFu, hi = 0;
+  int some = 0;
+  for (int i = 0; i < chunks; ++i) {
+    const uint32_t key = tops[i * 32 + lane];
+    hi = max(hi, key);
+    if (key > kNone) { ++some; lo = min(lo, key); }
+  }
+  some = __reduce_add_sync(0xffffffffu, some);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  const int need = min(p.k + 1, p.N);
+  int n = 0;
+  if (some == 0) {                                     // nothing to choose from: the lowest ids
+    for (int j = lane; j < p.k; j += 32) s.place[j] = ~j;
+  } else if (hi == 0xFFFFFFFFu || some < need) {
+    sure = false;                                      // NaN, or candidates in too few runs
+  } else if (sure) {
+    while (lo < hi) {                                  // count(>= lo) >= need, count(> hi) == 0
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      int count = 0;
+#pragma unroll 8
+      for (int i = 0; i < chunks; ++i) count += tops[i * 32 + lane] >= mid;
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (count >= need) {
+        lo = mid;
+        if (count <= need + need / 4 + 2) break;
+      } else {
+        hi = mid - 1;
+      }
+    }
+    float edge = of_key(lo);
+    if (BIAS) edge -= 2.f * key_error(p, edge, inv_total);       // what may yet turn out to reach the bound
+    const uint32_t from = to_key(edge);
+    int runs = 0;
+    for (int i = 0; i < chunks; ++i) {
+      const bool hit = tops[i * 32 + lane] >= from;
+      const uint32_t votes = __ballot_sync(0xffffffffu, hit);
+      const int pos = runs + __popc(votes & ((1u << lane) - 1u));
+      if (hit && pos < kStreamHits) s.hits[pos] = static_cast<uint16_t>(i * 32 + lane);
+      runs += __popc(votes);
+    }
+    __syncwarp();
+    sure = runs <= kStreamHits && edge < INFINITY;
+    if (sure) {
+      for (int h = 0; h < runs; h += 32 / S) {
+        const int j = h + lane / S;
+        const int run = j < runs ? s.hits[j] : 0, i = run >> 5;
+        const int bt = i / kRuns, g = GROUPS ? bt / batches : 0;
+        const int c = ((bt - g * batches) * kBatch + (i - bt * kRuns) * S + lane % S) * 32 + (run & 31);     // within the group
+        float v = -INFINITY;
+        if (j < runs && c < per) v = stream_key<SIG, BIAS>(logit_of(zr, static_cast<long long>(g) * per + c), BIAS ? bias[g * per + c] : 0.f, m, inv_total);
+        const bool in = v >= edge && v > -INFINITY;
+        const uint32_t votes = __ballot_sync(0xffffffffu, in);
+        const int pos = n + __popc(votes & ((1u << lane) - 1u));
+        if (in && pos < kStreamCand) s.cand[pos] = static_cast<unsigned long long>(to_key(v)) << 32 | ~static_cast<uint32_t>(g * per + c);
+        n += __popc(votes);
+      }
+      __syncwarp();
+      sure = n <= kStreamCand && n >= min(need, p.k);
+    }
+  }
+  if (sure && some > 0) {
+    if (n > need + 16) {                               // a closer bound, from the candidates themselves
+      uint32_t key[kStreamCand / 32];
+      uint32_t l = 0xFFFFFFFFu, u = 0;
+#pragma unroll
+      for (int q = 0; q < kStreamCand / 32; ++q) {
+        key[q] = lane + 32 * q < n ? static_cast<uint32_t>(s.cand[lane + 32 * q] >> 32) : 0u;
+        u = max(u, key[q]);
+        if (key[q] != 0) l = min(l, key[q]);
+      }
+      u = __reduce_max_sync(0xffffffffu, u);
+      l = __reduce_min_sync(0xffffffffu, l);
+      while (l < u) {
+        const uint32_t mid = l + (u - l + 1) / 2;
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < kStreamCand / 32; ++q) count += key[q] >= mid;
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (count >= need) {
+          l = mid;
+          if (count <= need + 4) break;
+        } else {
+          u = mid - 1;
+        }
+      }
+      float edge = of_key(l);
+      if (BIAS) edge -= 2.f * key_error(p, edge, inv_total);
+      const uint32_t from = to_key(edge);
+      int left = 0;
+#pragma unroll
+      for (int q = 0; q < kStreamCand / 32; ++q) {
+        const unsigned long long mine = lane + 32 * q < n ? s.cand[lane + 32 * q] : 0;
+        const bool in = key[q] >= from;
+        const uint32_t votes = __ballot_sync(0xffffffffu, in);        // (every lane has read its entry of this round)
+        if (in) s.cand[left + __popc(votes & ((1u << lane) - 1u))] = mine;
+        left += __popc(votes);
+        __syncwarp();
+      }
+      n = left;
+    }
+    bool close = false;
+    for (int t = lane; t < n; t += 32) {
+      const unsigned long long mine = s.cand[t];
+      unsigned long long next = 0;                     // the largest below it
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const unsigned long long o = s.cand[j];
+        rank += o > mine;
+        if (BIAS && o < mine && o > next) next = o;
+      }
+      if (rank < p.k) {
+        s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
+        if (BIAS && next != 0 &&
+            !apart(p, of_key(static_cast<uint32_t>(mine >> 32)), of_key(static_cast<uint32_t>(next >> 32)), inv_total)) close = true;
+      }
+    }
+    if (BIAS && __any_sync(0xffffffffu, close)) {      // again by 64-bit keys
+      double t64 = total;
+#pragma unroll 1
+      for (int round = 0; round < 2; ++round) {
+        for (int t = lane; t < n; t += 32) s.wide[t] = key64(p, zr, static_cast<int>(~static_cast<uint32_t>(s.cand[t])), m, t64, false);
+        __syncwarp();
+        if (!__any_sync(0xffffffffu, rank_wide(p, s.cand, s.wide, n, lane, 32, s.place)) || round > 0) break;
+        t64 = warp_total(total64(zr, p.N, m, lane, 32));
+      }
+    }
+  } else if (!sure) {
+    __syncwarp();
+    choose_warp64(p, zr, m, s.list);
+    for (int j = lane; j < p.k; j += 32) s.place[j] = chosen_from(s.list.key[j]) ? s.list.id[j] : ~s.list.id[j];
+  }
+  __syncwarp();
+  write_row<kStreamMostK / 32>(p, row, m, total, [&](int j, bool& good, float& logit) {
+    const int at = s.place[j], id = at >= 0 ? at : ~at;
+    good = at >= 0;
+    logit = logit_of(zr, id);
+    return id;
   });
 }
 
@@ -535,9 +959,9 @@ __device__ __noinline__ void choose_groups64(const SelectParams& p, CtaShared& s
   }
   __syncthreads();
 }
-// The same from fp32 keys; s.unsure where they cannot tell.
-template <int TH>
-__device__ __forceinline__ void choose_groups(const SelectParams& p, CtaShared& s, const float* keys, float inv_total) {
+// The same from fp32 keys, 64 bits where those close: 0 for a group that stays and -inf for one that goes, behind the values.
+template <int TH, typename LT>
+__device__ __forceinline__ void choose_groups(const SelectParams& p, CtaShared& s, const float* keys, const LT* z, float m, float inv_total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* values = reinterpret_cast<float*>(s.group);
   for (int g = warp; g < p.groups; g += TH / 32) {
@@ -569,9 +993,11 @@ __device__ __forceinline__ void choose_groups(const SelectParams& p, CtaShared& 
     }
     least = of_key(__reduce_min_sync(0xffffffffu, to_key(least)));
     most = of_key(__reduce_max_sync(0xffffffffu, to_key(most)));
-    const bool sure = (p.bias == nullptr && !p.top2) || (least == -INFINITY && most == -INFINITY) ||
-                      least - most > 2.f * (key_error(p, least, inv_total) + key_error(p, most, inv_total));
-    if (lane == 0 && !sure) s.unsure = 1;
+    if (!groups_apart(p, least, most, inv_total)) {
+      const unsigned long long kept = choose_groups_near(p, z, lane < p.groups ? values[lane] : -INFINITY,
+                                                         lane + 32 < p.groups ? values[lane + 32] : -INFINITY, least, most, m, inv_total);
+      for (int g = lane; g < p.groups; g += 32) values[kMostGroups + g] = kept >> g & 1 ? 0.f : -INFINITY;
+    }
   }
   __syncthreads();
 }
@@ -629,7 +1055,7 @@ select_cta_kernel(const SelectParams p) {
   __shared__ CtaShared s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = blockIdx.x;
-  if (p.clear_load)                        // (many barriers before the first count)
+  if (p.count_here)                        // (many barriers before the first count)
     for (int c = threadIdx.x; c < p.S + p.N; c += TH) p.load[c] = 0;
   const LT* zr = static_cast<const LT*>(p.logits) + row * p.ld + p.S;
   const bool biased = p.bias != nullptr, grouped = p.keep < p.groups, judged = grouped && p.top2 && !biased;
@@ -693,7 +1119,7 @@ select_cta_kernel(const SelectParams p) {
         if (threadIdx.x + TH * i < p.N) sk[threadIdx.x + TH * i] = v[i];
     }
     __syncthreads();
-    choose_groups<TH>(p, s, sk, inv_total);
+    choose_groups<TH>(p, s, sk, zr, m, inv_total);
     const float* off = reinterpret_cast<const float*>(s.group) + kMostGroups;          // 0 where the group stays, else -inf
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] += off[min(div_of(threadIdx.x + TH * i, p.per_group), kMostGroups - 1)];     // (NaN stays)
@@ -781,18 +1207,14 @@ select_cta_kernel(const SelectParams p) {
       }
       __syncthreads();
       if (s.close) {                                // the candidates again by 64-bit keys
-        double t64 = 1.0;
-        if (!p.sigmoid) t64 = cta_total<double, TH>(total64(zr, p.N, m, threadIdx.x, TH), s.red);
-        for (int t = threadIdx.x; t < n; t += TH) keys[t] = key64(p, zr, static_cast<int>(~static_cast<uint32_t>(s.cand[t])), m, t64, false);
-        __syncthreads();
-        for (int t = threadIdx.x; t < n; t += TH) {
-          const uint64_t mine = keys[t];
-          const uint32_t id = ~static_cast<uint32_t>(s.cand[t]);
-          int rank = 0;
-          for (int j = 0; j < n; ++j) rank += keys[j] > mine || (keys[j] == mine && ~static_cast<uint32_t>(s.cand[j]) < id);
-          if (rank < p.k) s.place[rank] = static_cast<int>(id);
+        double t64 = total;
+#pragma unroll 1
+        for (int round = 0; round < 2; ++round) {
+          for (int t = threadIdx.x; t < n; t += TH) keys[t] = key64(p, zr, static_cast<int>(~static_cast<uint32_t>(s.cand[t])), m, t64, false);
+          __syncthreads();
+          if (!__syncthreads_or(rank_wide(p, s.cand, keys, n, threadIdx.x, TH, s.place)) || round > 0) break;
+          t64 = cta_total<double, TH>(total64(zr, p.N, m, threadIdx.x, TH), s.red);
         }
-        __syncthreads();
       }
     }
   }
@@ -893,6 +1315,33 @@ select_bwd_kernel(const SelectGrads p) {
     }
 }
 
+// load[c] = how many of the `n` picks are c, by one cluster of kLoadCtas CTAs: each counts its share in shared memory, then adds up
+// a share of the chapters over all of them.  (Counted by the selecting CTAs with atomics in global memory, 65,536 picks among 64
+// chapters took 30 us: the counters share two cache lines.)
+constexpr int kLoadCtas = 8;
+__global__ void __launch_bounds__(1024)
+select_load_kernel(const long long* __restrict__ idx, long long n, int C, int* __restrict__ load) {
+  extern __shared__ int counts[];          // [C]
+  const int rank = blockIdx.x;
+  for (int c = threadIdx.x; c < C; c += 1024) counts[c] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (long long i = rank * 1024 + threadIdx.x; i < n; i += kLoadCtas * 1024) atomicAdd(counts + static_cast<int>(idx[i]), 1);
+  cluster_sync();
+  const uint32_t base = smem_u32(counts);
+  for (int c = rank * 1024 + threadIdx.x; c < C; c += kLoadCtas * 1024) {
+    int sum = 0;
+#pragma unroll
+    for (int r = 0; r < kLoadCtas; ++r) {
+      int v;
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_map(base + c * 4, r)));
+      sum += v;
+    }
+    load[c] = sum;
+  }
+  cluster_sync();                          // nobody leaves while its counts are read
+}
+
 __global__ void balance_bias_kernel(float* __restrict__ bias, const int* __restrict__ load, int C, int S, float rate) {
   __shared__ double red[32];
   double n = 0.0;
@@ -914,7 +1363,7 @@ int check(const moc_select_shape* s) {
   MOC_REQUIRE(s->rows > 0 && s->num_chapters > 0 && s->num_shared >= 0 && s->num_shared < s->num_chapters,
               "rows must be positive and num_shared leave a chapter to choose from");
   const int n = s->num_chapters - s->num_shared;
-  MOC_REQUIRE(n <= kMostN, "at most 16384 chapters to choose from");
+  MOC_REQUIRE(n <= kMostN && s->num_shared <= kMostN, "at most 16384 chapters to choose from, and as many shared ones");
   MOC_REQUIRE(s->num_groups >= 1 && s->num_groups <= kMostGroups && n % s->num_groups == 0,
               "num_groups must divide the chapters to choose from and be at most 64");
   MOC_REQUIRE(s->top_groups >= 1 && s->top_groups <= s->num_groups, "top_groups must be in 1..num_groups");
@@ -926,16 +1375,33 @@ int check(const moc_select_shape* s) {
   return MOC_OK;
 }
 
+template <typename LT, int S> int select_stream(const SelectParams& p, cudaStream_t stream) {
+  const bool grouped = p.keep < p.groups, biased = p.bias != nullptr;
+  const int per = grouped ? p.per : p.N;
+  const int chunks = (grouped ? p.groups : 1) * ((per + 32 * kBatch - 1) / (32 * kBatch)) * (kBatch / S);
+  auto kern = grouped ? (p.sigmoid ? (biased ? select_stream_kernel<LT, S, true, true, true> : select_stream_kernel<LT, S, true, false, true>)
+                                   : (biased ? select_stream_kernel<LT, S, false, true, true> : select_stream_kernel<LT, S, false, false, true>))
+                      : (p.sigmoid ? (biased ? select_stream_kernel<LT, S, true, true, false> : select_stream_kernel<LT, S, true, false, false>)
+                                   : (biased ? select_stream_kernel<LT, S, false, true, false> : select_stream_kernel<LT, S, false, false, false>));
+  const size_t bytes = static_cast<size_t>(kWarpRows) * chunks * 128;
+  MOC_CUDA_OK(allow_shared(kern, bytes, 128 * 1024));
+  kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, bytes, stream>>>(p, chunks);
+  MOC_CUDA_OK(cudaGetLastError());
+  return MOC_OK;
+}
 template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream) {
+  const bool grouped = p.keep < p.groups;
   if (p.N <= kWarpMostN && p.k <= kWarpMostK) {
     auto kern = p.N <= 64 ? select_warp_kernel<LT, 2> : p.N <= 128 ? select_warp_kernel<LT, 4>
                 : p.N <= 256 ? select_warp_kernel<LT, 8> : select_warp_kernel<LT, 16>;
     kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, 0, stream>>>(p);
+  } else if (p.rows >= kStreamRows && p.k <= kStreamMostK && p.N > kWarpMostN && (!grouped || p.per >= 256)) {
+    return p.N > 2048 ? select_stream<LT, 16>(p, stream) : select_stream<LT, 4>(p, stream);
   } else {
     const bool big = p.N > 4096;
     auto kern = p.N <= 1024 ? select_cta_kernel<LT, 4, 256> : p.N <= 2048 ? select_cta_kernel<LT, 8, 256>
                 : !big ? select_cta_kernel<LT, 16, 256> : p.N <= 8192 ? select_cta_kernel<LT, 8, 1024> : select_cta_kernel<LT, 16, 1024>;
-    if (p.N > 4096) MOC_CUDA_OK(allow_shared(kern, static_cast<size_t>(p.N) * 8, kMostN * 8));      // (48 KB need no leave)
+    if (big) MOC_CUDA_OK(allow_shared(kern, static_cast<size_t>(p.N) * 8, kMostN * 8));      // (48 KB need no leave)
     kern<<<p.rows, big ? 1024 : 256, static_cast<size_t>(p.N) * 8, stream>>>(p);
   }
   MOC_CUDA_OK(cudaGetLastError());
@@ -969,9 +1435,14 @@ extern "C" int moc_select_fwd(const moc_select_shape* s, const void* logits, con
   p.per_group = fast_div(p.per);
   p.sigmoid = s->score == MOC_SCORE_SIGMOID; p.top2 = s->group_top2 != 0; p.renorm = s->renormalize != 0; p.rho = s->routed_scale;
   const bool warps = p.N <= kWarpMostN && p.k <= kWarpMostK;
-  p.clear_load = load != nullptr && p.rows <= (warps ? kWarpRows : 1);
-  if (load != nullptr && !p.clear_load) MOC_CUDA_OK(cudaMemsetAsync(load, 0, static_cast<size_t>(s->num_chapters) * sizeof(int32_t), stream));
-  return s->dtype == MOC_F32 ? select_fwd<float>(p, stream) : select_fwd<__nv_bfloat16>(p, stream);
+  p.count_here = load != nullptr && p.rows <= (warps ? kWarpRows : 1);
+  const int done = s->dtype == MOC_F32 ? select_fwd<float>(p, stream) : select_fwd<__nv_bfloat16>(p, stream);
+  if (done != MOC_OK || load == nullptr || p.count_here) return done;
+  const size_t bytes = static_cast<size_t>(s->num_chapters) * sizeof(int32_t);
+  if (bytes > 48 * 1024) MOC_CUDA_OK(allow_shared(select_load_kernel, bytes, kSharedMost));
+  MOC_CUDA_OK(launch_clustered(select_load_kernel, dim3(kLoadCtas), 1024, static_cast<int>(bytes), kLoadCtas, stream,
+                               static_cast<const long long*>(p.idx), static_cast<long long>(p.rows) * p.k, s->num_chapters, load));
+  return MOC_OK;
 }
 
 extern "C" int moc_select_bwd(const moc_select_shape* s, const void* logits, const int64_t* idx, const float* weights,

@@ -106,6 +106,27 @@ def test_selection_and_gradient(rows, c, k, shared, groups, keep, top2, biased, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("c, k, shared, groups, keep, top2", [
+    (513, 1, 0, 1, 1, False), (514, 64, 1, 1, 1, False), (1026, 16, 2, 4, 2, True), (2049, 64, 1, 8, 3, False), (2050, 8, 1, 1, 1, False),
+    (4097, 16, 1, 8, 4, True), (4097, 64, 1, 1, 1, False), (4100, 5, 3, 17, 2, True), (8200, 33, 8, 32, 7, True), (16385, 64, 1, 64, 9, True),
+    (16384, 20, 0, 1, 1, False), (700, 31, 0, 2, 1, True)])
+def test_many_rows(c, k, shared, groups, keep, top2, biased, score):
+    """Numbers of rows at which a warp takes a row of a large bank, some of them masked, equal, or with one candidate."""
+    rows = 613
+    z, b = _logits(rows, c, c + k), _bias(c, c) if biased else None
+    z[5], z[6], z[7, 1:] = float("-inf"), 0.5, torch.finfo(torch.float32).min
+    z[8, ::3] = float("-inf")
+    z[9, c // 2:] = float("-inf")
+    z[10] = z[10].bfloat16().float()
+    _compare(z, b, k, score, shared, groups, keep, top2)
+    _compare(z.bfloat16(), b, k, score, shared, groups, keep, top2, False, grad=False)
+    if biased:
+        _compare(z, torch.zeros(c, device="cuda"), k, score, shared, groups, keep, top2, grad=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("c, k, groups, keep", [(65, 8, 1, 1), (257, 8, 8, 4), (4097, 16, 8, 4), (4097, 64, 1, 1)])
 def test_bf16_logits_with_ties(c, k, groups, keep):
     """bf16 logits hold equal values, so the order among them is that of the ids; the bias makes near ties that only 64 bits part."""
@@ -116,11 +137,13 @@ def test_bf16_logits_with_ties(c, k, groups, keep):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [50, 700])
 @pytest.mark.parametrize("c", [64, 300, 1500, 4096, 6000])
-def test_near_ties_are_told_apart(c):
+def test_near_ties_are_told_apart(c, rows):
     """Sums that fp32 cannot order: scores and biases that cancel to differences around 1e-9."""
     g = torch.Generator(device="cuda").manual_seed(7)
-    z = torch.randn(50, c, generator=g, device="cuda")
+    z = torch.randn(rows, c, generator=g, device="cuda")
+    z[1:4] = z[0]
     for score in ("softmax", "sigmoid"):
         s = torch.sigmoid(z[0].double()) if score == "sigmoid" else torch.softmax(z[0].double(), 0)
         b = (0.9 - s + 1e-9 * torch.randn(c, generator=g, device="cuda", dtype=torch.float64)).float()
@@ -152,20 +175,20 @@ def test_equal_and_masked_rows(c, k, score):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("c", [50, 4096])
-def test_nan_and_infinite_logits_show_and_stay_in_range(c):
+@pytest.mark.parametrize("c, rows", [(50, 3), (4096, 3), (4096, 700)])
+def test_nan_and_infinite_logits_show_and_stay_in_range(c, rows):
     import memory_b200 as M
-    z = _logits(3, c, 1)
+    z = _logits(rows, c, 1)
     z[0, 7], z[1, 9] = float("nan"), float("inf")
     for b in (None, _bias(c, 1)):
         got = M.select_chapters(z, 5, score="sigmoid", balance_bias=b)
         assert got.weights[0].isnan().all() and got.indices[0, 0] == 7
         assert got.weights[1].isfinite().all() and (b is not None or got.indices[1, 0] == 9)
         soft = M.select_chapters(z, 5, balance_bias=b)
-        assert soft.weights[:2].isnan().all() and soft.weights[2].isfinite().all()
+        assert soft.weights[:2].isnan().all() and soft.weights[2:].isfinite().all()
         for s in (got, soft):
             assert ((s.indices >= 0) & (s.indices < c)).all()
-            assert all(len(set(r.tolist())) == 5 for r in s.indices)
+            assert all(len(set(r.tolist())) == 5 for r in s.indices[:5])
 
 
 @pytest.mark.gpu
