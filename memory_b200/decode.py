@@ -139,7 +139,9 @@ class ProjectedBankCache:
             raise ValueError("chapter_indices and chapter_weights must both be [B, n]")
         if counts is not None and tuple(counts.shape) != (b,):
             raise ValueError("counts must be [B]")
-        if any(t is not None and t.device != self.kv_bank.device for t in (q, chapter_indices, chapter_weights, counts)):
+        device = self.kv_bank.device
+        if q.device != device or chapter_indices.device != device or chapter_weights.device != device or (
+                counts is not None and counts.device != device):
             raise ValueError("all tensors must be on the device of the cache")
         if b == 0 or n_q == 0 or chapter_indices.shape[1] == 0:
             out, lse = torch.zeros_like(q), q.new_full((b, n_q, heads), float("-inf"), dtype=torch.float32)

@@ -949,7 +949,11 @@ def _differentiated(*tensors) -> bool:
     """Whether autograd has to see a call on these tensors (forward-mode gradients included, which it then refuses)."""
     if forward_ad._current_level >= 0:
         return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _Select(torch.autograd.Function):

@@ -4,8 +4,9 @@ Every function requires CUDA tensors; nothing here computes on the host.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+from array import array
+from operator import attrgetter
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -18,14 +19,6 @@ def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if t is None else (t if t.is_contiguous() else t.contiguous())
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch where it is not: a stream belongs to its device."""
-    return _HERE if torch._C._cuda_getDevice() == L.device_index(device) else torch.cuda.device(device)
-
-
 # Kernel-launch accounting and optional per-call CUDA-event timing (used by the benchmark).  A kernel that leaves at once because the
 # call's chapters are the other one's (the token mixture asks them on the device) does not count.
 LAUNCHES = 0
@@ -34,6 +27,24 @@ LAUNCH_HOOK = None   # when callable: called with "<operator>:<bf16|f32|...>" fo
                      # assert which arithmetic path ran)
 
 _DTYPE_TAG = {torch.bfloat16: "bf16", torch.float32: "f32", torch.float16: "f16"}
+
+
+def _issue(name: str, tag: str, launches: int, device: torch.device, args) -> None:
+    """Calls the C entry ``moc_<name>`` with ``args`` and the current stream of ``device`` (which is made current where it is not:
+    a stream belongs to its device), and accounts for it as :func:`_instrument` does."""
+    global LAUNCHES
+    fn = getattr(L.lib(), "moc_" + name)
+    index = L.device_index(device)
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _issue(name, tag, launches, device, args)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    rc = fn(*args, stream) if TIMER is None else _timed(name, lambda: fn(*args, stream))
+    if rc:
+        L.check(rc, "moc_" + name)
+    LAUNCHES += launches
+    if LAUNCH_HOOK is not None:
+        LAUNCH_HOOK(f"{name}:{tag}")
 
 
 def _instrument(name: str, launches):
@@ -304,13 +315,9 @@ def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, wa
     comb_w = torch.empty((rows, joint), dtype=f32, device=dev)
     load = torch.empty(s.num_chapters, dtype=i32, device=dev)
     stats = torch.empty((rows, 4), dtype=f32, device=dev) if want_stats else None
-    with _on(dev):
-        args = (C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(),
-                comb_w.data_ptr(), L.ptr(stats), load.data_ptr(), L.stream_ptr(dev))
-        rc = L.lib().moc_select_fwd(*args) if TIMER is None else _timed("select_fwd", lambda: L.lib().moc_select_fwd(*args))
-    if rc:
-        L.check(rc, "moc_select_fwd")
-    _report(1, lambda: ("select_fwd:" + _DTYPE_TAG[logits.dtype],))
+    _issue("select_fwd", _DTYPE_TAG[logits.dtype], 2 if rows > 4 else 1, dev,
+           (C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(), comb_w.data_ptr(),
+            L.ptr(stats), load.data_ptr()))
     return idx, weights, comb_idx, comb_w, load, stats
 
 
@@ -318,17 +325,12 @@ def select_bwd(logits: torch.Tensor, s, idx, weights, comb_w, stats, g_weights, 
     """Gradient of the logits [rows, C] (dense, their type) from those of the weights and the joint weights (either may be None)."""
     dev = logits.device
     d = torch.empty((s.rows, s.num_chapters), dtype=logits.dtype, device=dev)
-    with _on(dev):
-        args = (C.byref(s), logits.data_ptr(), idx.data_ptr(), weights.data_ptr(), comb_w.data_ptr(), stats.data_ptr(),
-                L.ptr(g_weights), L.ptr(g_comb), d.data_ptr(), L.stream_ptr(dev))
-        rc = L.lib().moc_select_bwd(*args) if TIMER is None else _timed("select_bwd", lambda: L.lib().moc_select_bwd(*args))
-    if rc:
-        L.check(rc, "moc_select_bwd")
-    _report(1, lambda: ("select_bwd:" + _DTYPE_TAG[logits.dtype],))
+    _issue("select_bwd", _DTYPE_TAG[logits.dtype], 1, dev,
+           (C.byref(s), logits.data_ptr(), idx.data_ptr(), weights.data_ptr(), comb_w.data_ptr(), stats.data_ptr(), L.ptr(g_weights),
+            L.ptr(g_comb), d.data_ptr()))
     return d
 
 
-@_instrument("balance_bias_step", 1)
 def balance_bias_step(bias: torch.Tensor, load: torch.Tensor, num_shared: int, rate: float) -> None:
     """bias[c] += rate * sign(mean load - load[c]) in place over the chapters behind the shared ones."""
     L.require_cuda(bias, load)
@@ -336,9 +338,7 @@ def balance_bias_step(bias: torch.Tensor, load: torch.Tensor, num_shared: int, r
         raise TypeError("the balance bias must be a contiguous fp32 vector")
     if load.dtype != torch.int32 or load.shape != bias.shape or load.device != bias.device or not load.is_contiguous():
         raise ValueError("load must be int32 counts shaped like the bias, on its device")
-    with _on(bias.device):
-        L.check(L.lib().moc_balance_bias_step(L.ptr(bias), L.ptr(load), bias.numel(), int(num_shared), float(rate),
-                                              L.stream_ptr(bias.device)), "moc_balance_bias_step")
+    _issue("balance_bias_step", "f32", 1, bias.device, (bias.data_ptr(), load.data_ptr(), bias.numel(), int(num_shared), float(rate)))
 
 
 # --------------------------------------------------------------------------------------------
@@ -589,30 +589,28 @@ def bank_adamw_step(param: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torc
 _GRAD_DTYPES = {torch.float32: L.MOC_F32, torch.bfloat16: L.MOC_BF16, torch.float16: L.MOC_F16}
 
 
-def grad_clip(grads, out, banks, max_norm: float, eps: float, device: torch.device) -> torch.Tensor:
-    """``moc_grad_clip`` on dense, contiguous ``grads`` and the tensors ``out`` that receive them clipped (or the gradients
-    themselves), and on compact rows ``banks``: (rows, count, elements of a unit, weight), which count in the norm alone.  Returns
-    [2] fp32 = (norm, coefficient)."""
+_data_ptr, _numel, _dtype = torch.Tensor.data_ptr, torch.Tensor.numel, attrgetter("dtype")
+
+
+def grad_clip(grads, ptrs, out, banks, max_norm: float, eps: float, device: torch.device) -> torch.Tensor:
+    """``moc_grad_clip`` on dense, contiguous ``grads`` (at ``ptrs``) and the tensors ``out`` that receive them clipped (or the
+    gradients themselves), and on compact rows ``banks``: (rows, count, elements of a unit, weight), which count in the norm alone.
+    Returns [2] fp32 = (norm, coefficient)."""
     n, m = len(grads), len(banks)
-    codes, lib = _GRAD_DTYPES, L.lib()
-    total = n + m
-    # one column of the table per list comprehension: a third of the time of a loop over the tensors
-    ptrs = [g.data_ptr() for g in grads] + [b[0].data_ptr() for b in banks]
-    sizes = [g.numel() for g in grads] + [b[0].numel() for b in banks]
-    types = [codes[g.dtype] for g in grads] + [codes[b[0].dtype] for b in banks]
+    codes, total = _GRAD_DTYPES.__getitem__, len(grads) + len(banks)
+    tensors = [*grads, *(b[0] for b in banks)]
+    # the columns of the table, without a Python step per tensor
+    grad_ptrs = array("Q", [*ptrs, *(b[0].data_ptr() for b in banks)])
+    sizes, types = array("q", map(_numel, tensors)), array("B", map(codes, map(_dtype, tensors)))
     same = out is grads
-    outs = ptrs[:n] if same else [o.data_ptr() for o in out]
-    out_types = types[:n] if same else [codes[o.dtype] for o in out]
+    outs, out_types = (grad_ptrs, types) if same else (array("Q", map(_data_ptr, out)), array("B", map(codes, map(_dtype, out))))
+    counts, units = array("Q", [b[1].data_ptr() for b in banks]), array("i", [b[2] for b in banks])
+    weights = array("f", [b[3] for b in banks])
     result = torch.empty(2, dtype=torch.float32, device=device)
-    ws = torch.empty(lib.moc_grad_clip_workspace_bytes(total), dtype=torch.uint8, device=device)
-    with _on(device):
-        args = (total, n, (C.c_void_p * total)(*ptrs), (C.c_int64 * total)(*sizes), (C.c_uint8 * total)(*types),
-                (C.c_void_p * n)(*outs), (C.c_uint8 * n)(*out_types), (C.c_void_p * m)(*[b[1].data_ptr() for b in banks]),
-                (C.c_int32 * m)(*[b[2] for b in banks]), (C.c_float * m)(*[b[3] for b in banks]), float(max_norm), float(eps),
-                result.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(device))
-        rc = lib.moc_grad_clip(*args) if TIMER is None else _timed("grad_clip", lambda: lib.moc_grad_clip(*args))
-    L.check(rc, "moc_grad_clip")
-    _report(2 * (1 if total <= 64 else -(-total // 680)), lambda: ("grad_clip:-",))
+    ws = torch.empty(L.lib().moc_grad_clip_workspace_bytes(total), dtype=torch.uint8, device=device)
+    at = [a.buffer_info()[0] for a in (grad_ptrs, sizes, types, outs, out_types, counts, units, weights)]
+    _issue("grad_clip", "-", 2 * (1 if total <= 64 else -(-total // 680)), device,
+           (total, n, *at, float(max_norm), float(eps), result.data_ptr(), ws.data_ptr(), ws.numel()))
     return result
 
 
@@ -1313,37 +1311,26 @@ def gated_residual_fwd(s, x, f, weight, bias, gate, next_weight, next_bias, want
     y = torch.empty_like(x)
     n = torch.empty_like(f) if next_weight is not None else None
     stats = torch.empty((s.rows, 4), dtype=torch.float32, device=dev) if want_stats else None
-    with _on(dev):
-        args = (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), p(next_bias), y.data_ptr(),
-                p(n), p(stats), L.stream_ptr(dev))
-        rc = (L.lib().moc_gated_residual_fwd(*args) if TIMER is None
-              else _timed("gated_residual_fwd", lambda: L.lib().moc_gated_residual_fwd(*args)))
-    if rc:
-        L.check(rc, "moc_gated_residual_fwd")
-    _report(1, lambda: ("gated_residual_fwd:" + _DTYPE_TAG[x.dtype],))
+    _issue("gated_residual_fwd", _DTYPE_TAG[x.dtype], 1, dev,
+           (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), p(next_bias), y.data_ptr(), p(n),
+            p(stats)))
     return y, n, stats
 
 
 def gated_residual_bwd(s, x, f, weight, bias, gate, next_weight, stats, d_y, d_n, want_dx: bool, want_bias: bool,
                        want_next_bias: bool):
     """Gradients of :func:`gated_residual_fwd`: (d_x or None, d_f, d_weight, d_bias, d_gate, d_next_weight, d_next_bias)."""
-    dev, p, lib = x.device, L.ptr, L.lib()
+    dev, p = x.device, L.ptr
     d_x = torch.empty_like(x) if want_dx else None
     d_f = torch.empty_like(f)
     d_w, d_gate = torch.empty_like(weight), None if gate is None else torch.empty_like(gate)
     d_b = torch.empty_like(weight) if want_bias else None
     d_nw = None if next_weight is None else torch.empty_like(weight)
     d_nb = torch.empty_like(weight) if want_next_bias else None
-    with _on(dev):
-        scratch = torch.empty(lib.moc_gated_residual_bwd_scratch_bytes(C.byref(s), int(gate is not None)), dtype=torch.uint8, device=dev)
-        args = (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), stats.data_ptr(), p(d_y),
-                p(d_n), p(d_x), d_f.data_ptr(), d_w.data_ptr(), p(d_b), p(d_gate), p(d_nw), p(d_nb), scratch.data_ptr(),
-                L.stream_ptr(dev))
-        rc = (lib.moc_gated_residual_bwd(*args) if TIMER is None
-              else _timed("gated_residual_bwd", lambda: lib.moc_gated_residual_bwd(*args)))
-    if rc:
-        L.check(rc, "moc_gated_residual_bwd")
-    _report(2, lambda: ("gated_residual_bwd:" + _DTYPE_TAG[x.dtype],))
+    scratch = torch.empty(L.lib().moc_gated_residual_bwd_scratch_bytes(C.byref(s), int(gate is not None)), dtype=torch.uint8, device=dev)
+    _issue("gated_residual_bwd", _DTYPE_TAG[x.dtype], 2, dev,
+           (C.byref(s), x.data_ptr(), f.data_ptr(), weight.data_ptr(), p(bias), p(gate), p(next_weight), stats.data_ptr(), p(d_y), p(d_n),
+            p(d_x), d_f.data_ptr(), d_w.data_ptr(), p(d_b), p(d_gate), p(d_nw), p(d_nb), scratch.data_ptr()))
     return d_x, d_f, d_w, d_b, d_gate, d_nw, d_nb
 
 
@@ -1369,7 +1356,6 @@ def check_cache(kv_bank: torch.Tensor, kv_scale: Optional[torch.Tensor], scale_r
         raise ValueError("kv_scale and kv_bank must be on one device")
 
 
-@_instrument("quantize_rows", 1)
 def quantize_rows(rows: torch.Tensor, scale_rows: int, head_dim: int, values: torch.Tensor, scales: torch.Tensor) -> None:
     """bf16 ``rows`` [n, heads * head_dim] -> ``values`` (e4m3, same shape) and ``scales`` fp32 [n / scale_rows, heads]
     (``moc_quantize_rows``); both are dense."""
@@ -1381,10 +1367,8 @@ def quantize_rows(rows: torch.Tensor, scale_rows: int, head_dim: int, values: to
             or not (values.is_contiguous() and scales.is_contiguous())):
         raise ValueError("values must be dense and shaped like the rows, scales [rows / scale_rows, heads]")
     rows = _contig(rows)
-    with _on(rows.device):
-        rc = L.lib().moc_quantize_rows(rows.data_ptr(), rows.shape[0], heads, int(head_dim), int(scale_rows), values.data_ptr(),
-                                       scales.data_ptr(), L.stream_ptr(rows.device))
-    L.check(rc, "moc_quantize_rows")
+    _issue("quantize_rows", "bf16", 1, rows.device,
+           (rows.data_ptr(), rows.shape[0], heads, int(head_dim), int(scale_rows), values.data_ptr(), scales.data_ptr()))
 
 
 def decode_attn_cache(q, kv_bank, kv_scale, scale_rows: int, idx, weights, counts, num_heads: int, num_kv_heads: int,
@@ -1396,14 +1380,9 @@ def decode_attn_cache(q, kv_bank, kv_scale, scale_rows: int, idx, weights, count
     s = L.DecodeShape(b, n_q, num_heads, num_kv_heads, hd // num_heads, idx.shape[1], tokens_per_chapter, scale)
     out = torch.empty_like(q)
     lse = torch.empty((b, n_q, num_heads), dtype=torch.float32, device=dev) if want_lse else None
-    with _on(dev):
-        args = (C.byref(s), q.data_ptr(), kv_bank.data_ptr(), L.ptr(kv_scale), scale_rows, kv_bank.shape[0], idx.data_ptr(),
-                weights.data_ptr(), L.ptr(counts), out.data_ptr(), L.ptr(lse), L.status_word(dev).data_ptr(), L.stream_ptr(dev))
-        rc = (L.lib().moc_decode_attn_cache(*args) if TIMER is None
-              else _timed("decode_attn", lambda: L.lib().moc_decode_attn_cache(*args)))
-    if rc:
-        L.check(rc, "moc_decode_attn_cache")
-    _report(1, lambda: ("decode_attn:bf16" if kv_scale is None else "decode_attn:e4m3",))
+    _issue("decode_attn_cache", "bf16" if kv_scale is None else "e4m3", 1, dev,
+           (C.byref(s), q.data_ptr(), kv_bank.data_ptr(), L.ptr(kv_scale), scale_rows, kv_bank.shape[0], idx.data_ptr(), weights.data_ptr(),
+            L.ptr(counts), out.data_ptr(), L.ptr(lse), L.status_word(dev).data_ptr()))
     return out, lse
 
 

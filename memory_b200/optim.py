@@ -9,6 +9,7 @@ compact ones, without a host round trip.
 """
 from __future__ import annotations
 
+from operator import attrgetter
 from typing import Iterable, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -97,19 +98,20 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     step.  ``out``: one tensor per gradient (same shape, any of the three types) that receives the clipped values instead of the gradients.
 
     As with ``torch.nn.utils.clip_grad_norm_`` a norm that is NaN makes every gradient NaN and an infinite one gives the coefficient 0.
-    Squares are summed in 64 bits.  A tensor listed twice counts once; tensors that overlap otherwise are refused."""
+    Squares are summed in 64 bits.  A tensor listed twice counts once; tensors that overlap otherwise are refused, and so are
+    more than 4096 of them."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    grads = [_gradient(p) for p in ((parameters,) if torch.is_tensor(parameters) else parameters)]
+    grads = list(map(_gradient, (parameters,) if torch.is_tensor(parameters) else parameters))
     outs = grads if out is None else list(out)
     if len(outs) != len(grads):
         raise ValueError(f"out must have one tensor per gradient: {len(outs)} vs {len(grads)}")
-    if any(g is None for g in grads):
+    if any(map(_is_none, grads)):
         outs = [o for g, o in zip(grads, outs) if g is not None]
         grads = outs if out is None else [g for g in grads if g is not None]
-    known, banks = ops._GRAD_DTYPES, []
+    banks = []
     for sink in bank_grads:
         if len(sink.entries) > 1:
             raise NotImplementedError("one compact entry per bank: sum several layers' entries first (ops.bank_grad_merge)")
@@ -118,20 +120,31 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     if not grads and not banks:
         raise ValueError("no gradients to clip")
     device = grads[0].device if grads else banks[0][0].device
-    tensors = [*grads, *(b[0] for b in banks), *(b[1] for b in banks)] + ([] if outs is grads else outs)
-    if device.type != "cuda" or any(t.device != device or t.layout is not torch.strided for t in tensors):
+    bank_rows = [b[0] for b in banks]
+    written = [] if outs is grads else outs
+    every = [*grads, *written, *bank_rows, *(b[1] for b in banks)]
+    if device.type != "cuda" or set(map(_device, every)) != {device} or set(map(_layout, every)) != {torch.strided}:
         raise ValueError("gradients must be dense CUDA tensors on one device")
-    if any(t.dtype not in known for t in (*grads, *outs, *(b[0] for b in banks))):
+    if not set(map(_dtype, [*grads, *written, *bank_rows])) <= ops._GRAD_DTYPES.keys():
         raise TypeError("gradients must be float32, bfloat16 or float16")
-    if outs is not grads and any(o.shape != g.shape for g, o in zip(grads, outs)):
+    if written and list(map(_shape, written)) != list(map(_shape, grads)):
         raise ValueError("out must match the gradients in shape")
     copies: list = []
-    if len({(g.data_ptr(), g.shape) for g in grads}) < len(grads) or not all(t.is_contiguous() for t in (*grads, *outs)):
+    ptrs = list(map(torch.Tensor.data_ptr, grads))
+    if len(set(ptrs)) < len(ptrs) or not all(map(torch.Tensor.is_contiguous, [*grads, *written])):
         grads, outs, copies = _distinct_and_dense(grads, outs)
-    result = ops.grad_clip(grads, outs, banks, max_norm, eps, device)
+        ptrs = list(map(torch.Tensor.data_ptr, grads))
+    result = ops.grad_clip(grads, ptrs, outs, banks, max_norm, eps, device)
     for o, dense in copies:
         o.copy_(dense)
     return GradClip(*result.unbind())
+
+
+_device, _layout, _dtype, _shape = map(attrgetter, ("device", "layout", "dtype", "shape"))
+
+
+def _is_none(t) -> bool:
+    return t is None
 
 
 def _gradient(p: torch.Tensor) -> Optional[torch.Tensor]:
