@@ -280,7 +280,9 @@ decode_attn_kernel(const DecodeParams p) {
 // values = e4m3(x / scale), scale = (largest |x|) / 448 of each block of `block` rows and one head of 64 columns; a warp takes a
 // block, eight lanes a row (16 bytes of its 128 each), four rows a load.  Blocks of up to 4 R rows stay in registers; longer ones
 // are read a second time.  A block of zeros has scale 0 and values 0; one with a NaN or an infinity gets a scale that is
-// NaN or infinite and stands for NaN as a whole.  Bound by HBM (2 bytes read and 1 written an element).
+// NaN or infinite and stands for NaN as a whole.  Bound by HBM (2 bytes read and 1 written an element) once the quotient is a product
+// corrected by its remainder (Markstein), equal to the division where its last bit can matter: 262,208 x 1,536: 371 us with
+// divisions, 245 with products.
 template <int R>
 __global__ void __launch_bounds__(kDecThreads)
 quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int heads, int block, uint8_t* __restrict__ values,
@@ -292,7 +294,8 @@ quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int h
   const int head = static_cast<int>(tile - blk * heads);
   const long long width = static_cast<long long>(heads) * kDD, first = blk * block * width + head * kDD + part * 8;
   uint4 raw[R];
-  float top = 0.f;
+  uint32_t top2 = 0;                 // magnitudes order like their bits, NaN above infinity; two columns at a time
+  auto most = [&](uint32_t v) { asm("max.u16x2 %0, %0, %1;" : "+r"(top2) : "r"(v & 0x7FFF7FFFu)); };
   for (int r0 = 0; r0 < block; r0 += 4 * R) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -300,17 +303,14 @@ quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int h
       raw[i] = r < block ? __ldcs(reinterpret_cast<const uint4*>(x + first + r * width)) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float f[8];
-      unpack8(raw[i], f);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max_nan(top, fabsf(f[j]));
-    }
+    for (int i = 0; i < R; ++i) { most(raw[i].x); most(raw[i].y); most(raw[i].z); most(raw[i].w); }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float scale = top * (1.f / 448.f);       // (a product, as torch divides by a constant: the last bit follows it)
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
+  const float scale = __uint_as_float(bits << 16) * (1.f / 448.f);       // (a product, as torch divides by a constant: the last bit follows it)
   if (lane == 0) scales[tile] = scale;
+  // A quotient of the correction below its range (x < 2^-100) rounds to 0 all the same while the scale is above 2^-80.
+  const bool plain = scale > 0x1p-80f && scale < 0x1p80f;
+  const float inv = plain ? 1.f / scale : 0.f;
   for (int r0 = 0; r0 < block; r0 += 4 * R) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -319,15 +319,23 @@ quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int h
       if (block > 4 * R) raw[i] = *reinterpret_cast<const uint4*>(x + first + r * width);
       float f[8];
       unpack8(raw[i], f);
+      if (plain) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = scale > 0.f ? f[j] / scale : 0.f;
+        for (int j = 0; j < 8; ++j) {
+          const float q = f[j] * inv;
+          f[j] = fmaf(fmaf(-q, scale, f[j]), inv, q);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = scale > 0.f ? f[j] / scale : 0.f;
+      }
       uint32_t w[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
             "mov.b32 %0, {a, b};\n\t}"
             : "=r"(w[j]) : "f"(f[4 * j]), "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3]));
-      *reinterpret_cast<uint2*>(values + first + r * width) = make_uint2(w[0], w[1]);
+      __stcs(reinterpret_cast<uint2*>(values + first + r * width), make_uint2(w[0], w[1]));
     }
   }
 }

@@ -11,9 +11,12 @@
 // y is formed again from x and f (it was rounded on its way out, and the sums over rows would carry that rounding): the same
 // bytes as reading y.
 //
-// Bound by HBM (f, x -> y, n; backward d_y, d_n, x, f -> d_x, d_f).  A row belongs to one CTA of as many threads as the row has
-// pieces of four columns (up to 256; past 1,024 columns up to 512 of 2 or 4 pieces each), which holds it in registers between the passes: every
-// tensor is read once and a row's reductions are one barrier each.  Small CTAs beside each other hide the barriers.
+// Bound by HBM (f, x -> y, n; backward d_y, d_n, x, f -> d_x, d_f).  A row belongs to one warp (up to 768 columns; 2 to 8 warps
+// beyond), which holds it in registers between the passes, so every tensor is read once and a row's sums are shuffles.  The
+// warps stay for many rows; while one is worked on, the next ones are on their way into shared memory (asynchronous copies,
+// each thread its own columns, so nobody waits for anybody else).  The backward pass runs one CTA an SM; its warps keep the
+// column sums of their rows in registers.
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -22,10 +25,8 @@
 namespace moc {
 namespace {
 
-constexpr int kResBlocks = 148 * 4;       // CTAs of the backward pass: each keeps its column sums over its rows
-
-// threads of a CTA: 256 where a thread has one piece, 512 otherwise
-constexpr int most_threads(int nv, int v) { return nv * v == 4 ? 256 : 512; }
+constexpr int kResThreads = 256;
+constexpr int kResCtas = 148;             // CTAs of the backward pass
 
 struct ResParams {
   const void *x, *f;
@@ -35,6 +36,7 @@ struct ResParams {
   long long rows;
   int d, seq;                   // rows of a sequence (gate_rows) 
   int ln, gate_rows, next;      // gate_rows: the gate has a row for every sequence
+  int group;                    // warps of a row
   float scale, eps, eps2;
 };
 struct ResGrads {
@@ -46,23 +48,23 @@ struct ResGrads {
   long long items;              // sequences * chunks
 };
 
-// the pieces of four columns of one row that a thread has: lane-wise, so a warp's loads are contiguous
+// the pieces of V columns of a row that a thread has: lane-wise, so a warp's loads are contiguous
 template <typename T, int V> struct Piece;
 template <> struct Piece<float, 4> {
-  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  }
+  using Raw = float4;
+  static __device__ __forceinline__ void unpack(const float4& a, float (&v)[4]) { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; }
+  static __device__ __forceinline__ void load(const float* p, float (&v)[4]) { unpack(*reinterpret_cast<const float4*>(p), v); }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
   }
 };
 template <> struct Piece<__nv_bfloat16, 4> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
+  using Raw = uint2;
+  static __device__ __forceinline__ void unpack(const uint2& a, float (&v)[4]) {
     v[0] = __uint_as_float(a.x << 16); v[1] = __uint_as_float(a.x & 0xFFFF0000u);
     v[2] = __uint_as_float(a.y << 16); v[3] = __uint_as_float(a.y & 0xFFFF0000u);
   }
+  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[4]) { unpack(*reinterpret_cast<const uint2*>(p), v); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[4]) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
   }
@@ -76,54 +78,59 @@ template <> struct Piece<__nv_bfloat16, 1> {
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[1]) { *p = __float2bfloat16(v[0]); }
 };
 
-// Sum over the CTA, the same in every thread.  One barrier: the next call uses the other half of `red`.
-struct RowSum {
-  float2* red;        // [2][16]
+// This thread's place: `t` of the `n` threads of its row (n: 32 times 1, 2, 4 or 8 warps), and the row's sums, the same in
+// each of them (one barrier of those warps; the next call uses the other half of `red`).
+struct RowGroup {
+  int t, n, id;       // id: of the group in the CTA
+  float2* red;        // [2][warps of the CTA]
   int half;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  __device__ __forceinline__ RowGroup(int warps, float2* r) : t(threadIdx.x % (32 * warps)), n(32 * warps), id(threadIdx.x / (32 * warps)), red(r), half(0) {}
+  __device__ __forceinline__ float2 sum(float a, float b) {
     a = warp_sum(a);
     b = warp_sum(b);
-    if (blockDim.x == 32) return make_float2(a, b);
-    float2* r = red + half * 16;
+    return across(a, b);
+  }
+  __device__ __forceinline__ float sum(float a) { return across(warp_sum(a), 0.f).x; }
+  __device__ __forceinline__ float2 across(float a, float b) {
+    if (n == 32) return make_float2(a, b);
+    float2* r = red + half * (kResThreads / 32) + id * (n >> 5);
     half ^= 1;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    float2 t = make_float2(0.f, 0.f);
-    const int nw = blockDim.x >> 5;
-    for (int i = 0; i < nw; ++i) { t.x += r[i].x; t.y += r[i].y; }
-    return t;
+    if ((threadIdx.x & 31) == 0) r[t >> 5] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(n) : "memory");
+    float2 s = r[0];
+    for (int i = 1; i < (n >> 5); ++i) { s.x += r[i].x; s.y += r[i].y; }
+    return s;
   }
 };
 
-// mean and 1 / sqrt(variance + eps) of the row in `v` (zero past its end); LayerNorm sums twice, as the difference of the mean of
+// mean and 1 / sqrt(variance + eps) of the row in `v`; LayerNorm sums twice, as the difference of the mean of
 // squares and the squared mean loses what is small against the mean
 template <int NV, int V>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][V], int ln, float eps, int d, RowSum& sum) {
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][V], int ln, float eps, int d, RowGroup& g) {
   float mean = 0.f, ss = 0.f;
   if (ln) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += v[i][j];
-    mean = sum(s, 0.f).x / static_cast<float>(d);
+      for (int j = 0; j < V; ++j) s += (g.t + i * g.n) * V < d ? v[i][j] : 0.f;       // (the affine step leaves its bias in unused columns)
+    mean = g.sum(s) / static_cast<float>(d);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (threadIdx.x + i * blockDim.x) * V + j;
-      const float u = c < d ? v[i][j] - mean : 0.f;
+      const float u = (g.t + i * g.n) * V + j < d ? v[i][j] - mean : 0.f;
       ss = fmaf(u, u, ss);
     }
-  return make_float2(mean, 1.f / sqrtf(sum(ss, 0.f).x / static_cast<float>(d) + eps));
+  return make_float2(mean, 1.f / sqrtf(g.sum(ss) / static_cast<float>(d) + eps));
 }
 
 template <typename T, int NV, int V>
-__device__ __forceinline__ void load_row(const T* p, int d, float (&v)[NV][V]) {
+__device__ __forceinline__ void load_row(const RowGroup& g, const T* p, int d, float (&v)[NV][V]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * V;
+    const int c = (g.t + i * g.n) * V;
     if (c < d) {
       Piece<T, V>::load(p + c, v[i]);
     } else {
@@ -132,79 +139,161 @@ __device__ __forceinline__ void load_row(const T* p, int d, float (&v)[NV][V]) {
     }
   }
 }
+// A row on its way through shared memory: thread-private slots of one piece, kResThreads of them behind each other.  Single columns
+// (V = 1) are not staged: they are read from their place when they are needed.
+template <typename T, int NV, int V> __host__ __device__ constexpr int row_bytes() { return V == 1 ? 0 : NV * V * static_cast<int>(sizeof(T)) * kResThreads; }
+__device__ __forceinline__ void cp_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src));
+}
 template <typename T, int NV, int V>
-__device__ __forceinline__ void store_row(T* p, int d, const float (&v)[NV][V]) {
+__device__ __forceinline__ void stage_row(const RowGroup& g, const T* p, int d, char* slots) {
+  if constexpr (V > 1) {
+    using Raw = typename Piece<T, V>::Raw;
+    Raw* to = reinterpret_cast<Raw*>(slots) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (g.t + i * g.n) * V;
+      if (c >= d) continue;
+      if constexpr (sizeof(Raw) == 16) cp_async16(to + i * kResThreads, p + c);
+      else cp_async8(to + i * kResThreads, p + c);
+    }
+  }
+}
+template <typename T, int NV, int V>
+__device__ __forceinline__ void staged_row(const RowGroup& g, const T* p, int d, const char* slots, float (&v)[NV][V]) {
+  if constexpr (V == 1) {
+    load_row(g, p, d, v);
+  } else {
+    using Raw = typename Piece<T, V>::Raw;
+    const Raw* from = reinterpret_cast<const Raw*>(slots) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) Piece<T, V>::unpack(from[i * kResThreads], v[i]);       // (what lies in unused slots is put away)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = (g.t + i * g.n) * V < d ? v[i][j] : 0.f;
+  }
+}
+// waits until at most `ahead` of this thread's committed rows are still on their way
+__device__ __forceinline__ void wait_rows(int ahead) {
+  if (ahead == 0) cp_async_wait<0>();
+  else if (ahead == 1) cp_async_wait<1>();
+  else if (ahead == 2) cp_async_wait<2>();
+  else cp_async_wait<3>();
+}
+__device__ __forceinline__ void warm(const RowGroup& g, const float* p, int d) {       // a parameter row on its way into L1
+  if (p == nullptr) return;
+  for (int c = g.t * 32; c < d; c += g.n * 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(p + c));
+}
+template <typename T, int NV, int V>
+__device__ __forceinline__ void store_row(const RowGroup& g, T* p, int d, const float (&v)[NV][V]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * V;
+    const int c = (g.t + i * g.n) * V;
     if (c < d) Piece<T, V>::store(p + c, v[i]);
   }
 }
-// v = v * w (+ b), columns past the end stay zero; w / b may be NULL
+// A row of parameters.  Without a branch a piece, so that all are requested together: columns past the end read the first ones,
+// and meet zeros wherever it matters.
 template <int NV, int V>
-__device__ __forceinline__ void affine(float (&v)[NV][V], const float* w, const float* b, int d) {
+__device__ __forceinline__ void load_param(const RowGroup& g, const float* p, int d, float (&a)[NV][V]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (threadIdx.x + i * blockDim.x) * V;
-    if (c >= d) continue;
-    float a[V];
-    if (w != nullptr) {
-      Piece<float, V>::load(w + c, a);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] *= a[j];
-    }
-    if (b != nullptr) {
-      Piece<float, V>::load(b + c, a);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] += a[j];
-    }
+    const int c = (g.t + i * g.n) * V;
+    Piece<float, V>::load(p + (c < d ? c : 0), a[i]);
   }
+}
+// v = v * w (+ b)
+template <int NV, int V>
+__device__ __forceinline__ void affine(const RowGroup& g, float (&v)[NV][V], const float* w, const float* b, int d) {
+  float a[NV][V];
+  load_param(g, w, d, a);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] *= a[i][j];
+  if (b == nullptr) return;
+  load_param(g, b, d, a);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] += a[i][j];
 }
 template <int NV, int V>
-__device__ __forceinline__ void normalise(float (&v)[NV][V], float2 st, int d) {
+__device__ __forceinline__ void normalise(const RowGroup& g, float (&v)[NV][V], float2 st, int d) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = (threadIdx.x + i * blockDim.x) * V + j < d ? (v[i][j] - st.x) * st.y : 0.f;
+    for (int j = 0; j < V; ++j) v[i][j] = (g.t + i * g.n) * V + j < d ? (v[i][j] - st.x) * st.y : 0.f;
 }
 
+// depth: rows of a warp group in shared memory at once
 template <typename XT, typename FT, int NV, int V>
-__global__ void __launch_bounds__(most_threads(NV, V))
-residual_fwd_kernel(const ResParams p) {
-  __shared__ float2 red[32];
-  RowSum sum{red, 0};
-  const long long row = blockIdx.x;
-  float f[NV][V], x[NV][V];
-  load_row(static_cast<const FT*>(p.f) + row * p.d, p.d, f);
-  load_row(static_cast<const XT*>(p.x) + row * p.d, p.d, x);
-  const float2 st = row_stats(f, p.ln, p.eps, p.d, sum);
-  normalise(f, st, p.d);
-  affine(f, p.w, p.b, p.d);
-  if (p.gate != nullptr) affine(f, p.gate + (p.gate_rows ? row / p.seq * p.d : 0), nullptr, p.d);
+__global__ void __launch_bounds__(kResThreads, NV * V <= 24 ? 2 : 1)
+residual_fwd_kernel(const ResParams p, const int depth) {
+  __shared__ float2 red[2 * kResThreads / 32];
+  extern __shared__ __align__(16) char slots[];
+  constexpr int kF = row_bytes<FT, NV, V>(), kSlots = kF + row_bytes<XT, NV, V>();
+  RowGroup g(p.group, red);
+  const int groups = kResThreads / g.n;
+  const long long stride = static_cast<long long>(gridDim.x) * groups;
+  const FT* fp = static_cast<const FT*>(p.f);
+  const XT* xp = static_cast<const XT*>(p.x);
+  long long ahead = static_cast<long long>(blockIdx.x) * groups + g.id;
+  int fill = 0;
+  auto fetch = [&]() {
+    if (ahead < p.rows) {
+      stage_row<FT, NV, V>(g, fp + ahead * p.d, p.d, slots + fill * kSlots);
+      stage_row<XT, NV, V>(g, xp + ahead * p.d, p.d, slots + fill * kSlots + kF);
+    }
+    cp_async_commit();
+    ahead += stride;
+    fill = fill + 1 == depth ? 0 : fill + 1;
+  };
+  int stage = 0;
+  for (int i = 1; i < depth; ++i) fetch();
+  warm(g, p.w, p.d); warm(g, p.b, p.d); warm(g, p.w2, p.d); warm(g, p.b2, p.d);
+  if (!p.gate_rows) warm(g, p.gate, p.d);
+  for (long long row = static_cast<long long>(blockIdx.x) * groups + g.id; row < p.rows; row += stride) {
+    fetch();
+    wait_rows(depth - 1);
+    float f[NV][V], x[NV][V];
+    staged_row(g, fp + row * p.d, p.d, slots + stage * kSlots, f);
+    staged_row(g, xp + row * p.d, p.d, slots + stage * kSlots + kF, x);
+    stage = stage + 1 == depth ? 0 : stage + 1;
+    const float2 st = row_stats(f, p.ln, p.eps, p.d, g);
+    normalise(g, f, st, p.d);
+    affine(g, f, p.w, p.b, p.d);
+    if (p.gate != nullptr) affine(g, f, p.gate + (p.gate_rows ? row / p.seq * p.d : 0), nullptr, p.d);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[i][j] = fmaf(p.scale, x[i][j], f[i][j]);
-  store_row(static_cast<XT*>(p.y) + row * p.d, p.d, x);
-  float2 st2 = make_float2(0.f, 0.f);
-  if (p.next) {
-    st2 = row_stats(x, p.ln, p.eps2, p.d, sum);
-    normalise(x, st2, p.d);
-    affine(x, p.w2, p.b2, p.d);
-    store_row(static_cast<FT*>(p.n) + row * p.d, p.d, x);
+      for (int j = 0; j < V; ++j) x[i][j] = fmaf(p.scale, x[i][j], f[i][j]);
+    store_row(g, static_cast<XT*>(p.y) + row * p.d, p.d, x);
+    float2 st2 = make_float2(0.f, 0.f);
+    if (p.next) {
+      st2 = row_stats(x, p.ln, p.eps2, p.d, g);
+      normalise(g, x, st2, p.d);
+      affine(g, x, p.w2, p.b2, p.d);
+      store_row(g, static_cast<FT*>(p.n) + row * p.d, p.d, x);
+    }
+    if (p.stats != nullptr && g.t == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(st.x, st.y, st2.x, st2.y);
   }
-  if (p.stats != nullptr && threadIdx.x == 0) reinterpret_cast<float4*>(p.stats)[row] = make_float4(st.x, st.y, st2.x, st2.y);
 }
 
-// Column sums a thread keeps over the rows of its CTA: [0] t fhat (times the gate where it has a row for every sequence),
+// Column sums a thread keeps over its rows: [0] t fhat (times the gate where it has a row for every sequence),
 // [1] the same without fhat, [2] d_n yhat, [3] d_n; LayerNorm has all four, RMSNorm [0] and [2].  A gate row's own sum
 // leaves with each item (a run of rows of one sequence).
 template <typename XT, typename FT, int NV, int V, bool LN>
-__global__ void __launch_bounds__(most_threads(NV, V))
-residual_bwd_kernel(const ResParams p, const ResGrads g) {
-  __shared__ float2 red[32];
-  RowSum sum{red, 0};
+__global__ void __launch_bounds__(kResThreads, 1)
+residual_bwd_kernel(const ResParams p, const ResGrads q, const int depth) {
+  __shared__ float2 red[2 * kResThreads / 32];
+  extern __shared__ __align__(16) char slots[];         // rows on their way, at the end [groups of the CTA][d] column sums
+  float* columns = reinterpret_cast<float*>(slots);
+  constexpr int kF = row_bytes<FT, NV, V>(), kX = row_bytes<XT, NV, V>(), kSlots = 2 * (kF + kX);
+  RowGroup g(p.group, red);
   constexpr int kSums = LN ? 4 : 2, kStep = LN ? 1 : 2;
+  const int groups = kResThreads / g.n;
   float acc[kSums][NV][V];
 #pragma unroll
   for (int k = 0; k < kSums; ++k)
@@ -214,21 +303,49 @@ residual_bwd_kernel(const ResParams p, const ResGrads g) {
       for (int j = 0; j < V; ++j) acc[k][i][j] = 0.f;
   const float inv_d = 1.f / static_cast<float>(p.d);
 
-  for (long long item = blockIdx.x; item < g.items; item += gridDim.x) {
-    const long long s = item / g.chunks;
-    const long long r0 = s * p.seq + (item - s * g.chunks) * g.chunk_rows;
-    const long long r1 = min(r0 + g.chunk_rows, min((s + 1) * p.seq, p.rows));
+  const long long first = static_cast<long long>(blockIdx.x) * groups + g.id, stride = static_cast<long long>(gridDim.x) * groups;
+  auto rows_of = [&](long long item, long long& r0, long long& r1) {       // of a run; none behind the last
+    const long long s = item / q.chunks;
+    r0 = s * p.seq + (item - s * q.chunks) * q.chunk_rows;
+    r1 = item < q.items ? min(r0 + q.chunk_rows, min((s + 1) * p.seq, p.rows)) : r0;
+  };
+  long long next_item = first, next_row, next_end;
+  rows_of(next_item, next_row, next_end);
+  int fill = 0, stage = 0;
+  auto fetch = [&]() {
+    if (next_row < next_end) {
+      char* to = slots + fill * kSlots;
+      const long long at = next_row * p.d;
+      stage_row<FT, NV, V>(g, static_cast<const FT*>(p.f) + at, p.d, to);
+      if (q.dy != nullptr) stage_row<XT, NV, V>(g, static_cast<const XT*>(q.dy) + at, p.d, to + kF);
+      if (q.dn != nullptr) {
+        stage_row<XT, NV, V>(g, static_cast<const XT*>(p.x) + at, p.d, to + kF + kX);
+        stage_row<FT, NV, V>(g, static_cast<const FT*>(q.dn) + at, p.d, to + kF + 2 * kX);
+      }
+      if (++next_row == next_end) {
+        next_item += stride;
+        rows_of(next_item, next_row, next_end);
+      }
+    }
+    cp_async_commit();
+    fill = fill + 1 == depth ? 0 : fill + 1;
+  };
+  for (int i = 1; i < depth; ++i) fetch();
+  for (long long item = first; item < q.items; item += stride) {
+    const long long s = item / q.chunks;
+    long long r0, r1;
+    rows_of(item, r0, r1);
     const float* gate = p.gate == nullptr ? nullptr : p.gate + (p.gate_rows ? s * p.d : 0);
-    float gsum[NV][V];
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) gsum[i][j] = 0.f;
+    // (a gate row's sum is rare: it is kept in its place in memory)
     for (long long row = r0; row < r1; ++row) {
+      fetch();
+      wait_rows(depth - 1);
+      const char* from = slots + stage * kSlots;
+      stage = stage + 1 == depth ? 0 : stage + 1;
       float f[NV][V], t[NV][V];
-      load_row(static_cast<const FT*>(p.f) + row * p.d, p.d, f);
-      if (g.dy != nullptr) {
-        load_row(static_cast<const XT*>(g.dy) + row * p.d, p.d, t);
+      staged_row(g, static_cast<const FT*>(p.f) + row * p.d, p.d, from, f);
+      if (q.dy != nullptr) {
+        staged_row(g, static_cast<const XT*>(q.dy) + row * p.d, p.d, from + kF, t);
       } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -236,23 +353,25 @@ residual_bwd_kernel(const ResParams p, const ResGrads g) {
           for (int j = 0; j < V; ++j) t[i][j] = 0.f;
       }
       const float4 st = reinterpret_cast<const float4*>(p.stats)[row];
-      if (g.dn != nullptr) {
+      if (q.dn != nullptr) {
         float y[NV][V], n[NV][V];
-        load_row(static_cast<const XT*>(p.x) + row * p.d, p.d, y);
-        load_row(static_cast<const FT*>(g.dn) + row * p.d, p.d, n);
-        normalise(f, make_float2(st.x, st.y), p.d);
-        float z[NV][V];
+        staged_row(g, static_cast<const XT*>(p.x) + row * p.d, p.d, from + kF + kX, y);
+        staged_row(g, static_cast<const FT*>(q.dn) + row * p.d, p.d, from + kF + 2 * kX, n);
+        normalise(g, f, make_float2(st.x, st.y), p.d);
+        {
+          float z[NV][V];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+          for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) z[i][j] = f[i][j];
-        affine(z, p.w, p.b, p.d);
-        if (gate != nullptr) affine(z, gate, nullptr, p.d);
+            for (int j = 0; j < V; ++j) z[i][j] = f[i][j];
+          affine(g, z, p.w, p.b, p.d);
+          if (gate != nullptr) affine(g, z, gate, nullptr, p.d);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+          for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[i][j] = fmaf(p.scale, y[i][j], z[i][j]);
-        normalise(y, make_float2(st.z, st.w), p.d);
+            for (int j = 0; j < V; ++j) y[i][j] = fmaf(p.scale, y[i][j], z[i][j]);
+        }
+        normalise(g, y, make_float2(st.z, st.w), p.d);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -260,43 +379,55 @@ residual_bwd_kernel(const ResParams p, const ResGrads g) {
             acc[LN ? 2 : 1][i][j] = fmaf(n[i][j], y[i][j], acc[LN ? 2 : 1][i][j]);
             if (LN) acc[kSums - 1][i][j] += n[i][j];
           }
-        affine(n, p.w2, nullptr, p.d);
+        affine(g, n, p.w2, nullptr, p.d);
         float c1 = 0.f, c2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) { c1 = fmaf(n[i][j], y[i][j], c1); c2 += n[i][j]; }
-        const float2 c = sum(c1, c2);
+          for (int j = 0; j < V; ++j) { c1 = fmaf(n[i][j], y[i][j], c1); if (LN) c2 += n[i][j]; }
+        const float2 c = LN ? g.sum(c1, c2) : make_float2(g.sum(c1), 0.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if ((threadIdx.x + i * blockDim.x) * V + j < p.d)
-              t[i][j] += st.w * (n[i][j] - (LN ? c.y * inv_d : 0.f) - y[i][j] * (c.x * inv_d));
+            if ((g.t + i * g.n) * V + j < p.d) t[i][j] += st.w * (n[i][j] - (LN ? c.y * inv_d : 0.f) - y[i][j] * (c.x * inv_d));
       } else {
-        normalise(f, make_float2(st.x, st.y), p.d);
+        normalise(g, f, make_float2(st.x, st.y), p.d);
       }
       // t: the gradient at y; f: the normalised branch
-      if (g.dx != nullptr) {
-        float dx[NV][V];
+      if (q.dx != nullptr) {
+        XT* dx = static_cast<XT*>(q.dx) + row * p.d;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+          float u[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) dx[i][j] = p.scale * t[i][j];
-        store_row(static_cast<XT*>(g.dx) + row * p.d, p.d, dx);
+          for (int j = 0; j < V; ++j) u[j] = p.scale * t[i][j];
+          const int c = (g.t + i * g.n) * V;
+          if (c < p.d) Piece<XT, V>::store(dx + c, u);
+        }
       }
       if (p.gate_rows) {
+        float* sum = q.gate_part + item * p.d;
         float z[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) z[i][j] = f[i][j];
-        affine(z, p.w, p.b, p.d);
+        affine(g, z, p.w, p.b, p.d);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) gsum[i][j] = fmaf(t[i][j], z[i][j], gsum[i][j]);
-        affine(t, gate, nullptr, p.d);
+          for (int j = 0; j < V; ++j) z[i][j] *= t[i][j];
+        if (row > r0) {
+          float old[NV][V];
+          load_row(g, const_cast<const float*>(sum), p.d, old);
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) z[i][j] += old[i][j];
+        }
+        store_row(g, sum, p.d, z);
+        affine(g, t, gate, nullptr, p.d);
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -305,24 +436,38 @@ residual_bwd_kernel(const ResParams p, const ResGrads g) {
           acc[0][i][j] = fmaf(t[i][j], f[i][j], acc[0][i][j]);
           if (LN) acc[1][i][j] += t[i][j];
         }
-      if (!p.gate_rows && gate != nullptr) affine(t, gate, nullptr, p.d);
-      affine(t, p.w, nullptr, p.d);
+      if (!p.gate_rows && gate != nullptr) affine(g, t, gate, nullptr, p.d);
+      affine(g, t, p.w, nullptr, p.d);
       float c1 = 0.f, c2 = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) { c1 = fmaf(t[i][j], f[i][j], c1); c2 += t[i][j]; }
-      const float2 c = sum(c1, c2);
+        for (int j = 0; j < V; ++j) { c1 = fmaf(t[i][j], f[i][j], c1); if (LN) c2 += t[i][j]; }
+      const float2 c = LN ? g.sum(c1, c2) : make_float2(g.sum(c1), 0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) t[i][j] = st.y * (t[i][j] - (LN ? c.y * inv_d : 0.f) - f[i][j] * (c.x * inv_d));
-      store_row(static_cast<FT*>(g.df) + row * p.d, p.d, t);
+      store_row(g, static_cast<FT*>(q.df) + row * p.d, p.d, t);
     }
-    if (p.gate_rows) store_row(g.gate_part + item * p.d, p.d, gsum);
   }
+  // the groups' column sums -> the CTA's
 #pragma unroll
-  for (int k = 0; k < kSums; ++k) store_row(g.partial + (static_cast<long long>(blockIdx.x) * 4 + k * kStep) * p.d, p.d, acc[k]);
+  for (int k = 0; k < kSums; ++k) {
+    float* out = q.partial + (static_cast<long long>(blockIdx.x) * 4 + k * kStep) * p.d;
+    if (groups == 1) {
+      store_row(g, out, p.d, acc[k]);
+      continue;
+    }
+    __syncthreads();
+    store_row(g, columns + g.id * p.d, p.d, acc[k]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.d; c += kResThreads) {
+      float t = 0.f;
+      for (int i = 0; i < groups; ++i) t += columns[i * p.d + c];
+      out[c] = t;
+    }
+  }
 }
 
 struct ResSums {
@@ -331,28 +476,19 @@ struct ResSums {
   float *dw, *db, *dgate, *dw2, *db2;
   int blocks, d, chunks, ln, gate_rows;
 };
-// 32 columns a CTA, 8 warps share the partial rows.  blockIdx.y == 0: the sums over all rows; blockIdx.y - 1: a sequence's gate row.
-__global__ void __launch_bounds__(256)
+// 32 columns a CTA, 32 warps share the partial rows.  blockIdx.y == 0: the sums over all rows; blockIdx.y - 1: a sequence's gate row.
+__global__ void __launch_bounds__(1024)
 residual_sums_kernel(const ResSums s) {
-  __shared__ float red[4][8][32];
+  __shared__ float red[4][32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
   if (blockIdx.y > 0) {
     const long long q = blockIdx.y - 1;
     if (c < s.d)
-      for (int k = warp; k < s.chunks; k += 8) a[0] += s.gate_part[(q * s.chunks + k) * s.d + c];
-    red[0][warp][lane] = a[0];
-    __syncthreads();
-    if (warp == 0 && c < s.d) {
-      float t = 0.f;
-      for (int k = 0; k < 8; ++k) t += red[0][k][lane];
-      s.dgate[q * s.d + c] = t;
-    }
-    return;
-  }
-  if (c < s.d) {
+      for (int k = warp; k < s.chunks; k += 32) a[0] += s.gate_part[(q * s.chunks + k) * s.d + c];
+  } else if (c < s.d) {
 #pragma unroll 4
-    for (int k = warp; k < s.blocks; k += 8) {
+    for (int k = warp; k < s.blocks; k += 32) {
       const float* p = s.partial + static_cast<long long>(k) * 4 * s.d + c;
       a[0] += p[0];
       a[2] += p[2 * static_cast<long long>(s.d)];
@@ -360,45 +496,52 @@ residual_sums_kernel(const ResSums s) {
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) red[k][warp][lane] = a[k];
+  for (int k = 0; k < 4; ++k) red[k][lane][warp] = a[k];
   __syncthreads();
-  if (warp > 0 || c >= s.d) return;
+  // warp w adds column w up over the 32 warps
+  const int col = blockIdx.x * 32 + warp;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    a[k] = 0.f;
-    for (int i = 0; i < 8; ++i) a[k] += red[k][i][lane];
+  for (int k = 0; k < 4; ++k) a[k] = warp_sum(red[k][warp][lane]);
+  if (lane > 0 || col >= s.d) return;
+  if (blockIdx.y > 0) {
+    s.dgate[static_cast<long long>(blockIdx.y - 1) * s.d + col] = a[0];
+    return;
   }
   // with a gate of one row the sums are without it: d_w = gate * sum t fhat, d_gate = sum t (w fhat + b)
-  const float gate = s.gate != nullptr && !s.gate_rows ? s.gate[c] : 1.f;
-  if (s.dw != nullptr) s.dw[c] = gate * a[0];
-  if (s.db != nullptr) s.db[c] = gate * a[1];
-  if (s.dgate != nullptr && !s.gate_rows) s.dgate[c] = s.w[c] * a[0] + (s.b != nullptr ? s.b[c] * a[1] : 0.f);
-  if (s.dw2 != nullptr) s.dw2[c] = a[2];
-  if (s.db2 != nullptr) s.db2[c] = a[3];
+  const float gate = s.gate != nullptr && !s.gate_rows ? s.gate[col] : 1.f;
+  if (s.dw != nullptr) s.dw[col] = gate * a[0];
+  if (s.db != nullptr) s.db[col] = gate * a[1];
+  if (s.dgate != nullptr && !s.gate_rows) s.dgate[col] = s.w[col] * a[0] + (s.b != nullptr ? s.b[col] * a[1] : 0.f);
+  if (s.dw2 != nullptr) s.dw2[col] = a[2];
+  if (s.db2 != nullptr) s.db2[col] = a[3];
 }
 
 struct Plan {
-  int v, nv, threads;
+  int v, each, group;              // columns of an access, of a thread; warps of a row
 };
-// pieces of four columns wherever rows and base addresses allow 16-byte (fp32) accesses, single columns otherwise
-Plan plan_of(int d, bool wide) {
-  const int each = d <= 1024 ? 4 : d <= 4096 ? 8 : 16;       // columns of a thread
+// Pieces of four columns wherever rows and base addresses allow 16-byte (fp32) accesses, single columns otherwise.  24 columns a
+// lane fill a row of 768 with one warp; the backward pass of a LayerNorm keeps four sums a column and takes 16.
+Plan plan_of(int d, bool wide, bool lean) {
   Plan p;
   p.v = wide ? 4 : 1;
-  p.nv = each / p.v;
-  p.threads = ((d + each - 1) / each + 31) / 32 * 32;
+  p.each = d <= 256 ? 8 : d <= 768 && !lean ? 24 : d <= 4096 ? 16 : 32;
+  p.group = 1;
+  while (p.group * 32 * p.each < d) p.group *= 2;
   return p;
 }
-template <typename Go> int with_plan(const Plan& p, Go go) {
+template <int V, typename Go> int with_each(int each, Go go) {
   using std::integral_constant;
-  if (p.v == 4) {
-    if (p.nv == 1) return go(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    if (p.nv == 2) return go(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    return go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-  }
-  if (p.nv == 4) return go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  if (p.nv == 8) return go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-  return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  using W = integral_constant<int, V>;
+  if (each == 8) return go(integral_constant<int, 8 / V>{}, W{});
+  if (each == 16) return go(integral_constant<int, 16 / V>{}, W{});
+  if (each == 24) return go(integral_constant<int, 24 / V>{}, W{});
+  return go(integral_constant<int, 32 / V>{}, W{});
+}
+template <typename Go> int with_plan(const Plan& p, Go go) { return p.v == 4 ? with_each<4>(p.each, go) : with_each<1>(p.each, go); }
+// Rows in flight a warp group: as many of `bytes` a CTA as fit, four at most
+int depth_of(const Plan& p, int bytes, int room) {
+  if (p.v == 1) return 1;
+  return std::max(1, std::min(4, room / bytes));
 }
 template <typename Go> int with_types(const moc_residual_shape* s, Go go) {
   if (s->x_dtype == MOC_F32) return s->f_dtype == MOC_F32 ? go(float{}, float{}) : go(float{}, __nv_bfloat16{});
@@ -435,16 +578,17 @@ struct Split {
   int chunks, chunk_rows, blocks;
   long long items;
 };
-// Runs of rows of one sequence: about as many as there are CTAs, whole sequences where those are shorter.
+// Runs of rows of one sequence: about as many as there are groups of warps, whole sequences where those are shorter.
 Split split_of(const ResParams& p) {
   Split s;
   const long long seqs = p.rows / p.seq;
-  long long per = (kResBlocks + seqs - 1) / seqs;           // runs of a sequence
+  const int groups = kResThreads / (32 * p.group), most = kResCtas * groups;
+  long long per = (most + seqs - 1) / seqs;                 // runs of a sequence
   if (per > p.seq) per = p.seq;
   s.chunk_rows = static_cast<int>((p.seq + per - 1) / per);
   s.chunks = (p.seq + s.chunk_rows - 1) / s.chunk_rows;
   s.items = seqs * s.chunks;
-  s.blocks = static_cast<int>(s.items < kResBlocks ? s.items : kResBlocks);
+  s.blocks = static_cast<int>(std::min<long long>((s.items + groups - 1) / groups, kResCtas));
   return s;
 }
 
@@ -462,11 +606,19 @@ extern "C" int moc_gated_residual_fwd(const moc_residual_shape* s, const void* x
   MOC_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "stats must be 16-byte aligned");
   ResParams p = params(s, x, f, weight, bias, gate, next_weight, next_bias, stats);
   p.y = y; p.n = n;
-  const Plan plan = plan_of(s->dim, wide(s->dim, {x, f, weight, bias, gate, next_weight, next_bias, y, n}));
+  const Plan plan = plan_of(s->dim, wide(s->dim, {x, f, weight, bias, gate, next_weight, next_bias, y, n}), false);
+  p.group = plan.group;
+  const int groups = kResThreads / (32 * p.group), ctas = plan.each <= 24 ? 2 : 1;         // on an SM
+  const int bytes = plan.each * kResThreads * ((s->x_dtype == MOC_F32 ? 4 : 2) + (s->f_dtype == MOC_F32 ? 4 : 2));
+  const int depth = depth_of(plan, bytes, 160 * 1024 / ctas);          // (the rest is L1, for the parameters)
+  const long long most = (p.rows + groups - 1) / groups;
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(most, static_cast<long long>(kResCtas) * ctas));
   return with_types(s, [&](auto xt, auto ft) {
     return with_plan(plan, [&](auto nv, auto v) {
-      residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value>
-          <<<static_cast<unsigned>(p.rows), plan.threads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+      auto kern = residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value>;
+      const size_t shared = plan.v == 1 ? 0 : static_cast<size_t>(depth) * bytes;
+      MOC_CUDA_OK(allow_shared(kern, shared, 216 * 1024));
+      kern<<<grid, kResThreads, shared, static_cast<cudaStream_t>(stream)>>>(p, depth);
       MOC_CUDA_OK(cudaGetLastError());
       return static_cast<int>(MOC_OK);
     });
@@ -478,6 +630,7 @@ extern "C" int64_t moc_gated_residual_bwd_scratch_bytes(const moc_residual_shape
   ResParams p{};
   p.rows = s->rows;
   p.seq = with_gate && s->gate_seq > 0 ? s->gate_seq : static_cast<int>(s->rows);
+  p.group = plan_of(s->dim, true, s->kind == MOC_NORM_LAYERNORM).group;          // (the same for single columns)
   const Split sp = split_of(p);
   return (static_cast<int64_t>(sp.blocks) * 4 + (with_gate && s->gate_seq > 0 ? sp.items : 0)) * s->dim * 4 + 256;
 }
@@ -494,6 +647,8 @@ extern "C" int moc_gated_residual_bwd(const moc_residual_shape* s, const void* x
   MOC_REQUIRE(((reinterpret_cast<uintptr_t>(stats) | reinterpret_cast<uintptr_t>(scratch)) & 15) == 0,
               "stats and scratch must be 16-byte aligned");
   ResParams p = params(s, x, f, weight, bias, gate, next_weight, nullptr, const_cast<float*>(stats));
+  const Plan plan = plan_of(p.d, wide(p.d, {x, f, weight, bias, gate, next_weight, d_y, d_n, d_x, d_f}), p.ln);
+  p.group = plan.group;
   const Split sp = split_of(p);
   MOC_REQUIRE(!p.gate_rows || sp.items / sp.chunks <= 65534, "too many sequences with a gate row of their own (65,534)");
   ResGrads g{};
@@ -501,13 +656,18 @@ extern "C" int moc_gated_residual_bwd(const moc_residual_shape* s, const void* x
   g.partial = static_cast<float*>(scratch);
   g.gate_part = g.partial + static_cast<long long>(sp.blocks) * 4 * p.d;
   g.chunks = sp.chunks; g.chunk_rows = sp.chunk_rows; g.items = sp.items;
-  const Plan plan = plan_of(p.d, wide(p.d, {x, f, weight, bias, gate, next_weight, d_y, d_n, d_x, d_f}));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int bytes = 2 * plan.each * kResThreads * ((s->x_dtype == MOC_F32 ? 4 : 2) + (s->f_dtype == MOC_F32 ? 4 : 2));
+  const int depth = depth_of(plan, bytes, 216 * 1024);
   rc = with_types(s, [&](auto xt, auto ft) {
     return with_plan(plan, [&](auto nv, auto v) {
       auto kern = p.ln ? residual_bwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, true>
                        : residual_bwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, false>;
-      kern<<<sp.blocks, plan.threads, 0, st>>>(p, g);
+      const int groups = kResThreads / (32 * p.group);
+      const size_t shared = std::max(plan.v == 1 ? size_t{0} : static_cast<size_t>(depth) * bytes,
+                                     groups > 1 ? static_cast<size_t>(groups) * p.d * sizeof(float) : size_t{0});
+      MOC_CUDA_OK(allow_shared(kern, shared, 216 * 1024));
+      kern<<<sp.blocks, kResThreads, shared, st>>>(p, g, depth);
       MOC_CUDA_OK(cudaGetLastError());
       return static_cast<int>(MOC_OK);
     });
@@ -517,7 +677,7 @@ extern "C" int moc_gated_residual_bwd(const moc_residual_shape* s, const void* x
     ResSums q{g.partial, g.gate_part, weight, bias, gate, d_weight, d_bias, d_gate, d_next_weight, d_next_bias,
               sp.blocks, p.d, sp.chunks, p.ln, p.gate_rows};
     const unsigned seqs = p.gate_rows && d_gate ? static_cast<unsigned>(sp.items / sp.chunks) : 0u;
-    residual_sums_kernel<<<dim3((p.d + 31) / 32, 1 + seqs), 256, 0, st>>>(q);
+    residual_sums_kernel<<<dim3((p.d + 31) / 32, 1 + seqs), 1024, 0, st>>>(q);
     MOC_CUDA_OK(cudaGetLastError());
   }
   return MOC_OK;
