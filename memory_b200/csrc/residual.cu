@@ -103,27 +103,28 @@ struct RowGroup {
   }
 };
 
-// mean and 1 / sqrt(variance + eps) of the row in `v`; LayerNorm sums twice, as the difference of the mean of
-// squares and the squared mean loses what is small against the mean
-template <int NV, int V>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][V], int ln, float eps, int d, RowGroup& g) {
-  float mean = 0.f, ss = 0.f;
-  if (ln) {
+// mean and 1 / sqrt(variance + eps) of the row in `v`.  Columns past the end hold zeros, which an RMSNorm may sum with the others and
+// a LayerNorm leaves out; it sums twice, as the difference of the mean of squares and the squared mean loses what is small against
+// the mean.
+template <bool LN, int NV, int V>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][V], float eps, int d, RowGroup& g) {
+  float mean = 0.f, ss[2] = {0.f, 0.f};
+  if constexpr (LN) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += (g.t + i * g.n) * V < d ? v[i][j] : 0.f;       // (the affine step leaves its bias in unused columns)
+      for (int j = 0; j < V; ++j) s += (g.t + i * g.n) * V < d ? v[i][j] : 0.f;       // (the affine step leaves its bias there)
     mean = g.sum(s) / static_cast<float>(d);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float u = (g.t + i * g.n) * V + j < d ? v[i][j] - mean : 0.f;
-      ss = fmaf(u, u, ss);
+      const float u = !LN ? v[i][j] : (g.t + i * g.n) * V + j < d ? v[i][j] - mean : 0.f;
+      ss[i & 1] = fmaf(u, u, ss[i & 1]);
     }
-  return make_float2(mean, 1.f / sqrtf(g.sum(ss) / static_cast<float>(d) + eps));
+  return make_float2(mean, 1.f / sqrtf(g.sum(ss[0] + ss[1]) / static_cast<float>(d) + eps));
 }
 
 template <typename T, int NV, int V>
@@ -131,12 +132,9 @@ __device__ __forceinline__ void load_row(const RowGroup& g, const T* p, int d, f
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (g.t + i * g.n) * V;
-    if (c < d) {
-      Piece<T, V>::load(p + c, v[i]);
-    } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) v[i][j] = 0.f;
+    if (c < d) Piece<T, V>::load(p + c, v[i]);
   }
 }
 // A row on its way through shared memory: thread-private slots of one piece, kResThreads of them behind each other.  Single columns
@@ -167,12 +165,14 @@ __device__ __forceinline__ void staged_row(const RowGroup& g, const T* p, int d,
     using Raw = typename Piece<T, V>::Raw;
     const Raw* from = reinterpret_cast<const Raw*>(slots) + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) Piece<T, V>::unpack(from[i * kResThreads], v[i]);       // (what lies in unused slots is put away)
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = (g.t + i * g.n) * V < d ? v[i][j] : 0.f;
+    for (int i = 0; i < NV; ++i) Piece<T, V>::unpack(from[i * kResThreads], v[i]);       // (unused slots hold zeros)
   }
+}
+// zeros in the slots of columns that no row has (this thread's own)
+template <int V> __device__ __forceinline__ void clear_slots(char* slots, int bytes) {
+  if constexpr (V > 1)
+    for (int i = threadIdx.x * 16; i < bytes; i += kResThreads * 16) *reinterpret_cast<uint4*>(slots + i) = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
 }
 // waits until at most `ahead` of this thread's committed rows are still on their way
 __device__ __forceinline__ void wait_rows(int ahead) {
@@ -193,43 +193,33 @@ __device__ __forceinline__ void store_row(const RowGroup& g, T* p, int d, const 
     if (c < d) Piece<T, V>::store(p + c, v[i]);
   }
 }
-// A row of parameters.  Without a branch a piece, so that all are requested together: columns past the end read the first ones,
-// and meet zeros wherever it matters.
-template <int NV, int V>
-__device__ __forceinline__ void load_param(const RowGroup& g, const float* p, int d, float (&a)[NV][V]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (g.t + i * g.n) * V;
-    Piece<float, V>::load(p + (c < d ? c : 0), a[i]);
-  }
-}
-// v = v * w (+ b)
+// v = v * w (+ b); columns past the end meet zeros
 template <int NV, int V>
 __device__ __forceinline__ void affine(const RowGroup& g, float (&v)[NV][V], const float* w, const float* b, int d) {
   float a[NV][V];
-  load_param(g, w, d, a);
+  load_row(g, w, d, a);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) v[i][j] *= a[i][j];
   if (b == nullptr) return;
-  load_param(g, b, d, a);
+  load_row(g, b, d, a);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < V; ++j) v[i][j] += a[i][j];
 }
-template <int NV, int V>
+template <bool LN, int NV, int V>
 __device__ __forceinline__ void normalise(const RowGroup& g, float (&v)[NV][V], float2 st, int d) {
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = (g.t + i * g.n) * V + j < d ? (v[i][j] - st.x) * st.y : 0.f;
+    for (int j = 0; j < V; ++j) v[i][j] = !LN ? v[i][j] * st.y : (g.t + i * g.n) * V + j < d ? (v[i][j] - st.x) * st.y : 0.f;
 }
 
 // depth: rows of a warp group in shared memory at once
-template <typename XT, typename FT, int NV, int V>
-__global__ void __launch_bounds__(kResThreads, NV * V <= 24 ? 2 : 1)
+template <typename XT, typename FT, int NV, int V, bool LN>
+__global__ void __launch_bounds__(kResThreads, NV * V <= 12 ? 4 : NV * V <= 24 ? 2 : 1)
 residual_fwd_kernel(const ResParams p, const int depth) {
   __shared__ float2 red[2 * kResThreads / 32];
   extern __shared__ __align__(16) char slots[];
@@ -251,6 +241,7 @@ residual_fwd_kernel(const ResParams p, const int depth) {
     fill = fill + 1 == depth ? 0 : fill + 1;
   };
   int stage = 0;
+  clear_slots<V>(slots, depth * kSlots);
   for (int i = 1; i < depth; ++i) fetch();
   warm(g, p.w, p.d); warm(g, p.b, p.d); warm(g, p.w2, p.d); warm(g, p.b2, p.d);
   if (!p.gate_rows) warm(g, p.gate, p.d);
@@ -261,8 +252,8 @@ residual_fwd_kernel(const ResParams p, const int depth) {
     staged_row(g, fp + row * p.d, p.d, slots + stage * kSlots, f);
     staged_row(g, xp + row * p.d, p.d, slots + stage * kSlots + kF, x);
     stage = stage + 1 == depth ? 0 : stage + 1;
-    const float2 st = row_stats(f, p.ln, p.eps, p.d, g);
-    normalise(g, f, st, p.d);
+    const float2 st = row_stats<LN>(f, p.eps, p.d, g);
+    normalise<LN>(g, f, st, p.d);
     affine(g, f, p.w, p.b, p.d);
     if (p.gate != nullptr) affine(g, f, p.gate + (p.gate_rows ? row / p.seq * p.d : 0), nullptr, p.d);
 #pragma unroll
@@ -272,8 +263,8 @@ residual_fwd_kernel(const ResParams p, const int depth) {
     store_row(g, static_cast<XT*>(p.y) + row * p.d, p.d, x);
     float2 st2 = make_float2(0.f, 0.f);
     if (p.next) {
-      st2 = row_stats(x, p.ln, p.eps2, p.d, g);
-      normalise(g, x, st2, p.d);
+      st2 = row_stats<LN>(x, p.eps2, p.d, g);
+      normalise<LN>(g, x, st2, p.d);
       affine(g, x, p.w2, p.b2, p.d);
       store_row(g, static_cast<FT*>(p.n) + row * p.d, p.d, x);
     }
@@ -330,6 +321,7 @@ residual_bwd_kernel(const ResParams p, const ResGrads q, const int depth) {
     cp_async_commit();
     fill = fill + 1 == depth ? 0 : fill + 1;
   };
+  clear_slots<V>(slots, depth * kSlots);
   for (int i = 1; i < depth; ++i) fetch();
   for (long long item = first; item < q.items; item += stride) {
     const long long s = item / q.chunks;
@@ -357,7 +349,7 @@ residual_bwd_kernel(const ResParams p, const ResGrads q, const int depth) {
         float y[NV][V], n[NV][V];
         staged_row(g, static_cast<const XT*>(p.x) + row * p.d, p.d, from + kF + kX, y);
         staged_row(g, static_cast<const FT*>(q.dn) + row * p.d, p.d, from + kF + 2 * kX, n);
-        normalise(g, f, make_float2(st.x, st.y), p.d);
+        normalise<LN>(g, f, make_float2(st.x, st.y), p.d);
         {
           float z[NV][V];
 #pragma unroll
@@ -371,7 +363,7 @@ residual_bwd_kernel(const ResParams p, const ResGrads q, const int depth) {
 #pragma unroll
             for (int j = 0; j < V; ++j) y[i][j] = fmaf(p.scale, y[i][j], z[i][j]);
         }
-        normalise(g, y, make_float2(st.z, st.w), p.d);
+        normalise<LN>(g, y, make_float2(st.z, st.w), p.d);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -390,9 +382,9 @@ residual_bwd_kernel(const ResParams p, const ResGrads q, const int depth) {
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if ((g.t + i * g.n) * V + j < p.d) t[i][j] += st.w * (n[i][j] - (LN ? c.y * inv_d : 0.f) - y[i][j] * (c.x * inv_d));
+            if (!LN || (g.t + i * g.n) * V + j < p.d) t[i][j] += st.w * (n[i][j] - (LN ? c.y * inv_d : 0.f) - y[i][j] * (c.x * inv_d));
       } else {
-        normalise(g, f, make_float2(st.x, st.y), p.d);
+        normalise<LN>(g, f, make_float2(st.x, st.y), p.d);
       }
       // t: the gradient at y; f: the normalised branch
       if (q.dx != nullptr) {
@@ -521,10 +513,10 @@ struct Plan {
 };
 // Pieces of four columns wherever rows and base addresses allow 16-byte (fp32) accesses, single columns otherwise.  24 columns a
 // lane fill a row of 768 with one warp; the backward pass of a LayerNorm keeps four sums a column and takes 16.
-Plan plan_of(int d, bool wide, bool lean) {
+Plan plan_of(int d, bool wide, bool lean, bool fwd = false) {
   Plan p;
   p.v = wide ? 4 : 1;
-  p.each = d <= 256 ? 8 : d <= 768 && !lean ? 24 : d <= 4096 ? 16 : 32;
+  p.each = d <= 256 ? 8 : d <= 768 ? (fwd ? 12 : lean ? 16 : 24) : d <= 4096 ? 16 : 32;
   p.group = 1;
   while (p.group * 32 * p.each < d) p.group *= 2;
   return p;
@@ -533,6 +525,7 @@ template <int V, typename Go> int with_each(int each, Go go) {
   using std::integral_constant;
   using W = integral_constant<int, V>;
   if (each == 8) return go(integral_constant<int, 8 / V>{}, W{});
+  if (each == 12) return go(integral_constant<int, 12 / V>{}, W{});
   if (each == 16) return go(integral_constant<int, 16 / V>{}, W{});
   if (each == 24) return go(integral_constant<int, 24 / V>{}, W{});
   return go(integral_constant<int, 32 / V>{}, W{});
@@ -606,16 +599,17 @@ extern "C" int moc_gated_residual_fwd(const moc_residual_shape* s, const void* x
   MOC_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 15) == 0, "stats must be 16-byte aligned");
   ResParams p = params(s, x, f, weight, bias, gate, next_weight, next_bias, stats);
   p.y = y; p.n = n;
-  const Plan plan = plan_of(s->dim, wide(s->dim, {x, f, weight, bias, gate, next_weight, next_bias, y, n}), false);
+  const Plan plan = plan_of(s->dim, wide(s->dim, {x, f, weight, bias, gate, next_weight, next_bias, y, n}), false, true);
   p.group = plan.group;
-  const int groups = kResThreads / (32 * p.group), ctas = plan.each <= 24 ? 2 : 1;         // on an SM
+  const int groups = kResThreads / (32 * p.group), ctas = plan.each <= 12 ? 4 : plan.each <= 24 ? 2 : 1;         // on an SM
   const int bytes = plan.each * kResThreads * ((s->x_dtype == MOC_F32 ? 4 : 2) + (s->f_dtype == MOC_F32 ? 4 : 2));
   const int depth = depth_of(plan, bytes, 160 * 1024 / ctas);          // (the rest is L1, for the parameters)
   const long long most = (p.rows + groups - 1) / groups;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(most, static_cast<long long>(kResCtas) * ctas));
   return with_types(s, [&](auto xt, auto ft) {
     return with_plan(plan, [&](auto nv, auto v) {
-      auto kern = residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value>;
+      auto kern = p.ln ? residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, true>
+                       : residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, false>;
       const size_t shared = plan.v == 1 ? 0 : static_cast<size_t>(depth) * bytes;
       MOC_CUDA_OK(allow_shared(kern, shared, 216 * 1024));
       kern<<<grid, kResThreads, shared, static_cast<cudaStream_t>(stream)>>>(p, depth);
