@@ -12,17 +12,13 @@
 // shared memory, then distributed shared memory.  One sequence, 12 heads, 4,160 rows: 34 us with a CTA per head -> 7.4 with
 // a cluster of eight; 64 sequences: 162 us -> 120.
 //
-// The cache may also be held in 8 bits: e4m3 values v8 with an fp32 scale for each block of `scale_rows` rows, KV head, and K
-// or V (moc_quantize_rows).  A row's scale leaves the products, so the values go into them as they are stored:
-//   s_r = scale * u_c * ks_r * <q, K8[r]>,   out = sum_r softmax(s)_r * (u_c * vs_r) * V8[r].
-// e4m3 -> fp16 is exact, and everything from there on is fp32, as with the bf16 cache.
-#include <cuda_fp16.h>
-
-#include <type_traits>
-
+// A cache in 8 bits has kernels of its own (decode_attn8.cu).
 #include "host_pass.cuh"
 
 namespace moc {
+int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* values, const float* scales, int scale_rows, int64_t bank_rows,
+                     const int32_t* comb_idx, const float* comb_w, const int32_t* counts, void* out, float* lse, int32_t* status,
+                     void* stream);
 namespace {
 
 constexpr int kDD = 64;
@@ -46,20 +42,8 @@ __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
 constexpr int kDecUnroll = 8;
 constexpr int kDecRows = 4 * kDecUnroll;
 
-// four e4m3 values -> two pairs of fp32
-__device__ __forceinline__ void unpack_e4m3(uint32_t v, uint64_t& lo, uint64_t& hi) {
-  uint32_t h0, h1;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(h0), "=r"(h1) : "r"(v));
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-  lo = f2_pack(a.x, a.y);
-  hi = f2_pack(b.x, b.y);
-}
-
 struct DecodeParams {
-  const __nv_bfloat16* q;
-  const void* kv_bank;
-  const float* kv_scale;               // 8-bit cache: [bank_rows / scale_rows, 2 * HK]
+  const __nv_bfloat16 *q, *kv_bank;
   long long bank_rows;
   const int* comb_idx;
   const float* comb_w;
@@ -68,18 +52,14 @@ struct DecodeParams {
   float* lse;
   int n_q, H, HK, n_ch, T, split;
   float scale;
-  FastDiv scale_rows;
   int* status;
 };
 
-// K8: the cache is held in 8 bits.
-template <int G, bool K8>
+template <int G>
 __global__ void __launch_bounds__(kDecThreads, G == 1 ? 2 : 1)
 decode_attn_kernel(const DecodeParams p) {
   __shared__ __align__(16) float red[G][kDecWarps][kDD + 4];
   __shared__ __align__(16) float cta_part[G][kDD + 4];        // accumulator, maximum, sum of this CTA
-  using Elem = typename std::conditional<K8, uint8_t, __nv_bfloat16>::type;
-  using Raw = typename std::conditional<K8, uint2, uint4>::type;           // eight elements
   const int split = p.split, H = p.H, HK = p.HK, T = p.T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rg = lane >> 3, part = lane & 7;          // row group 0..3, 8-element slice of the head dimension
@@ -113,51 +93,29 @@ decode_attn_kernel(const DecodeParams p) {
       continue;
     }
     const float u = weights[c];
-    const Elem* base = static_cast<const Elem*>(p.kv_bank) + static_cast<long long>(ch) * T * row_elems + kh * kDD + part * 8;
-    Raw kr[kDecUnroll], vr[kDecUnroll];
+    const __nv_bfloat16* base = p.kv_bank + static_cast<long long>(ch) * T * row_elems + kh * kDD + part * 8;
+    uint4 kr[kDecUnroll], vr[kDecUnroll];
 #pragma unroll
     for (int sidx = 0; sidx < kDecUnroll; ++sidx) {
       const int r = r0 + sidx * 4 + rg;
-      const Elem* rp = base + static_cast<long long>(r < T ? r : 0) * row_elems;
-      kr[sidx] = *reinterpret_cast<const Raw*>(rp);
-      vr[sidx] = *reinterpret_cast<const Raw*>(rp + HK * kDD);
-    }
-    const int own = r0 + part * 4 + rg;               // the row whose score this lane ends up with
-    const bool in = own < T;
-    float ks = 1.f, vs = 1.f;
-    if constexpr (K8) {
-      const long long blk = static_cast<long long>(ch) * (T / p.scale_rows.d) + div_of(in ? own : 0, p.scale_rows);
-      ks = p.kv_scale[blk * 2 * HK + kh];
-      vs = p.kv_scale[blk * 2 * HK + HK + kh];
+      const __nv_bfloat16* rp = base + static_cast<long long>(r < T ? r : 0) * row_elems;
+      kr[sidx] = *reinterpret_cast<const uint4*>(rp);
+      vr[sidx] = *reinterpret_cast<const uint4*>(rp + HK * kDD);
     }
     float dot[G][kDecUnroll];
 #pragma unroll
     for (int sidx = 0; sidx < kDecUnroll; ++sidx) {
-      if constexpr (K8) {
-        uint64_t f[4];
-        unpack_e4m3(kr[sidx].x, f[0], f[1]);
-        unpack_e4m3(kr[sidx].y, f[2], f[3]);
+      float f[8];
+      unpack8(kr[sidx], f);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          uint64_t t = f2_mul(f2_pack(qf[g][0], qf[g][1]), f[0]);
+      for (int g = 0; g < G; ++g) {
+        float t = 0.f;
 #pragma unroll
-          for (int j = 1; j < 4; ++j) t = f2_fma(f2_pack(qf[g][2 * j], qf[g][2 * j + 1]), f[j], t);
-          float lo, hi;
-          f2_unpack(t, lo, hi);
-          dot[g][sidx] = lo + hi;
-        }
-      } else {
-        float f[8];
-        unpack8(kr[sidx], f);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float t = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) t = fmaf(qf[g][j], f[j], t);
-          dot[g][sidx] = t;
-        }
+        for (int j = 0; j < 8; ++j) t = fmaf(qf[g][j], f[j], t);
+        dot[g][sidx] = t;
       }
     }
+    const bool in = r0 + part * 4 + rg < T;           // the row whose score this lane ends up with
     float pu[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -171,7 +129,7 @@ decode_attn_kernel(const DecodeParams p) {
           dot[g][i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
         }
       }
-      const float sc = in ? (K8 ? dot[g][0] * ks : dot[g][0]) * u * c2 : -INFINITY;
+      const float sc = in ? dot[g][0] * u * c2 : -INFINITY;
       float mx = fmaxf(sc, __shfl_xor_sync(0xffffffffu, sc, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
@@ -180,35 +138,20 @@ decode_attn_kernel(const DecodeParams p) {
       const float corr = exp2f(m[g] - ref);                    // 0 on the first rows (m = -inf)
       const float pr = exp2f(sc - ref);
       l[g] = l[g] * corr + pr;
-      pu[g] = K8 ? pr * (in ? u * vs : 0.f) : pr * u;
+      pu[g] = pr * u;
       m[g] = m_new;
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[g][j] *= corr;
     }
 #pragma unroll
     for (int sidx = 0; sidx < kDecUnroll; ++sidx) {
-      if constexpr (K8) {
-        uint64_t f[4];
-        unpack_e4m3(vr[sidx].x, f[0], f[1]);
-        unpack_e4m3(vr[sidx].y, f[2], f[3]);
+      float f[8];
+      unpack8(vr[sidx], f);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float w = __shfl_sync(0xffffffffu, pu[g], (lane & 24) | sidx);
+      for (int g = 0; g < G; ++g) {
+        const float w = __shfl_sync(0xffffffffu, pu[g], (lane & 24) | sidx);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t a = f2_fma(f2_pack(w, w), f[j], f2_pack(acc[g][2 * j], acc[g][2 * j + 1]));
-            f2_unpack(a, acc[g][2 * j], acc[g][2 * j + 1]);
-          }
-        }
-      } else {
-        float f[8];
-        unpack8(vr[sidx], f);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float w = __shfl_sync(0xffffffffu, pu[g], (lane & 24) | sidx);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[g][j] = fmaf(w, f[j], acc[g][j]);
-        }
+        for (int j = 0; j < 8; ++j) acc[g][j] = fmaf(w, f[j], acc[g][j]);
       }
     }
   }
@@ -268,76 +211,11 @@ decode_attn_kernel(const DecodeParams p) {
         a = a * f0 + ((e & 1) ? ab.y : ab.x) * f1;
         mt = m_new;
       }
-      // (a list without rows has no sum; with the 8-bit cache a NaN in it, or in the query, stays one)
-      const bool any = K8 ? lt != 0.f : lt > 0.f;
-      p.out[(q_row + h0 + g) * kDD + e] = __float2bfloat16(any ? a / lt : 0.f);
-      if (e == 0 && p.lse != nullptr) p.lse[q_row + h0 + g] = any ? (mt + log2f(lt)) / kDecLog2e : -INFINITY;
+      p.out[(q_row + h0 + g) * kDD + e] = __float2bfloat16(lt > 0.f ? a / lt : 0.f);
+      if (e == 0 && p.lse != nullptr) p.lse[q_row + h0 + g] = lt > 0.f ? (mt + log2f(lt)) / kDecLog2e : -INFINITY;
     }
   }
   if (split > 1) cluster_sync();       // nobody leaves while its part is read
-}
-
-// values = e4m3(x / scale), scale = (largest |x|) / 448 of each block of `block` rows and one head of 64 columns; a warp takes a
-// block, eight lanes a row (16 bytes of its 128 each), four rows a load.  Blocks of up to 4 R rows stay in registers; longer ones
-// are read a second time.  A block of zeros has scale 0 and values 0; one with a NaN or an infinity gets a scale that is
-// NaN or infinite and stands for NaN as a whole.  Bound by HBM (2 bytes read and 1 written an element) once the quotient is a product
-// corrected by its remainder (Markstein), equal to the division where its last bit can matter: 262,208 x 1,536: 371 us with
-// divisions, 245 with products.
-template <int R>
-__global__ void __launch_bounds__(kDecThreads)
-quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int heads, int block, uint8_t* __restrict__ values,
-                     float* __restrict__ scales) {
-  const long long tile = static_cast<long long>(blockIdx.x) * kDecWarps + (threadIdx.x >> 5);
-  if (tile >= tiles) return;
-  const int lane = threadIdx.x & 31, rg = lane >> 3, part = lane & 7;
-  const long long blk = tile / heads;
-  const int head = static_cast<int>(tile - blk * heads);
-  const long long width = static_cast<long long>(heads) * kDD, first = blk * block * width + head * kDD + part * 8;
-  uint4 raw[R];
-  uint32_t top2 = 0;                 // magnitudes order like their bits, NaN above infinity; two columns at a time
-  auto most = [&](uint32_t v) { asm("max.u16x2 %0, %0, %1;" : "+r"(top2) : "r"(v & 0x7FFF7FFFu)); };
-  for (int r0 = 0; r0 < block; r0 += 4 * R) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + 4 * i + rg;
-      raw[i] = r < block ? __ldcs(reinterpret_cast<const uint4*>(x + first + r * width)) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) { most(raw[i].x); most(raw[i].y); most(raw[i].z); most(raw[i].w); }
-  }
-  const uint32_t bits = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
-  const float scale = __uint_as_float(bits << 16) * (1.f / 448.f);       // (a product, as torch divides by a constant: the last bit follows it)
-  if (lane == 0) scales[tile] = scale;
-  // A quotient of the correction below its range (x < 2^-100) rounds to 0 all the same while the scale is above 2^-80.
-  const bool plain = scale > 0x1p-80f && scale < 0x1p80f;
-  const float inv = plain ? 1.f / scale : 0.f;
-  for (int r0 = 0; r0 < block; r0 += 4 * R) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + 4 * i + rg;
-      if (r >= block) continue;
-      if (block > 4 * R) raw[i] = *reinterpret_cast<const uint4*>(x + first + r * width);
-      float f[8];
-      unpack8(raw[i], f);
-      if (plain) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float q = f[j] * inv;
-          f[j] = fmaf(fmaf(-q, scale, f[j]), inv, q);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = scale > 0.f ? f[j] / scale : 0.f;
-      }
-      uint32_t w[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
-            "mov.b32 %0, {a, b};\n\t}"
-            : "=r"(w[j]) : "f"(f[4 * j]), "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3]));
-      __stcs(reinterpret_cast<uint2*>(values + first + r * width), make_uint2(w[0], w[1]));
-    }
-  }
 }
 
 // dst[b] = the last dst_rows of (cache[b] followed by h[b]); rows of 16-byte pieces
@@ -376,10 +254,8 @@ int64_t carve(const moc_decode_step_desc* s, StepArena* a) {
 
 using namespace moc;
 
-template <bool K8>
-static int decode_attn(const moc_decode_shape* s, const void* q, const void* kv_bank, const float* kv_scale, int scale_rows,
-                       int64_t bank_rows, const int32_t* comb_idx, const float* comb_w, const int32_t* counts, void* out, float* lse,
-                       int32_t* status, void* stream_) {
+static int decode_attn(const moc_decode_shape* s, const void* q, const void* kv_bank, int64_t bank_rows, const int32_t* comb_idx,
+                       const float* comb_w, const int32_t* counts, void* out, float* lse, int32_t* status, void* stream_) {
   MOC_REQUIRE(s && q && kv_bank && comb_idx && comb_w && out && status, "NULL decode-attention argument");
   MOC_REQUIRE(s->head_dim == kDD, "decode attention needs head_dim 64");
   MOC_REQUIRE(s->batch > 0 && s->n_q > 0 && s->n_chapters > 0 && s->tokens_per_chapter > 0 && bank_rows > 0,
@@ -392,8 +268,8 @@ static int decode_attn(const moc_decode_shape* s, const void* q, const void* kv_
   // query heads that share a KV head go together: their rows are fetched once
   const int per_kv = s->num_heads / s->num_kv_heads;
   const int group = per_kv % 4 == 0 ? 4 : per_kv % 3 == 0 ? 3 : per_kv % 2 == 0 ? 2 : 1;
-  auto kern = group == 4 ? decode_attn_kernel<4, K8> : group == 3 ? decode_attn_kernel<3, K8>
-              : group == 2 ? decode_attn_kernel<2, K8> : decode_attn_kernel<1, K8>;
+  auto kern = group == 4 ? decode_attn_kernel<4> : group == 3 ? decode_attn_kernel<3>
+              : group == 2 ? decode_attn_kernel<2> : decode_attn_kernel<1>;
   // A cluster per group while all of them are resident at once and every warp has rows to take.  How many are depends on
   // the registers (an SM holds two CTAs of one head, one of a group) and on what is left of each GPC beside whole clusters:
   // 33 clusters of eight single-head CTAs, 15 of grouped ones.  With 296 slots counted for either, 12 heads on 4 KV heads
@@ -405,10 +281,10 @@ static int decode_attn(const moc_decode_shape* s, const void* q, const void* kv_
   while (split > 1 && (split / 2 * kDecWarps >= units || groups > resident_clusters(kern, kDecThreads, 0, split))) split /= 2;
   dim3 grid(s->num_heads / group * split, s->n_q, s->batch);
   DecodeParams p{};
-  p.q = static_cast<const __nv_bfloat16*>(q); p.kv_bank = kv_bank; p.kv_scale = kv_scale; p.bank_rows = bank_rows;
+  p.q = static_cast<const __nv_bfloat16*>(q); p.kv_bank = static_cast<const __nv_bfloat16*>(kv_bank); p.bank_rows = bank_rows;
   p.comb_idx = comb_idx; p.comb_w = comb_w; p.counts = counts; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
   p.n_q = s->n_q; p.H = s->num_heads; p.HK = s->num_kv_heads; p.n_ch = s->n_chapters; p.T = s->tokens_per_chapter;
-  p.split = split; p.scale = s->scale; p.scale_rows = fast_div(scale_rows); p.status = status;
+  p.split = split; p.scale = s->scale; p.status = status;
   MOC_CUDA_OK(launch_clustered(kern, grid, kDecThreads, 0, split, static_cast<cudaStream_t>(stream_), p));
   MOC_CUDA_OK(cudaGetLastError());
   return MOC_OK;
@@ -417,35 +293,14 @@ static int decode_attn(const moc_decode_shape* s, const void* q, const void* kv_
 extern "C" int moc_decode_attn(const moc_decode_shape* s, const void* q, const void* kv_bank, int64_t bank_rows,
                                const int32_t* comb_idx, const float* comb_w, void* out, float* lse,
                                int32_t* status, void* stream) {
-  return decode_attn<false>(s, q, kv_bank, nullptr, 1, bank_rows, comb_idx, comb_w, nullptr, out, lse, status, stream);
+  return decode_attn(s, q, kv_bank, bank_rows, comb_idx, comb_w, nullptr, out, lse, status, stream);
 }
 
 extern "C" int moc_decode_attn_cache(const moc_decode_shape* s, const void* q, const void* kv_bank, const float* kv_scale,
                                      int32_t scale_rows, int64_t bank_rows, const int32_t* comb_idx, const float* comb_w,
                                      const int32_t* counts, void* out, float* lse, int32_t* status, void* stream) {
-  if (kv_scale == nullptr)
-    return decode_attn<false>(s, q, kv_bank, nullptr, 1, bank_rows, comb_idx, comb_w, counts, out, lse, status, stream);
-  MOC_REQUIRE(s != nullptr && scale_rows > 0 && s->tokens_per_chapter > 0 && s->tokens_per_chapter % scale_rows == 0,
-              "a chapter must be whole blocks of scale_rows");
-  return decode_attn<true>(s, q, kv_bank, kv_scale, scale_rows, bank_rows, comb_idx, comb_w, counts, out, lse, status, stream);
-}
-
-extern "C" int moc_quantize_rows(const void* rows_bf16, int64_t rows, int32_t heads, int32_t head_dim, int32_t scale_rows,
-                                 void* values, float* scales, void* stream) {
-  MOC_REQUIRE(rows_bf16 && values && scales, "NULL quantisation buffer");
-  MOC_REQUIRE(head_dim == kDD, "the 8-bit cache needs head_dim 64");
-  MOC_REQUIRE(rows > 0 && heads > 0 && scale_rows > 0 && rows % scale_rows == 0, "rows must be whole blocks of scale_rows");
-  MOC_REQUIRE(((reinterpret_cast<uintptr_t>(rows_bf16) | reinterpret_cast<uintptr_t>(values)) & 15) == 0,
-              "rows and values must be 16-byte aligned");
-  const long long tiles = rows / scale_rows * heads;
-  MOC_REQUIRE(tiles < (1ll << 33), "too many blocks in one call");
-  const unsigned grid = static_cast<unsigned>((tiles + kDecWarps - 1) / kDecWarps);
-  auto kern = scale_rows <= 8 ? quantize_rows_kernel<2> : scale_rows <= 16 ? quantize_rows_kernel<4>
-              : scale_rows <= 32 ? quantize_rows_kernel<8> : quantize_rows_kernel<16>;
-  kern<<<grid, kDecThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(rows_bf16), tiles, heads,
-                                                                   scale_rows, static_cast<uint8_t*>(values), scales);
-  MOC_CUDA_OK(cudaGetLastError());
-  return MOC_OK;
+  if (kv_scale == nullptr) return decode_attn(s, q, kv_bank, bank_rows, comb_idx, comb_w, counts, out, lse, status, stream);
+  return decode_attn_e4m3(s, q, kv_bank, kv_scale, scale_rows, bank_rows, comb_idx, comb_w, counts, out, lse, status, stream);
 }
 
 extern "C" int moc_roll_window(const void* cache, int64_t cache_stride, int32_t cache_rows, const void* h, int64_t h_stride,

@@ -1,0 +1,458 @@
+// Decode-time memory attention over a cache of projected bank rows held in 8 bits, and the cache's making.
+//
+// The cache is e4m3 values v8 with an fp32 scale for each block of `scale_rows` rows, KV head, and K or V.  A row's scale leaves the
+// products, so the values go into them as they are stored (u_c: the weight of chapter c):
+//   s_r = scale * u_c * ks_r * <q, K8[r]>,   out = sum_r softmax(s)_r * u_c * vs_r * V8[r]   (one joint softmax).
+//
+// Bound by HBM for a full batch (one byte an element), by latency for a few sequences.  All queries on a KV head (its heads, the
+// tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted once for up to 16 of them;
+// e4m3 -> fp16 is exact.  On CUDA cores a unit of 32 rows took 554 instructions (64 sequences of 4,160 rows, 12 heads: 95 us, bound by
+// issuing); with matrix instructions of single warps about half, whatever the number of columns.
+//   - scores: A = 16 keys x 16 dims, B = dims x 8 queries.  The order of the dims is free, so a lane's 16 bytes of its row are
+//     the A fragments of four steps as they come.  Queries are scaled by a power of two into fp16's range (their largest to
+//     128..256; what falls below fp16's smallest number is 2^-31 of the largest).
+//   - values: A = 16 dims x 16 rows, transposed from rows by byte permutations within a lane; B = the probabilities, which a matrix
+//     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
+//     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
+// Maxima, sums and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts
+// merge through shared memory, then distributed shared memory.
+#include <cuda_fp16.h>
+
+#include "host_pass.cuh"
+
+namespace moc {
+namespace {
+
+constexpr int kDD = 64, kThreads = 256, kWarps = kThreads / 32, kRows = 32;      // rows of a unit
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Attn8Params {
+  const __nv_bfloat16* q;
+  const uint8_t* values;
+  const float* scales;                 // [bank_rows / scale_rows, 2 * HK]
+  long long bank_rows;
+  const int* comb_idx;
+  const float* comb_w;
+  const int* counts;                   // chapters of each list that count (NULL: all)
+  __nv_bfloat16* out;
+  float* lse;
+  int n_q, H, HK, n_ch, T, split, tiles;        // tiles of columns of a KV head
+  float scale;
+  FastDiv scale_rows, runs;
+  int* status;
+};
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t two) {       // the low 16 bits
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16_high(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {           // of a warp's 8 x 8 matrix of 16-bit values
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// NT: tiles of 8 columns.  Lane (g, t) = (lane / 4, lane % 4).
+template <int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+decode_attn8_kernel(const Attn8Params p) {
+  constexpr int kCols = 8 * NT;
+  __shared__ __align__(16) float red[kCols][kWarps][kDD + 4];
+  __shared__ __align__(16) float cta_part[kCols][kDD + 4];        // accumulator, maximum, sum of this CTA
+  const int split = p.split, HK = p.HK, T = p.T;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int rank = static_cast<int>(blockIdx.x) % split, tile = static_cast<int>(blockIdx.x) / split % p.tiles;
+  const int kh = static_cast<int>(blockIdx.x) / split / p.tiles, b = blockIdx.y;
+  const int per_kv = p.H / HK, columns = min(kCols, p.n_q * per_kv - tile * kCols);      // column j: token j / per_kv, head kh per_kv + j % per_kv
+  const long long row_bytes = 2ll * HK * kDD;
+  auto q_row = [&](int col) {
+    const int j = tile * kCols + col, iq = j / per_kv;
+    return (static_cast<long long>(b) * p.n_q + iq) * p.H + kh * per_kv + (j - iq * per_kv);
+  };
+  int n_ch = p.n_ch;
+  if (p.counts != nullptr) n_ch = max(0, min(n_ch, p.counts[b]));
+  const int* list = p.comb_idx + static_cast<long long>(b) * p.n_ch;
+  const float* weights = p.comb_w + static_cast<long long>(b) * p.n_ch;
+
+  // queries: B fragments (column g, dims 16 t + 4 s + {0, 1} and {2, 3} in step s), and the factors of this lane's score columns
+  uint32_t qb[NT][4][2];
+  float factor[NT][2], acc[NT][4][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float f[16], top = 0.f;
+    const int col = nt * 8 + g;
+    const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row(col < columns ? col : 0) * kDD + 16 * t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 raw = src[h];
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[8 * h + 2 * i] = col < columns ? __uint_as_float(w[i] << 16) : 0.f;
+        f[8 * h + 2 * i + 1] = col < columns ? __uint_as_float(w[i] & 0xFFFF0000u) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(f[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = static_cast<int>(__float_as_uint(top) >> 23);          // of 2^(e - 127); infinite queries and tiny ones stay as they are
+    const bool shift = e > 27 && e < 255;
+    const float up = shift ? __uint_as_float(static_cast<uint32_t>(261 - e) << 23) : 1.f;       // 2^(134 - e)
+    const float down = shift ? __uint_as_float(static_cast<uint32_t>(max(e - 7, 1)) << 23) : 1.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      qb[nt][s][0] = pack_f16(f[4 * s] * up, f[4 * s + 1] * up);
+      qb[nt][s][1] = pack_f16(f[4 * s + 2] * up, f[4 * s + 3] * up);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      factor[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale * kLog2e;
+      m[nt][j] = -INFINITY;
+      l[nt][j] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.f;
+  }
+
+  const bool one_block = p.scale_rows.d % kRows == 0;          // a unit lies in one block of scales
+  for (int unit = rank * kWarps + warp; unit < n_ch * p.runs.d; unit += split * kWarps) {
+    const int c = div_of(unit, p.runs), r0 = (unit - c * p.runs.d) * kRows;
+    const int ch = list[c];
+    if (ch < 0 || (static_cast<long long>(ch) + 1) * T > p.bank_rows) {
+      if (lane == 0) atomicMax(p.status, MOC_DEV_BAD_INDEX);
+      continue;
+    }
+    const float u = weights[c];
+    const uint8_t* chapter = p.values + static_cast<long long>(ch) * T * row_bytes + kh * kDD;
+    uint4 kr[2][2];                    // rows 16 mt + g and + 8, bytes 16 t ..
+    uint2 vr[2][4];                    // rows 16 ks + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}, bytes 8 g ..
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = r0 + 16 * mt + 8 * h + g;
+        kr[mt][h] = *reinterpret_cast<const uint4*>(chapter + (r < T ? r : 0) * row_bytes + 16 * t);
+      }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * ks + 2 * t + (i & 1) + 8 * (i >> 1);
+        vr[ks][i] = *reinterpret_cast<const uint2*>(chapter + (r < T ? r : 0) * row_bytes + HK * kDD + 8 * g);
+      }
+    // row factors of this lane's four rows (mt, h): scores, and values relative to `w_top`
+    float kf[2][2], vf[2][2], w_top;
+    const long long blk0 = static_cast<long long>(ch) * (T / p.scale_rows.d);
+    if (one_block) {
+      const float* sc = p.scales + (blk0 + div_of(r0, p.scale_rows)) * 2 * HK + kh;
+      const float ks = sc[0] * u;
+      w_top = sc[HK] * u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { kf[i >> 1][i & 1] = ks; vf[i >> 1][i & 1] = 1.f; }
+    } else {
+      w_top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * (i >> 1) + 8 * (i & 1) + g;
+        const float* sc = p.scales + (blk0 + div_of(r < T ? r : 0, p.scale_rows)) * 2 * HK + kh;
+        kf[i >> 1][i & 1] = sc[0] * u;
+        vf[i >> 1][i & 1] = sc[HK];
+        w_top = max_nan(w_top, sc[HK]);
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) w_top = max_nan(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
+      const float inv = w_top > 0.f ? 1.f / w_top : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vf[i >> 1][i & 1] *= inv;
+      w_top *= u;
+    }
+    uint32_t pb[NT][2][2];             // probabilities as B fragments: rows 16 ks + 2 t + {0, 1} and + 8, column g
+    float corr[NT][2];
+    bool moved = false;
+    {
+      float sc[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint32_t lo[4] = {kr[mt][0].x, kr[mt][0].y, kr[mt][0].z, kr[mt][0].w}, hi[4] = {kr[mt][1].x, kr[mt][1].y, kr[mt][1].z, kr[mt][1].w};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[mt][nt][j] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t a0 = e4m3x2_to_f16(lo[s]), a1 = e4m3x2_to_f16(hi[s]), a2 = e4m3x2_to_f16_high(lo[s]), a3 = e4m3x2_to_f16_high(hi[s]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[mt][nt], a0, a1, a2, a3, qb[nt][s][0], qb[nt][s][1]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {           // rows (mt, h) = (i / 2, i % 2)
+            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+            s = r0 + 16 * (i >> 1) + 8 * (i & 1) + g < T ? s * kf[i >> 1][i & 1] * factor[nt][j] : -INFINITY;
+            top = fmaxf(top, s);
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float m_new = fmaxf(m[nt][j], top), ref = m_new == -INFINITY ? 0.f : m_new;
+          corr[nt][j] = exp2_fast(m[nt][j] - ref);               // 0 on the first rows (m = -inf)
+          moved |= m_new != m[nt][j];
+          m[nt][j] = m_new;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+            s = exp2_fast(s - ref);
+            sum += s;
+          }
+          l[nt][j] = fmaf(l[nt][j], corr[nt][j], sum);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1]));
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[nt][i][j] *= corr[nt][j & 1];
+    }
+    // values: tile i of 16 dims, dims 8 g + 2 i (fragment row g) and 8 g + 2 i + 1 (row g + 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[nt][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+        const uint32_t v01 = __byte_perm(i < 2 ? vr[ks][0].x : vr[ks][0].y, i < 2 ? vr[ks][1].x : vr[ks][1].y, sel);
+        const uint32_t v89 = __byte_perm(i < 2 ? vr[ks][2].x : vr[ks][2].y, i < 2 ? vr[ks][3].x : vr[ks][3].y, sel);
+        const uint32_t a0 = e4m3x2_to_f16(v01), a1 = e4m3x2_to_f16_high(v01), a2 = e4m3x2_to_f16(v89), a3 = e4m3x2_to_f16_high(v89);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nt][i][j] = fmaf(w_top, d[nt][j], acc[nt][i][j]);
+    }
+  }
+
+  // a warp's part: columns 2 t + j, dims 8 g ..
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum = l[nt][j];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int col = nt * 8 + 2 * t + j;
+      float* to = red[col][warp];
+      *reinterpret_cast<float4*>(to + 8 * g) = make_float4(acc[nt][0][j], acc[nt][0][2 + j], acc[nt][1][j], acc[nt][1][2 + j]);
+      *reinterpret_cast<float4*>(to + 8 * g + 4) = make_float4(acc[nt][2][j], acc[nt][2][2 + j], acc[nt][3][j], acc[nt][3][2 + j]);
+      if (g == 0) {
+        to[kDD] = m[nt][j];
+        to[kDD + 1] = sum;
+      }
+    }
+  __syncthreads();
+  // warps -> CTA: thread i finishes output element i % 64 of column i / 64
+  for (int i = threadIdx.x; i < columns * kDD; i += kThreads) {
+    const int col = i / kDD, e = i % kDD;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, red[col][w][kDD]);
+    float lt = 0.f, a = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = (red[col][w][kDD] == -INFINITY) ? 0.f : exp2f(red[col][w][kDD] - mt);
+      // (a warp whose scores are all NaN has no maximum, but a sum that is NaN)
+      lt += red[col][w][kDD] == -INFINITY && red[col][w][kDD + 1] == 0.f ? 0.f : red[col][w][kDD + 1] * f;
+      a += red[col][w][e] * f;
+    }
+    cta_part[col][e] = a;
+    if (e == 0) { cta_part[col][kDD] = mt; cta_part[col][kDD + 1] = lt; }
+  }
+  // CTAs -> output: the cluster's first CTA reads the others' parts (one of its own needs no barrier beyond the CTA's)
+  if (split > 1) cluster_sync(); else __syncthreads();
+  if (rank == 0) {
+    for (int i = threadIdx.x; i < columns * kDD; i += kThreads) {
+      const int col = i / kDD, e = i % kDD;
+      const uint32_t stat = smem_u32(&cta_part[col][kDD]), elem = smem_u32(&cta_part[col][e & ~1]);
+      float mt = -INFINITY, lt = 0.f, a = 0.f;
+      for (int r = 0; r < split; ++r) {
+        const float2 st = split > 1 ? cluster_ld2(cluster_map(stat, r)) : make_float2(cta_part[col][kDD], cta_part[col][kDD + 1]);
+        const float2 ab = split > 1 ? cluster_ld2(cluster_map(elem, r)) : make_float2(cta_part[col][e & ~1], cta_part[col][e | 1]);
+        const float m_new = fmaxf(mt, st.x);
+        const float f0 = mt == -INFINITY ? 0.f : exp2f(mt - m_new), f1 = st.x == -INFINITY ? 0.f : exp2f(st.x - m_new);
+        lt = lt * f0 + st.y * f1;
+        a = a * f0 + ((e & 1) ? ab.y : ab.x) * f1;
+        mt = m_new;
+      }
+      const bool any = lt != 0.f;                // (a list without rows has no sum; a NaN in the cache or the query stays one)
+      p.out[q_row(col) * kDD + e] = __float2bfloat16(any ? a / lt : 0.f);
+      if (e == 0 && p.lse != nullptr) p.lse[q_row(col)] = any ? (mt + log2f(lt)) / kLog2e : -INFINITY;
+    }
+  }
+  if (split > 1) cluster_sync();       // nobody leaves while its part is read
+}
+
+__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+
+// values = e4m3(x / scale), scale = (largest |x|) / 448 of each block of `block` rows and one head of 64 columns; a warp takes a
+// block, eight lanes a row (16 bytes of its 128 each), four rows a load.  Blocks of up to 4 R rows stay in registers; longer ones
+// are read a second time.  A block of zeros has scale 0 and values 0; one with a NaN or an infinity gets a scale that is
+// NaN or infinite and stands for NaN as a whole.  Bound by HBM (2 bytes read and 1 written an element) once the quotient is a product
+// corrected by its remainder (Markstein), equal to the division where its last bit can matter: 262,208 x 1,536: 371 us with
+// divisions, 245 with products.
+template <int R>
+__global__ void __launch_bounds__(kThreads)
+quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int heads, int block, uint8_t* __restrict__ values,
+                     float* __restrict__ scales) {
+  const long long tile = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  if (tile >= tiles) return;
+  const int lane = threadIdx.x & 31, rg = lane >> 3, part = lane & 7;
+  const long long blk = tile / heads;
+  const int head = static_cast<int>(tile - blk * heads);
+  const long long width = static_cast<long long>(heads) * kDD, first = blk * block * width + head * kDD + part * 8;
+  uint4 raw[R];
+  uint32_t top2 = 0;                 // magnitudes order like their bits, NaN above infinity; two columns at a time
+  auto most = [&](uint32_t v) { asm("max.u16x2 %0, %0, %1;" : "+r"(top2) : "r"(v & 0x7FFF7FFFu)); };
+  for (int r0 = 0; r0 < block; r0 += 4 * R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + 4 * i + rg;
+      raw[i] = r < block ? __ldcs(reinterpret_cast<const uint4*>(x + first + r * width)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) { most(raw[i].x); most(raw[i].y); most(raw[i].z); most(raw[i].w); }
+  }
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
+  const float scale = __uint_as_float(bits << 16) * (1.f / 448.f);       // (a product, as torch divides by a constant: the last bit follows it)
+  if (lane == 0) scales[tile] = scale;
+  // A quotient of the correction below its range (x < 2^-100) rounds to 0 all the same while the scale is above 2^-80.
+  const bool plain = scale > 0x1p-80f && scale < 0x1p80f;
+  const float inv = plain ? 1.f / scale : 0.f;
+  for (int r0 = 0; r0 < block; r0 += 4 * R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int r = r0 + 4 * i + rg;
+      if (r >= block) continue;
+      if (block > 4 * R) raw[i] = *reinterpret_cast<const uint4*>(x + first + r * width);
+      float f[8];
+      unpack8(raw[i], f);
+      if (plain) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float q = f[j] * inv;
+          f[j] = fmaf(fmaf(-q, scale, f[j]), inv, q);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = scale > 0.f ? f[j] / scale : 0.f;
+      }
+      uint32_t w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        asm("{\n\t.reg .b16 a, b;\n\tcvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+            "mov.b32 %0, {a, b};\n\t}"
+            : "=r"(w[j]) : "f"(f[4 * j]), "f"(f[4 * j + 1]), "f"(f[4 * j + 2]), "f"(f[4 * j + 3]));
+      __stcs(reinterpret_cast<uint2*>(values + first + r * width), make_uint2(w[0], w[1]));
+    }
+  }
+}
+
+}  // namespace
+
+int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* values, const float* scales, int scale_rows, int64_t bank_rows,
+                     const int32_t* comb_idx, const float* comb_w, const int32_t* counts, void* out, float* lse, int32_t* status,
+                     void* stream) {
+  MOC_REQUIRE(s && q && values && scales && comb_idx && comb_w && out && status, "NULL decode-attention argument");
+  MOC_REQUIRE(s->head_dim == kDD, "decode attention needs head_dim 64");
+  MOC_REQUIRE(s->batch > 0 && s->n_q > 0 && s->n_chapters > 0 && s->tokens_per_chapter > 0 && bank_rows > 0, "empty decode-attention problem");
+  MOC_REQUIRE(s->num_heads > 0 && s->num_kv_heads > 0 && s->num_heads % s->num_kv_heads == 0,
+              "num_heads must be a positive multiple of num_kv_heads");
+  MOC_REQUIRE(scale_rows > 0 && s->tokens_per_chapter % scale_rows == 0, "a chapter must be whole blocks of scale_rows");
+  MOC_REQUIRE(s->n_q <= 65535 && s->batch <= 65535, "too many query tokens or sequences for one launch");
+  MOC_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(values)) & 15) == 0, "q and the K/V cache must be 16-byte aligned");
+  const long long columns = static_cast<long long>(s->n_q) * (s->num_heads / s->num_kv_heads);
+  const int nt = columns <= 8 ? 1 : 2, runs = ceil_div(s->tokens_per_chapter, kRows);
+  const long long tiles = (columns + 8 * nt - 1) / (8 * nt), units = static_cast<long long>(s->n_chapters) * runs;
+  MOC_REQUIRE(tiles * s->num_kv_heads < (1ll << 27) && units < (1ll << 30), "decode-attention problem too large for one launch");
+  auto kern = nt == 1 ? decode_attn8_kernel<1> : decode_attn8_kernel<2>;
+  // a cluster per (sequence, KV head, tile of columns) while all of them are resident at once and every warp has a unit to take
+  const long long groups = tiles * s->num_kv_heads * s->batch;
+  int split = 8;
+  while (split > 1 && (split / 2 * kWarps >= units || groups > resident_clusters(kern, kThreads, 0, split))) split /= 2;
+  Attn8Params p{};
+  p.q = static_cast<const __nv_bfloat16*>(q); p.values = static_cast<const uint8_t*>(values); p.scales = scales; p.bank_rows = bank_rows;
+  p.comb_idx = comb_idx; p.comb_w = comb_w; p.counts = counts; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
+  p.n_q = s->n_q; p.H = s->num_heads; p.HK = s->num_kv_heads; p.n_ch = s->n_chapters; p.T = s->tokens_per_chapter;
+  p.split = split; p.tiles = static_cast<int>(tiles); p.scale = s->scale; p.scale_rows = fast_div(scale_rows); p.runs = fast_div(runs);
+  p.status = status;
+  MOC_CUDA_OK(launch_clustered(kern, dim3(static_cast<unsigned>(tiles) * s->num_kv_heads * split, s->batch), kThreads, 0, split,
+                               static_cast<cudaStream_t>(stream), p));
+  MOC_CUDA_OK(cudaGetLastError());
+  return MOC_OK;
+}
+
+}  // namespace moc
+
+using namespace moc;
+
+extern "C" int moc_quantize_rows(const void* rows_bf16, int64_t rows, int32_t heads, int32_t head_dim, int32_t scale_rows,
+                                 void* values, float* scales, void* stream) {
+  MOC_REQUIRE(rows_bf16 && values && scales, "NULL quantisation buffer");
+  MOC_REQUIRE(head_dim == kDD, "the 8-bit cache needs head_dim 64");
+  MOC_REQUIRE(rows > 0 && heads > 0 && scale_rows > 0 && rows % scale_rows == 0, "rows must be whole blocks of scale_rows");
+  MOC_REQUIRE(((reinterpret_cast<uintptr_t>(rows_bf16) | reinterpret_cast<uintptr_t>(values)) & 15) == 0,
+              "rows and values must be 16-byte aligned");
+  const long long tiles = rows / scale_rows * heads;
+  MOC_REQUIRE(tiles < (1ll << 33), "too many blocks in one call");
+  const unsigned grid = static_cast<unsigned>((tiles + kWarps - 1) / kWarps);
+  auto kern = scale_rows <= 8 ? quantize_rows_kernel<2> : scale_rows <= 16 ? quantize_rows_kernel<4>
+              : scale_rows <= 32 ? quantize_rows_kernel<8> : quantize_rows_kernel<16>;
+  kern<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const __nv_bfloat16*>(rows_bf16), tiles, heads, scale_rows,
+                                                                static_cast<uint8_t*>(values), scales);
+  MOC_CUDA_OK(cudaGetLastError());
+  return MOC_OK;
+}

@@ -601,9 +601,12 @@ def grad_clip(grads, ptrs, out, banks, max_norm: float, eps: float, device: torc
     tensors = [*grads, *(b[0] for b in banks)]
     # the columns of the table, without a Python step per tensor
     grad_ptrs = array("Q", [*ptrs, *(b[0].data_ptr() for b in banks)])
-    sizes, types = array("q", map(_numel, tensors)), array("B", map(codes, map(_dtype, tensors)))
-    same = out is grads
-    outs, out_types = (grad_ptrs, types) if same else (array("Q", map(_data_ptr, out)), array("B", map(codes, map(_dtype, out))))
+    sizes, same = array("q", map(_numel, tensors)), out is grads
+    try:
+        types = array("B", map(codes, map(_dtype, tensors)))
+        outs, out_types = (grad_ptrs, types) if same else (array("Q", map(_data_ptr, out)), array("B", map(codes, map(_dtype, out))))
+    except KeyError as e:
+        raise TypeError(f"gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
     counts, units = array("Q", [b[1].data_ptr() for b in banks]), array("i", [b[2] for b in banks])
     weights = array("f", [b[3] for b in banks])
     result = torch.empty(2, dtype=torch.float32, device=device)

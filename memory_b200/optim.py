@@ -86,7 +86,6 @@ class GradClip(NamedTuple):
     coefficient: torch.Tensor
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, *,
                     bank_grads: Sequence[SparseBankGrad] = (), out: Optional[Sequence[torch.Tensor]] = None,
                     eps: float = 1e-6) -> GradClip:
@@ -104,13 +103,15 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    grads = list(map(_gradient, (parameters,) if torch.is_tensor(parameters) else parameters))
-    outs = grads if out is None else list(out)
-    if len(outs) != len(grads):
-        raise ValueError(f"out must have one tensor per gradient: {len(outs)} vs {len(grads)}")
-    if any(map(_is_none, grads)):
-        outs = [o for g, o in zip(grads, outs) if g is not None]
-        grads = outs if out is None else [g for g in grads if g is not None]
+    listed = (parameters,) if torch.is_tensor(parameters) else parameters
+    found = [p if type(p) is torch.Tensor and not p.requires_grad else _gradient(p) for p in listed]
+    grads = [g for g in found if g is not None]
+    outs = grads
+    if out is not None:
+        outs = list(out)
+        if len(outs) != len(found):
+            raise ValueError(f"out must have one tensor per gradient: {len(outs)} vs {len(found)}")
+        outs = [o for g, o in zip(found, outs) if g is not None]
     banks = []
     for sink in bank_grads:
         if len(sink.entries) > 1:
@@ -120,36 +121,31 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     if not grads and not banks:
         raise ValueError("no gradients to clip")
     device = grads[0].device if grads else banks[0][0].device
-    bank_rows = [b[0] for b in banks]
-    written = [] if outs is grads else outs
-    every = [*grads, *written, *bank_rows, *(b[1] for b in banks)]
-    if device.type != "cuda" or set(map(_device, every)) != {device} or set(map(_layout, every)) != {torch.strided}:
+    tensors = grads if outs is grads else [*grads, *outs]
+    where = set(map(torch.Tensor.get_device, tensors))
+    for rows, count, _, _ in banks:
+        where |= {rows.get_device(), count.get_device()}
+    if device.type != "cuda" or len(where) != 1 or any(map(_is_sparse, tensors)):
         raise ValueError("gradients must be dense CUDA tensors on one device")
-    if not set(map(_dtype, [*grads, *written, *bank_rows])) <= ops._GRAD_DTYPES.keys():
-        raise TypeError("gradients must be float32, bfloat16 or float16")
-    if written and list(map(_shape, written)) != list(map(_shape, grads)):
+    if outs is not grads and list(map(_shape, outs)) != list(map(_shape, grads)):
         raise ValueError("out must match the gradients in shape")
     copies: list = []
     ptrs = list(map(torch.Tensor.data_ptr, grads))
-    if len(set(ptrs)) < len(ptrs) or not all(map(torch.Tensor.is_contiguous, [*grads, *written])):
+    if len(set(ptrs)) < len(ptrs) or not all(map(torch.Tensor.is_contiguous, tensors)):
         grads, outs, copies = _distinct_and_dense(grads, outs)
         ptrs = list(map(torch.Tensor.data_ptr, grads))
     result = ops.grad_clip(grads, ptrs, outs, banks, max_norm, eps, device)
-    for o, dense in copies:
-        o.copy_(dense)
-    return GradClip(*result.unbind())
+    if copies:
+        with torch.no_grad():
+            for o, dense in copies:
+                o.copy_(dense)
+    return GradClip(result.as_strided((), (), 0), result.as_strided((), (), 1))
 
 
-_device, _layout, _dtype, _shape = map(attrgetter, ("device", "layout", "dtype", "shape"))
-
-
-def _is_none(t) -> bool:
-    return t is None
+_shape, _is_sparse = attrgetter("shape"), attrgetter("is_sparse")
 
 
 def _gradient(p: torch.Tensor) -> Optional[torch.Tensor]:
-    if type(p) is torch.Tensor and not p.requires_grad:
-        return p
     return p.grad if isinstance(p, torch.nn.Parameter) or p.is_leaf else p.detach()
 
 

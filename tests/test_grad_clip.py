@@ -188,6 +188,17 @@ def test_bank_step_takes_the_coefficient_from_the_device():
 
 
 @pytest.mark.gpu
+def test_other_types_and_layouts_are_refused():
+    import memory_b200 as M
+    g = torch.ones(4, 4, device="cuda")
+    for grads, out, error in (([g.double()], None, TypeError), ([g], [g.double()], TypeError), ([g.to_sparse()], None, ValueError),
+                              ([g, g.cpu()], None, ValueError), ([g], [g[:2]], ValueError), ([g], [g.cpu()], ValueError)):
+        with pytest.raises(error):
+            M.clip_grad_norm_(grads, 1.0, out=out)
+    assert torch.equal(g, torch.ones_like(g))
+
+
+@pytest.mark.gpu
 def test_overlaps_are_refused():
     import memory_b200 as M
     t = torch.zeros(100, device="cuda")
