@@ -4,23 +4,18 @@
 // products, so the values go into them as they are stored (u_c: the weight of chapter c):
 //   s_r = scale * u_c * ks_r * <q, K8[r]>,   out = sum_r softmax(s)_r * u_c * vs_r * V8[r]   (one joint softmax).
 //
-// Bound by HBM for a full batch (one byte an element), by latency for a few sequences.  On CUDA cores, and with fp16 matrix
-// instructions, 64 sequences of 4,160 rows and 12 heads took 95 to 97 us, bound by issuing 500 to 550 instructions for every 32 rows of
-// a head.  So the values go into e4m3 matrix instructions as they lie in memory, and the other operand is split into e4m3 terms:
-//   q = q0 + q1 / 16 + q2 / 256 (scaled so that its largest element is 128 to 256: 12 bits each, 2^-25 of the largest at the least),
-//   p = (p0 + p1 / 16 + p2 / 256) / 256 (12 bits, 2^-26 at the least), each four significant bits of what the terms before leave.
-// The terms are columns of the same instruction, which has eight and one query would use one of them: four columns a query.  e4m3
-// products sum up in fp32 as fp16's do (2^-22 of the magnitudes, measured).
-//   - scores: A = 16 keys x 32 dims.  The order of the dims is free, so a lane's 16 bytes of its row are the A fragments of both
-//     steps as they come; keys are taken in the order that leaves the probabilities' bytes in theirs.
-//   - values: A = 16 dims x 32 rows, transposed on the way out of shared memory (8-bit matrix loads); B = the probabilities, brought
-//     from the scores' layout by a 16-bit matrix transposition of byte pairs.  Row scales that differ within a unit go in
-//     relative to the unit's largest.
-// Each warp has a ring of units (32 rows, K and V of one KV head) that bulk tensor copies fill two units ahead.  Maxima, sums and
-// accumulators are fp32.  All queries on a KV head (its heads, the tokens of the step) share a row's fetch, up to eight a CTA.  A cluster
-// of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through shared memory, then distributed
-// shared memory.
-#define MOC_KERNEL_TAG 7
+// Bound by HBM for a full batch (one byte an element), by latency for a few sequences.  All queries on a KV head (its heads, the
+// tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted once for up to 16 of them;
+// e4m3 -> fp16 is exact.  On CUDA cores a unit of 32 rows took 554 instructions (64 sequences of 4,160 rows, 12 heads: 95 us, bound by
+// issuing); with matrix instructions of single warps about half, whatever the number of columns.
+//   - scores: A = 16 keys x 16 dims, B = dims x 8 queries.  The order of the dims is free, so a lane's 16 bytes of its row are
+//     the A fragments of four steps as they come.  Queries are scaled by a power of two into fp16's range (their largest to
+//     128..256; what falls below fp16's smallest number is 2^-31 of the largest).
+//   - values: A = 16 dims x 16 rows, transposed from rows by byte permutations within a lane; B = the probabilities, which a matrix
+//     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
+//     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
+// Maxima, sums and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts
+// merge through shared memory, then distributed shared memory.
 #include <cuda_fp16.h>
 
 #include "host_pass.cuh"
@@ -33,6 +28,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct Attn8Params {
   const __nv_bfloat16* q;
+  const uint8_t* values;
   const float* scales;                 // [bank_rows / scale_rows, 2 * HK]
   long long bank_rows;
   const int* comb_idx;
@@ -40,49 +36,34 @@ struct Attn8Params {
   const int* counts;                   // chapters of each list that count (NULL: all)
   __nv_bfloat16* out;
   float* lse;
-  int n_q, H, HK, n_ch, T, split, tiles;        // tiles of queries of a KV head
+  int n_q, H, HK, n_ch, T, split, tiles;        // tiles of columns of a KV head
   float scale;
   FastDiv scale_rows, runs;
   int* status;
 };
 
-// D = A B, A 16 x 32 and B 32 x 8 of e4m3
-__device__ __forceinline__ void mma_e4m3_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+__device__ __forceinline__ uint32_t e4m3x2_to_f16(uint32_t two) {       // the low 16 bits
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(two));
+  return r;
 }
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ uint32_t e4m3x2_to_f16_high(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two));
+  return r;
 }
-// Two 16 x 16 byte matrices, transposed: lane l gives row l (of the first for l < 16); A fragment of columns 0..15 x rows 0..31
-__device__ __forceinline__ void ldsm_bytes_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared::cta.b8 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {           // of a warp's 8 x 8 matrix of 16-bit values
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {    // in the low 16 bits
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 of_e4m3x2(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(two)));
-  return __half22float2(*reinterpret_cast<const __half2*>(&h));
-}
-// x, y (at most 448) as three e4m3 terms each, the second times 16 and the third times 256
-__device__ __forceinline__ void split_e4m3(float x, float y, uint32_t (&term)[3]) {
-  term[0] = to_e4m3x2(x, y);
-  float2 t = of_e4m3x2(term[0]);
-  x = (x - t.x) * 16.f; y = (y - t.y) * 16.f;
-  term[1] = to_e4m3x2(x, y);
-  t = of_e4m3x2(term[1]);
-  term[2] = to_e4m3x2((x - t.x) * 16.f, (y - t.y) * 16.f);
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -90,93 +71,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-constexpr int kStages = 3, kUnitBytes = 2 * kRows * kDD;
-constexpr int kShared = kWarps * kStages * kUnitBytes + 1024;          // (tiles start on 1,024 bytes)
-
-// NT: tiles of 8 columns, two queries each.  Lane (g, t) = (lane / 4, lane % 4).
+// NT: tiles of 8 columns.  Lane (g, t) = (lane / 4, lane % 4).
 template <int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1)
-decode_attn8_kernel(const __grid_constant__ CUtensorMap map, const Attn8Params p) {
-  constexpr int kCols = 2 * NT;        // queries
-  extern __shared__ char raw_ring[];
-  __shared__ __align__(8) uint64_t full[kWarps][kStages];
-  __shared__ int abort_flag;
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+decode_attn8_kernel(const Attn8Params p) {
+  constexpr int kCols = 8 * NT;
+  __shared__ __align__(16) float red[kCols][kWarps][kDD + 4];
   __shared__ __align__(16) float cta_part[kCols][kDD + 4];        // accumulator, maximum, sum of this CTA
-  char* ring = raw_ring + (1024 - (smem_u32(raw_ring) & 1023)) % 1024;
-  float (*red)[kWarps][kDD + 4] = reinterpret_cast<float (*)[kWarps][kDD + 4]>(ring);       // once the rings are done with
   const int split = p.split, HK = p.HK, T = p.T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rank = static_cast<int>(blockIdx.x) % split, tile = static_cast<int>(blockIdx.x) / split % p.tiles;
   const int kh = static_cast<int>(blockIdx.x) / split / p.tiles, b = blockIdx.y;
-  const int per_kv = p.H / HK, columns = min(kCols, p.n_q * per_kv - tile * kCols);      // query j: token j / per_kv, head kh per_kv + j % per_kv
+  const int per_kv = p.H / HK, columns = min(kCols, p.n_q * per_kv - tile * kCols);      // column j: token j / per_kv, head kh per_kv + j % per_kv
+  const long long row_bytes = 2ll * HK * kDD;
   auto q_row = [&](int col) {
     const int j = tile * kCols + col, iq = j / per_kv;
     return (static_cast<long long>(b) * p.n_q + iq) * p.H + kh * per_kv + (j - iq * per_kv);
   };
-  if (threadIdx.x == 0) {
-    abort_flag = 0;
-    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&full[0][0] + i, 1);
-    fence_mbar_init();
-    prefetch_tmap(&map);
-  }
-  __syncthreads();
   int n_ch = p.n_ch;
   if (p.counts != nullptr) n_ch = max(0, min(n_ch, p.counts[b]));
   const int* list = p.comb_idx + static_cast<long long>(b) * p.n_ch;
   const float* weights = p.comb_w + static_cast<long long>(b) * p.n_ch;
-  const int total = n_ch * p.runs.d, stride = split * kWarps, first = rank * kWarps + warp;
-  auto known = [&](int ch) { return ch >= 0 && (static_cast<long long>(ch) + 1) * T <= p.bank_rows; };
-  char* stages = ring + warp * kStages * kUnitBytes;
 
-  auto fetch = [&](int unit, int stage) {          // by one lane
-    if (unit >= total) return;
-    const int c = div_of(unit, p.runs), ch = list[c];
-    if (!known(ch)) {
-      atomicMax(p.status, MOC_DEV_BAD_INDEX);
-      mbar_arrive(&full[warp][stage]);
-      return;
-    }
-    const int row = ch * T + (unit - c * p.runs.d) * kRows;
-    mbar_arrive_expect_tx(&full[warp][stage], kUnitBytes);
-    tma_load_2d(stages + stage * kUnitBytes, &map, &full[warp][stage], kh * kDD, row);
-    tma_load_2d(stages + stage * kUnitBytes + kRows * kDD, &map, &full[warp][stage], (HK + kh) * kDD, row);
-  };
-  if (lane == 0)
-    for (int i = 0; i < kStages - 1; ++i) fetch(first + i * stride, i);
-
-  // a unit's factors, fetched one unit ahead: of this lane's rows 16 mt + 2 g + h, i = 2 mt + h (one block of scales: the first)
-  const bool one_block = p.scale_rows.d % kRows == 0;
-  struct Factors {
-    float u, k[4], v[4];
-    int r0;                            // first row within the chapter; -1: unknown chapter
-  };
-  auto factors_of = [&](int unit, Factors& f) {
-    if (unit >= total) return;
-    const int c = div_of(unit, p.runs), ch = list[c];
-    f.u = weights[c];
-    f.r0 = known(ch) ? (unit - c * p.runs.d) * kRows : -1;
-    if (f.r0 < 0) return;
-    const float* sc = p.scales + static_cast<long long>(ch) * (T / p.scale_rows.d) * 2 * HK + kh;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (one_block && i > 0) { f.k[i] = f.k[0]; f.v[i] = f.v[0]; continue; }
-      const int r = one_block ? f.r0 : f.r0 + 16 * (i >> 1) + 2 * g + (i & 1);
-      const float* at = sc + static_cast<long long>(div_of(r < T ? r : 0, p.scale_rows)) * 2 * HK;
-      f.k[i] = at[0];
-      f.v[i] = at[HK];
-    }
-  };
-  Factors now{}, next{};
-  factors_of(first, now);
-
-  // queries: B fragments (column g = term g % 4 of query g / 4; dims 16 t + 8 s + {0..3} and {4..7} in step s), and what this
-  // lane's two score columns count: the even one of a query's pair of lanes has the first two terms, the odd one the third
-  uint32_t qb[NT][2][2];
-  float fa[NT], fb[NT], acc[NT][4][4], m[NT], l[NT];
+  // queries: B fragments (column g, dims 16 t + 4 s + {0, 1} and {2, 3} in step s), and the factors of this lane's score columns
+  uint32_t qb[NT][4][2];
+  float factor[NT][2], acc[NT][4][4], m[NT][2], l[NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float f[16], top = 0.f;
-    const int col = 2 * nt + (g >> 2);
+    const int col = nt * 8 + g;
     const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row(col < columns ? col : 0) * kDD + 16 * t);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -184,181 +107,186 @@ decode_attn8_kernel(const __grid_constant__ CUtensorMap map, const Attn8Params p
       const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        f[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-        f[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        f[8 * h + 2 * i] = col < columns ? __uint_as_float(w[i] << 16) : 0.f;
+        f[8 * h + 2 * i + 1] = col < columns ? __uint_as_float(w[i] & 0xFFFF0000u) : 0.f;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max_nan(top, fabsf(f[i]));
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = static_cast<int>(__float_as_uint(top) >> 23);          // of 2^(e - 127); queries below 2^-99 count as zero
-    const float up = e > 27 && e < 255 ? __uint_as_float(static_cast<uint32_t>(261 - e) << 23) : 0.f;       // 2^(134 - e)
-    float down = e > 27 ? __uint_as_float(static_cast<uint32_t>(e - 7) << 23) : 0.f;
-    if (e == 255) down = NAN;                                            // (infinite or NaN queries: every score NaN)
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(f[i]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = static_cast<int>(__float_as_uint(top) >> 23);          // of 2^(e - 127); infinite queries and tiny ones stay as they are
+    const bool shift = e > 27 && e < 255;
+    const float up = shift ? __uint_as_float(static_cast<uint32_t>(261 - e) << 23) : 1.f;       // 2^(134 - e)
+    const float down = shift ? __uint_as_float(static_cast<uint32_t>(max(e - 7, 1)) << 23) : 1.f;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 4; ++s) {
+      qb[nt][s][0] = pack_f16(f[4 * s] * up, f[4 * s + 1] * up);
+      qb[nt][s][1] = pack_f16(f[4 * s + 2] * up, f[4 * s + 3] * up);
+    }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t lo[3], hi[3];
-        const float* x = f + 8 * s + 4 * h;
-        split_e4m3(up > 0.f ? x[0] * up : 0.f, up > 0.f ? x[1] * up : 0.f, lo);
-        split_e4m3(up > 0.f ? x[2] * up : 0.f, up > 0.f ? x[3] * up : 0.f, hi);
-        const int term = g & 3;
-        const uint32_t a = term == 0 ? lo[0] : term == 1 ? lo[1] : lo[2], c = term == 0 ? hi[0] : term == 1 ? hi[1] : hi[2];
-        qb[nt][s][h] = term == 3 || col >= columns ? 0u : a | c << 16;
-      }
-    const float factor = __shfl_sync(0xffffffffu, down, (t >> 1) * 16) * p.scale * kLog2e;
-    fa[nt] = t & 1 ? factor * (1.f / 256.f) : factor;
-    fb[nt] = t & 1 ? 0.f : factor * (1.f / 16.f);
-    m[nt] = -INFINITY;
-    l[nt] = 0.f;
+    for (int j = 0; j < 2; ++j) {
+      factor[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale * kLog2e;
+      m[nt][j] = -INFINITY;
+      l[nt][j] = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.f;
   }
 
-  int stage = 0;
-  uint32_t phase = 0;
-  const uint32_t k_at = 2 * g * kDD + ((t ^ (g & 3)) << 4);            // rows 2 g (and 2 g + 1, 64 bytes on), piece t, swizzled
-  for (int unit = first; unit < total; unit += stride) {
-    if (lane == 0) fetch(unit + (kStages - 1) * stride, stage == 0 ? kStages - 1 : stage - 1);
-    factors_of(unit + stride, next);
-    const bool alive = mbar_wait_w(&full[warp][stage], phase, &abort_flag, p.status);
-    if (!alive) {                          // the copies still on their way land before the bytes change owner, or as long again passes
-      for (int i = 0, at = stage; i < kStages && unit + i * stride < total; ++i) {
-        for (uint32_t it = 0; it < kWaitPollLimit && !mbar_try_wait(&full[warp][at], phase); ++it) {}
-        if (++at == kStages) { at = 0; phase ^= 1; }
-      }
-      break;
+  const bool one_block = p.scale_rows.d % kRows == 0;          // a unit lies in one block of scales
+  for (int unit = rank * kWarps + warp; unit < n_ch * p.runs.d; unit += split * kWarps) {
+    const int c = div_of(unit, p.runs), r0 = (unit - c * p.runs.d) * kRows;
+    const int ch = list[c];
+    if (ch < 0 || (static_cast<long long>(ch) + 1) * T > p.bank_rows) {
+      if (lane == 0) atomicMax(p.status, MOC_DEV_BAD_INDEX);
+      continue;
     }
-    char* kt = stages + stage * kUnitBytes;
-    char* vt = kt + kRows * kDD;
-    if (++stage == kStages) { stage = 0; phase ^= 1; }
-    if (now.r0 >= 0) {
-      if (now.r0 + kRows > T) {            // rows of the next chapter: their values may be NaN, and meet probabilities of 0
-        if (now.r0 + lane >= T) {
+    const float u = weights[c];
+    const uint8_t* chapter = p.values + static_cast<long long>(ch) * T * row_bytes + kh * kDD;
+    uint4 kr[2][2];                    // rows 16 mt + g and + 8, bytes 16 t ..
+    uint2 vr[2][4];                    // rows 16 ks + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}, bytes 8 g ..
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(vt + lane * kDD + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async();               // (before the next copy into these bytes)
-        __syncwarp();
-      }
-      float kf[4], vf[4], w_top;
-      if (one_block) {
-        w_top = now.v[0];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { kf[i] = now.k[0] * now.u; vf[i] = 256.f; }
-      } else {
-        w_top = max_nan(max_nan(now.v[0], now.v[1]), max_nan(now.v[2], now.v[3]));
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) w_top = max_nan(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
-        const float inv = w_top > 0.f ? 256.f / w_top : 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { kf[i] = now.k[i] * now.u; vf[i] = now.v[i] * inv; }
-      }
-      w_top *= now.u * (1.f / 256.f);
-      uint32_t kr[2][2][4];                // [mt][h]: rows 16 mt + 2 g + h, bytes 16 t ..
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 v = *reinterpret_cast<const uint4*>(kt + 16 * mt * kDD + k_at + h * kDD);
-          kr[mt][h][0] = v.x; kr[mt][h][1] = v.y; kr[mt][h][2] = v.z; kr[mt][h][3] = v.w;
-        }
-      uint32_t pb[NT][2];                  // probabilities as B fragments: rows 4 t .. 4 t + 3 and 16 on, column g
-      float corr[NT];
-      bool moved = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float s[4];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          float d[4];
-          mma_e4m3_new(d, kr[mt][0][0], kr[mt][1][0], kr[mt][0][1], kr[mt][1][1], qb[nt][0][0], qb[nt][0][1]);
-          mma_e4m3(d, kr[mt][0][2], kr[mt][1][2], kr[mt][0][3], kr[mt][1][3], qb[nt][1][0], qb[nt][1][1]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) s[2 * mt + h] = fmaf(d[2 * h + 1], fb[nt], d[2 * h] * fa[nt]);
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = (s[i] + __shfl_xor_sync(0xffffffffu, s[i], 1)) * kf[i];
-          if (now.r0 + 16 * (i >> 1) + 2 * g + (i & 1) >= T) s[i] = -INFINITY;
-          top = fmaxf(top, s[i]);
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m_new = fmaxf(m[nt], top), ref = m_new == -INFINITY ? 0.f : m_new;
-        corr[nt] = exp2_fast(m[nt] - ref);               // 0 on the first rows (m = -inf)
-        moved |= m_new != m[nt];
-        m[nt] = m_new;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[i] = exp2_fast(s[i] - ref);
-          sum += s[i];
-        }
-        l[nt] = fmaf(l[nt], corr[nt], sum);
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          uint32_t term[3];
-          split_e4m3(s[2 * mt] * vf[2 * mt], s[2 * mt + 1] * vf[2 * mt + 1], term);
-          pb[nt][mt] = transpose8(t & 1 ? term[2] : term[0] | term[1] << 16);
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          // (lane (g, t) has the column pair t in its accumulators: the maximum is that of the same query)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[nt][i][j] *= corr[nt];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {        // dims 16 i + g and + 8
-        uint32_t a[4];
-        ldsm_bytes_t(a, smem_u32(vt) + lane * kDD + ((i ^ ((lane >> 1) & 3)) << 4));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float d[4];
-          mma_e4m3_new(d, a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[nt][i][j] = fmaf(w_top, d[j], acc[nt][i][j]);
-        }
-      }
-    }
-    now = next;
-    __syncwarp();                          // the ring's place is free from here on
-  }
-  __syncthreads();
-  if (abort_flag) {                        // (reported in the status word; the same for the whole CTA)
-    if (split > 1) { cluster_sync(); cluster_sync(); }
-    return;
-  }
-  // a warp's part, the terms summed: query 2 nt + t / 2
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float sum = l[nt];
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    float* to = red[2 * nt + (t >> 1)][warp];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v = t & 1 ? acc[nt][i][2 * h] * (1.f / 256.f) : fmaf(acc[nt][i][2 * h + 1], 1.f / 16.f, acc[nt][i][2 * h]);
-        v += __shfl_xor_sync(0xffffffffu, v, 1);
-        if (!(t & 1)) to[16 * i + 8 * h + g] = v;
+        const int r = r0 + 16 * mt + 8 * h + g;
+        kr[mt][h] = *reinterpret_cast<const uint4*>(chapter + (r < T ? r : 0) * row_bytes + 16 * t);
       }
-    if (g == 0 && !(t & 1)) {
-      to[kDD] = m[nt];
-      to[kDD + 1] = sum;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * ks + 2 * t + (i & 1) + 8 * (i >> 1);
+        vr[ks][i] = *reinterpret_cast<const uint2*>(chapter + (r < T ? r : 0) * row_bytes + HK * kDD + 8 * g);
+      }
+    // row factors of this lane's four rows (mt, h): scores, and values relative to `w_top`
+    float kf[2][2], vf[2][2], w_top;
+    const long long blk0 = static_cast<long long>(ch) * (T / p.scale_rows.d);
+    if (one_block) {
+      const float* sc = p.scales + (blk0 + div_of(r0, p.scale_rows)) * 2 * HK + kh;
+      const float ks = sc[0] * u;
+      w_top = sc[HK] * u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { kf[i >> 1][i & 1] = ks; vf[i >> 1][i & 1] = 1.f; }
+    } else {
+      w_top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 16 * (i >> 1) + 8 * (i & 1) + g;
+        const float* sc = p.scales + (blk0 + div_of(r < T ? r : 0, p.scale_rows)) * 2 * HK + kh;
+        kf[i >> 1][i & 1] = sc[0] * u;
+        vf[i >> 1][i & 1] = sc[HK];
+        w_top = max_nan(w_top, sc[HK]);
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) w_top = max_nan(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
+      const float inv = w_top > 0.f ? 1.f / w_top : 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vf[i >> 1][i & 1] *= inv;
+      w_top *= u;
+    }
+    uint32_t pb[NT][2][2];             // probabilities as B fragments: rows 16 ks + 2 t + {0, 1} and + 8, column g
+    float corr[NT][2];
+    bool moved = false;
+    {
+      float sc[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint32_t lo[4] = {kr[mt][0].x, kr[mt][0].y, kr[mt][0].z, kr[mt][0].w}, hi[4] = {kr[mt][1].x, kr[mt][1].y, kr[mt][1].z, kr[mt][1].w};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[mt][nt][j] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t a0 = e4m3x2_to_f16(lo[s]), a1 = e4m3x2_to_f16(hi[s]), a2 = e4m3x2_to_f16_high(lo[s]), a3 = e4m3x2_to_f16_high(hi[s]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[mt][nt], a0, a1, a2, a3, qb[nt][s][0], qb[nt][s][1]);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {           // rows (mt, h) = (i / 2, i % 2)
+            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+            s = r0 + 16 * (i >> 1) + 8 * (i & 1) + g < T ? s * kf[i >> 1][i & 1] * factor[nt][j] : -INFINITY;
+            top = fmaxf(top, s);
+          }
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float m_new = fmaxf(m[nt][j], top), ref = m_new == -INFINITY ? 0.f : m_new;
+          corr[nt][j] = exp2_fast(m[nt][j] - ref);               // 0 on the first rows (m = -inf)
+          moved |= m_new != m[nt][j];
+          m[nt][j] = m_new;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+            s = exp2_fast(s - ref);
+            sum += s;
+          }
+          l[nt][j] = fmaf(l[nt][j], corr[nt][j], sum);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1]));
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[nt][i][j] *= corr[nt][j & 1];
+    }
+    // values: tile i of 16 dims, dims 8 g + 2 i (fragment row g) and 8 g + 2 i + 1 (row g + 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[nt][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+        const uint32_t v01 = __byte_perm(i < 2 ? vr[ks][0].x : vr[ks][0].y, i < 2 ? vr[ks][1].x : vr[ks][1].y, sel);
+        const uint32_t v89 = __byte_perm(i < 2 ? vr[ks][2].x : vr[ks][2].y, i < 2 ? vr[ks][3].x : vr[ks][3].y, sel);
+        const uint32_t a0 = e4m3x2_to_f16(v01), a1 = e4m3x2_to_f16_high(v01), a2 = e4m3x2_to_f16(v89), a3 = e4m3x2_to_f16_high(v89);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nt][i][j] = fmaf(w_top, d[nt][j], acc[nt][i][j]);
     }
   }
+
+  // a warp's part: columns 2 t + j, dims 8 g ..
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float sum = l[nt][j];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int col = nt * 8 + 2 * t + j;
+      float* to = red[col][warp];
+      *reinterpret_cast<float4*>(to + 8 * g) = make_float4(acc[nt][0][j], acc[nt][0][2 + j], acc[nt][1][j], acc[nt][1][2 + j]);
+      *reinterpret_cast<float4*>(to + 8 * g + 4) = make_float4(acc[nt][2][j], acc[nt][2][2 + j], acc[nt][3][j], acc[nt][3][2 + j]);
+      if (g == 0) {
+        to[kDD] = m[nt][j];
+        to[kDD + 1] = sum;
+      }
+    }
   __syncthreads();
   // warps -> CTA: thread i finishes output element i % 64 of column i / 64
   for (int i = threadIdx.x; i < columns * kDD; i += kThreads) {
@@ -485,37 +413,24 @@ int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* value
               "num_heads must be a positive multiple of num_kv_heads");
   MOC_REQUIRE(scale_rows > 0 && s->tokens_per_chapter % scale_rows == 0, "a chapter must be whole blocks of scale_rows");
   MOC_REQUIRE(s->n_q <= 65535 && s->batch <= 65535, "too many query tokens or sequences for one launch");
-  MOC_REQUIRE(bank_rows < (1ll << 31), "the 8-bit cache takes fewer than 2^31 rows");
   MOC_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(values)) & 15) == 0, "q and the K/V cache must be 16-byte aligned");
   const long long columns = static_cast<long long>(s->n_q) * (s->num_heads / s->num_kv_heads);
-  const int nt = columns <= 2 ? 1 : columns <= 4 ? 2 : 4, runs = ceil_div(s->tokens_per_chapter, kRows);
-  const long long tiles = (columns + 2 * nt - 1) / (2 * nt), units = static_cast<long long>(s->n_chapters) * runs;
+  const int nt = columns <= 8 ? 1 : 2, runs = ceil_div(s->tokens_per_chapter, kRows);
+  const long long tiles = (columns + 8 * nt - 1) / (8 * nt), units = static_cast<long long>(s->n_chapters) * runs;
   MOC_REQUIRE(tiles * s->num_kv_heads < (1ll << 27) && units < (1ll << 30), "decode-attention problem too large for one launch");
-  CUtensorMap map;
-  const int rc = make_tmap_u8_2d(&map, values, static_cast<uint64_t>(bank_rows), 2ull * s->num_kv_heads * kDD, kRows);
-  if (rc != MOC_OK) return rc;
-  auto kern = nt == 1 ? decode_attn8_kernel<1> : nt == 2 ? decode_attn8_kernel<2> : decode_attn8_kernel<4>;
-  static_assert(kShared - 1024 >= 8 * kWarps * (kDD + 4) * 4, "the warps' parts fit the rings");
-  MOC_CUDA_OK(allow_shared(kern, kShared, kShared));
-  // Clusters of 1 to 8 CTAs for each (sequence, KV head, tile of queries): the fewest units in a row, counting three for a CTA's start
-  // and end, over the rounds in which all of them run.
+  auto kern = nt == 1 ? decode_attn8_kernel<1> : decode_attn8_kernel<2>;
+  // a cluster per (sequence, KV head, tile of columns) while all of them are resident at once and every warp has a unit to take
   const long long groups = tiles * s->num_kv_heads * s->batch;
-  int split = 1;
-  long long best = 0;
-  for (int n = 1; n <= 8; n *= 2) {
-    const long long resident = n == 1 ? (nt <= 2 ? 2 : 1) * 148 : resident_clusters(kern, kThreads, kShared, n);
-    if (resident == 0) continue;
-    const long long cost = (groups + resident - 1) / resident * ((units + n * kWarps - 1) / (n * kWarps) + 3);
-    if (best == 0 || cost < best) { best = cost; split = n; }
-  }
+  int split = 8;
+  while (split > 1 && (split / 2 * kWarps >= units || groups > resident_clusters(kern, kThreads, 0, split))) split /= 2;
   Attn8Params p{};
-  p.q = static_cast<const __nv_bfloat16*>(q); p.scales = scales; p.bank_rows = bank_rows;
+  p.q = static_cast<const __nv_bfloat16*>(q); p.values = static_cast<const uint8_t*>(values); p.scales = scales; p.bank_rows = bank_rows;
   p.comb_idx = comb_idx; p.comb_w = comb_w; p.counts = counts; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
   p.n_q = s->n_q; p.H = s->num_heads; p.HK = s->num_kv_heads; p.n_ch = s->n_chapters; p.T = s->tokens_per_chapter;
   p.split = split; p.tiles = static_cast<int>(tiles); p.scale = s->scale; p.scale_rows = fast_div(scale_rows); p.runs = fast_div(runs);
   p.status = status;
-  MOC_CUDA_OK(launch_clustered(kern, dim3(static_cast<unsigned>(tiles) * s->num_kv_heads * split, s->batch), kThreads, kShared, split,
-                               static_cast<cudaStream_t>(stream), map, p));
+  MOC_CUDA_OK(launch_clustered(kern, dim3(static_cast<unsigned>(tiles) * s->num_kv_heads * split, s->batch), kThreads, 0, split,
+                               static_cast<cudaStream_t>(stream), p));
   MOC_CUDA_OK(cudaGetLastError());
   return MOC_OK;
 }

@@ -33,14 +33,13 @@ static EncodeTiledFn encode_fn() {
 }
 
 static int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, uint32_t esize, const void* base, uint64_t rows,
-                        uint64_t cols, uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols,
-                        uint32_t swizzle_bytes = 128) {
+                        uint64_t cols, uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) {
     set_last_error("cuTensorMapEncodeTiled", "driver entry point not found");
     return MOC_ERR_CUDA;
   }
-  MOC_REQUIRE((swizzle_bytes == 128 || swizzle_bytes == 64) && box_cols * esize == swizzle_bytes, "tile rows must be as long as the swizzle");
+  MOC_REQUIRE(box_cols * esize == 128, "tile rows must be 128 bytes for the 128-byte swizzle");
   MOC_REQUIRE(box_rows >= 1 && box_rows <= 256, "box rows out of range");
   MOC_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "tensor base must be 16-byte aligned");
   MOC_REQUIRE((row_stride_elems * esize) % 16 == 0, "row stride must be a multiple of 16 bytes");
@@ -59,8 +58,7 @@ static int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, uint32_t esi
     context_bound = true;
   }
   CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     // say what was asked for, and whether an earlier asynchronous error is what the driver is reporting
@@ -78,9 +76,6 @@ static int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType type, uint32_t esi
 int make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                       uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols) {
   return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, rows, cols, row_stride_elems, box_rows, box_cols);
-}
-int make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-  return make_tmap_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, cols, cols, box_rows, 64, 64);
 }
 int make_tmap_f32_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                      uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols) {

@@ -48,8 +48,6 @@ static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 // swizzle (box_cols * 2 bytes must be 128).
 int make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                       uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols);
-// 2-D byte tensor [rows, cols] without gaps; box = [box_rows, 64], 64-byte swizzle.
-int make_tmap_u8_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows);
 int make_tmap_f32_2d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                      uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_cols);
 
