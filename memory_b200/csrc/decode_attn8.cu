@@ -4,17 +4,20 @@
 // products, so the values go into them as they are stored (u_c: the weight of chapter c):
 //   s_r = scale * u_c * ks_r * <q, K8[r]>,   out = sum_r softmax(s)_r * u_c * vs_r * V8[r]   (one joint softmax).
 //
-// Bound by HBM for a full batch (one byte an element), by latency for a few sequences.  All queries on a KV head (its heads, the
-// tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted once for up to 16 of them;
-// e4m3 -> fp16 is exact.  On CUDA cores a unit of 32 rows took 554 instructions (64 sequences of 4,160 rows, 12 heads: 95 us, bound by
-// issuing); with matrix instructions of single warps about half, whatever the number of columns.
+// A full batch should be bound by HBM (one byte an element) and is bound by issuing; a few sequences by latency.  All queries on a KV
+// head (its heads, the tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted once for up to
+// 16 of them; e4m3 -> fp16 is exact.  64 sequences of 4,160 rows, 12 heads: 92 us (2.9 TB/s of HBM, 0.58 instructions a cycle and
+// scheduler, 450 a unit of 32 rows); 13 sequences of 3 tokens, 12 heads on 4, 47 chapters of 64 rows: 15.4 us.  The same on CUDA cores
+// took 95 and 19 us; units by bulk tensor copies into a ring, 99 and 16.5; e4m3 matrix instructions with queries and probabilities
+// in three terms, 102 and 33.
 //   - scores: A = 16 keys x 16 dims, B = dims x 8 queries.  The order of the dims is free, so a lane's 16 bytes of its row are
 //     the A fragments of four steps as they come.  Queries are scaled by a power of two into fp16's range (their largest to
 //     128..256; what falls below fp16's smallest number is 2^-31 of the largest).
 //   - values: A = 16 dims x 16 rows, transposed from rows by byte permutations within a lane; B = the probabilities, which a matrix
 //     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
 //     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
-// Maxima, sums and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts
+// The softmax's reference of a column is a score already met; it moves to the largest only when a score passes it by 2^8, which saves
+// most units the reduction across lanes and the rescaling (97 us without).  References, sums and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts
 // merge through shared memory, then distributed shared memory.
 #include <cuda_fp16.h>
 
@@ -25,6 +28,7 @@ namespace {
 
 constexpr int kDD = 64, kThreads = 256, kWarps = kThreads / 32, kRows = 32;      // rows of a unit
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kHeadroom = 8.f;       // a score may pass its column's reference by 2^8 before that moves: fp16 probabilities reach 65504
 
 struct Attn8Params {
   const __nv_bfloat16* q;
@@ -51,6 +55,11 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16_high(uint32_t two) {
   uint32_t r;
   asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(two));
   return r;
+}
+// D = A B + D of fp16, A 16 x 16, B 16 x 8 (_new: D = A B)
+__device__ __forceinline__ void mma_f16_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -145,6 +154,7 @@ decode_attn8_kernel(const Attn8Params p) {
       continue;
     }
     const float u = weights[c];
+    const bool whole = r0 + kRows <= T;
     const uint8_t* chapter = p.values + static_cast<long long>(ch) * T * row_bytes + kh * kDD;
     uint4 kr[2][2];                    // rows 16 mt + g and + 8, bytes 16 t ..
     uint2 vr[2][4];                    // rows 16 ks + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}, bytes 8 g ..
@@ -189,71 +199,75 @@ decode_attn8_kernel(const Attn8Params p) {
       w_top *= u;
     }
     uint32_t pb[NT][2][2];             // probabilities as B fragments: rows 16 ks + 2 t + {0, 1} and + 8, column g
-    float corr[NT][2];
-    bool moved = false;
-    {
-      float sc[2][NT][4];
+    float sc[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const uint32_t lo[4] = {kr[mt][0].x, kr[mt][0].y, kr[mt][0].z, kr[mt][0].w}, hi[4] = {kr[mt][1].x, kr[mt][1].y, kr[mt][1].z, kr[mt][1].w};
+    for (int mt = 0; mt < 2; ++mt) {
+      const uint32_t lo[4] = {kr[mt][0].x, kr[mt][0].y, kr[mt][0].z, kr[mt][0].w}, hi[4] = {kr[mt][1].x, kr[mt][1].y, kr[mt][1].z, kr[mt][1].w};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t a0 = e4m3x2_to_f16(lo[s]), a1 = e4m3x2_to_f16(hi[s]), a2 = e4m3x2_to_f16_high(lo[s]), a3 = e4m3x2_to_f16_high(hi[s]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sc[mt][nt][j] = 0.f;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint32_t a0 = e4m3x2_to_f16(lo[s]), a1 = e4m3x2_to_f16(hi[s]), a2 = e4m3x2_to_f16_high(lo[s]), a3 = e4m3x2_to_f16_high(hi[s]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[mt][nt], a0, a1, a2, a3, qb[nt][s][0], qb[nt][s][1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (s == 0) mma_f16_new(sc[mt][nt], a0, a1, a2, a3, qb[nt][s][0], qb[nt][s][1]);
+          else mma_f16(sc[mt][nt], a0, a1, a2, a3, qb[nt][s][0], qb[nt][s][1]);
         }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {           // rows (mt, h) = (i / 2, i % 2)
-            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
-            s = r0 + 16 * (i >> 1) + 8 * (i & 1) + g < T ? s * kf[i >> 1][i & 1] * factor[nt][j] : -INFINITY;
-            top = fmaxf(top, s);
-          }
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const float m_new = fmaxf(m[nt][j], top), ref = m_new == -INFINITY ? 0.f : m_new;
-          corr[nt][j] = exp2_fast(m[nt][j] - ref);               // 0 on the first rows (m = -inf)
-          moved |= m_new != m[nt][j];
-          m[nt][j] = m_new;
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& s = sc[i >> 1][nt][2 * (i & 1) + j];
-            s = exp2_fast(s - ref);
-            sum += s;
-          }
-          l[nt][j] = fmaf(l[nt][j], corr[nt][j], sum);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1]));
       }
     }
-    if (__any_sync(0xffffffffu, moved)) {
+    bool above = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {           // rows (mt, h) = (i / 2, i % 2)
+          float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+          s *= kf[i >> 1][i & 1] * factor[nt][j];
+          if (!whole && r0 + 16 * (i >> 1) + 8 * (i & 1) + g >= T) s = -INFINITY;
+          top = fmaxf(top, s);
+        }
+        above |= top > m[nt][j] + kHeadroom;
+      }
+    if (__any_sync(0xffffffffu, above)) {       // new references: the largest scores so far
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 2; ++j) {
+          float top = m[nt][j];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[nt][i][j] *= corr[nt][j & 1];
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[i >> 1][nt][2 * (i & 1) + j]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float corr = top == -INFINITY ? 0.f : exp2_fast(m[nt][j] - top);       // 0 on the first rows (m = -inf)
+          m[nt][j] = top;
+          l[nt][j] *= corr;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            acc[nt][i][j] *= corr;
+            acc[nt][i][2 + j] *= corr;
+          }
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& s = sc[i >> 1][nt][2 * (i & 1) + j];
+          s = exp2_fast(s - ref);
+          l[nt][j] += s;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1]));
     }
     // values: tile i of 16 dims, dims 8 g + 2 i (fragment row g) and 8 g + 2 i + 1 (row g + 8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float d[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) d[nt][j] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
@@ -261,7 +275,10 @@ decode_attn8_kernel(const Attn8Params p) {
         const uint32_t v89 = __byte_perm(i < 2 ? vr[ks][2].x : vr[ks][2].y, i < 2 ? vr[ks][3].x : vr[ks][3].y, sel);
         const uint32_t a0 = e4m3x2_to_f16(v01), a1 = e4m3x2_to_f16_high(v01), a2 = e4m3x2_to_f16(v89), a3 = e4m3x2_to_f16_high(v89);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if (ks == 0) mma_f16_new(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+          else mma_f16(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -343,7 +360,7 @@ __device__ __forceinline__ void unpack8(const uint4& v, float* f) {
 // are read a second time.  A block of zeros has scale 0 and values 0; one with a NaN or an infinity gets a scale that is
 // NaN or infinite and stands for NaN as a whole.  Bound by HBM (2 bytes read and 1 written an element) once the quotient is a product
 // corrected by its remainder (Markstein), equal to the division where its last bit can matter: 262,208 x 1,536: 371 us with
-// divisions, 245 with products.
+// divisions, 232 with products (185 at the copy rate).
 template <int R>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long tiles, int heads, int block, uint8_t* __restrict__ values,
