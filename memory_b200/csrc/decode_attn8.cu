@@ -80,11 +80,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
-// NT: tiles of 8 columns.  Lane (g, t) = (lane / 4, lane % 4).
-template <int NT>
+// NT: tiles of 8 columns.  Lane (g, t) = (lane / 4, lane % 4) has the scores of columns 2 t and 2 t + 1; NJ = 1: up to four queries take
+// the even ones and the odd ones' work is left out.
+template <int NT, int NJ>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 decode_attn8_kernel(const Attn8Params p) {
-  constexpr int kCols = 8 * NT;
+  constexpr int kCols = 4 * NJ * NT;
   __shared__ __align__(16) float red[kCols][kWarps][kDD + 4];
   __shared__ __align__(16) float cta_part[kCols][kDD + 4];        // accumulator, maximum, sum of this CTA
   const int split = p.split, HK = p.HK, T = p.T;
@@ -104,11 +105,11 @@ decode_attn8_kernel(const Attn8Params p) {
 
   // queries: B fragments (column g, dims 16 t + 4 s + {0, 1} and {2, 3} in step s), and the factors of this lane's score columns
   uint32_t qb[NT][4][2];
-  float factor[NT][2], acc[NT][4][4], m[NT][2], l[NT][2];
+  float factor[NT][NJ], acc[NT][4][2][NJ], m[NT][NJ], l[NT][NJ];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float f[16], top = 0.f;
-    const int col = nt * 8 + g;
+    const int col = NJ == 2 ? nt * 8 + g : g & 1 ? kCols : g >> 1;
     const uint4* src = reinterpret_cast<const uint4*>(p.q + q_row(col < columns ? col : 0) * kDD + 16 * t);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -134,7 +135,7 @@ decode_attn8_kernel(const Attn8Params p) {
       qb[nt][s][1] = pack_f16(f[4 * s + 2] * up, f[4 * s + 3] * up);
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       factor[nt][j] = __shfl_sync(0xffffffffu, down, (2 * t + j) * 4) * p.scale * kLog2e;
       m[nt][j] = -INFINITY;
       l[nt][j] = 0.f;
@@ -142,7 +143,7 @@ decode_attn8_kernel(const Attn8Params p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[nt][i][j] = 0.f;
+      for (int j = 0; j < NJ; ++j) acc[nt][i][0][j] = acc[nt][i][1][j] = 0.f;
   }
 
   const bool one_block = p.scale_rows.d % kRows == 0;          // a unit lies in one block of scales
@@ -217,7 +218,7 @@ decode_attn8_kernel(const Attn8Params p) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NJ; ++j) {
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {           // rows (mt, h) = (i / 2, i % 2)
@@ -232,7 +233,7 @@ decode_attn8_kernel(const Attn8Params p) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < NJ; ++j) {
           float top = m[nt][j];
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[i >> 1][nt][2 * (i & 1) + j]);
@@ -243,15 +244,15 @@ decode_attn8_kernel(const Attn8Params p) {
           l[nt][j] *= corr;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            acc[nt][i][j] *= corr;
-            acc[nt][i][2 + j] *= corr;
+            acc[nt][i][0][j] *= corr;
+            acc[nt][i][1][j] *= corr;
           }
         }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NJ; ++j) {
         const float ref = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -262,7 +263,7 @@ decode_attn8_kernel(const Attn8Params p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1]));
+        pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], NJ == 2 ? sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1] : 0.f));
     }
     // values: tile i of 16 dims, dims 8 g + 2 i (fragment row g) and 8 g + 2 i + 1 (row g + 8)
 #pragma unroll
@@ -283,22 +284,25 @@ decode_attn8_kernel(const Attn8Params p) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[nt][i][j] = fmaf(w_top, d[nt][j], acc[nt][i][j]);
+        for (int j = 0; j < NJ; ++j) {
+          acc[nt][i][0][j] = fmaf(w_top, d[nt][j], acc[nt][i][0][j]);
+          acc[nt][i][1][j] = fmaf(w_top, d[nt][2 + j], acc[nt][i][1][j]);
+        }
     }
   }
 
-  // a warp's part: columns 2 t + j, dims 8 g ..
+  // a warp's part, of this lane's columns: dims 8 g ..
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       float sum = l[nt][j];
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const int col = nt * 8 + 2 * t + j;
+      const int col = nt * 8 + NJ * t + j;
       float* to = red[col][warp];
-      *reinterpret_cast<float4*>(to + 8 * g) = make_float4(acc[nt][0][j], acc[nt][0][2 + j], acc[nt][1][j], acc[nt][1][2 + j]);
-      *reinterpret_cast<float4*>(to + 8 * g + 4) = make_float4(acc[nt][2][j], acc[nt][2][2 + j], acc[nt][3][j], acc[nt][3][2 + j]);
+      *reinterpret_cast<float4*>(to + 8 * g) = make_float4(acc[nt][0][0][j], acc[nt][0][1][j], acc[nt][1][0][j], acc[nt][1][1][j]);
+      *reinterpret_cast<float4*>(to + 8 * g + 4) = make_float4(acc[nt][2][0][j], acc[nt][2][1][j], acc[nt][3][0][j], acc[nt][3][1][j]);
       if (g == 0) {
         to[kDD] = m[nt][j];
         to[kDD + 1] = sum;
@@ -432,10 +436,10 @@ int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* value
   MOC_REQUIRE(s->n_q <= 65535 && s->batch <= 65535, "too many query tokens or sequences for one launch");
   MOC_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(values)) & 15) == 0, "q and the K/V cache must be 16-byte aligned");
   const long long columns = static_cast<long long>(s->n_q) * (s->num_heads / s->num_kv_heads);
-  const int nt = columns <= 8 ? 1 : 2, runs = ceil_div(s->tokens_per_chapter, kRows);
-  const long long tiles = (columns + 8 * nt - 1) / (8 * nt), units = static_cast<long long>(s->n_chapters) * runs;
+  const int wide = columns <= 4 ? 4 : columns <= 8 ? 8 : 16, runs = ceil_div(s->tokens_per_chapter, kRows);
+  const long long tiles = (columns + wide - 1) / wide, units = static_cast<long long>(s->n_chapters) * runs;
   MOC_REQUIRE(tiles * s->num_kv_heads < (1ll << 27) && units < (1ll << 30), "decode-attention problem too large for one launch");
-  auto kern = nt == 1 ? decode_attn8_kernel<1> : decode_attn8_kernel<2>;
+  auto kern = wide == 4 ? decode_attn8_kernel<1, 1> : wide == 8 ? decode_attn8_kernel<1, 2> : decode_attn8_kernel<2, 2>;
   // a cluster per (sequence, KV head, tile of columns) while all of them are resident at once and every warp has a unit to take
   const long long groups = tiles * s->num_kv_heads * s->batch;
   int split = 8;
