@@ -125,7 +125,7 @@ class ProjectedBankCache:
         scaled by the chapters' weights ([B, n] ids and weights: a router's joint list).  ``counts`` [B] int32: how many entries of
         each list count (what lies behind them is not read; none: zeros, lse -inf).  Returns [B, n_q, H*64] bf16, with
         ``return_lse`` also the natural log of the softmax's denominator [B, n_q, H] fp32.  A chapter id outside the cache raises the
-        device status and is left out."""
+        device status and is left out.  For generation: no gradients."""
         heads, kv_heads = int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads)
         L.require_cuda(q, chapter_indices, chapter_weights, counts)
         if q.dtype != torch.bfloat16 or q.dim() != 3:
@@ -202,7 +202,7 @@ class MemoryDecoder:
                  wq: torch.Tensor, wo: torch.Tensor, *, num_heads: int, num_kv_heads: Optional[int] = None,
                  top_k: int, num_shared_chapters: int = 1, routed_scaling_factor: float = 2.5, router=None):
         """``router``: a ``ChapterRouter`` that selects by other rules than the reference's (its scores, balance bias and groups); its
-        weights stand for ``router_weight`` and ``router_bias`` then, which are not read."""
+        weights and ``top_k`` stand for ``router_weight``, ``router_bias`` and ``top_k`` then, which are not read."""
         self.cache = cache
         self.router = router if router is not None and router.by_logits else None
         self.router_weight, self.router_bias = router_weight, router_bias

@@ -81,13 +81,13 @@ class MemorySubBlock(nn.Module):
             raise ValueError("memory must be provided")
         a = self.memory_attn
         if self.post_norm is not None:
+            if next_norm is not None and (type(next_norm) is not type(self.post_norm) or next_norm.weight is None):
+                raise ValueError("next_norm must be a norm of this module's kind, with a weight")
             branch = F_moc.cross_attention(
                 hidden_states, memory, a.q_proj.weight, a.k_proj.weight, a.v_proj.weight, a.o_proj.weight,
                 a.num_heads, a.num_kv_heads, a._compute_dtype(hidden_states),
                 pre_norm="rms" if self.use_rms_norm else "layernorm", norm_weight=self.memory_layernorm.weight,
                 norm_bias=getattr(self.memory_layernorm, "bias", None), norm_eps=self.norm_eps, add_residual=False)
-            if next_norm is not None and isinstance(next_norm, RMSNorm) != self.use_rms_norm:
-                raise ValueError("next_norm must be a norm of this module's kind")
             return F_moc.gated_residual_norm(
                 hidden_states, branch, self.post_norm.weight, getattr(self.post_norm, "bias", None),
                 norm_type="rms" if self.use_rms_norm else "layernorm", eps=self.norm_eps,

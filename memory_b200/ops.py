@@ -315,7 +315,8 @@ def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, wa
     comb_w = torch.empty((rows, joint), dtype=f32, device=dev)
     load = torch.empty(s.num_chapters, dtype=i32, device=dev)
     stats = torch.empty((rows, 4), dtype=f32, device=dev) if want_stats else None
-    _issue("select_fwd", _DTYPE_TAG[logits.dtype], 2 if rows > 4 else 1, dev,
+    alone = 4 if s.num_chapters - s.num_shared <= 512 and k <= 31 else 1          # rows of one CTA, which counts its own picks
+    _issue("select_fwd", _DTYPE_TAG[logits.dtype], 2 if rows > alone else 1, dev,
            (C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(), comb_w.data_ptr(),
             L.ptr(stats), load.data_ptr()))
     return idx, weights, comb_idx, comb_w, load, stats

@@ -97,8 +97,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     step.  ``out``: one tensor per gradient (same shape, any of the three types) that receives the clipped values instead of the gradients.
 
     As with ``torch.nn.utils.clip_grad_norm_`` a norm that is NaN makes every gradient NaN and an infinite one gives the coefficient 0.
-    Squares are summed in 64 bits.  A tensor listed twice counts once; tensors that overlap otherwise are refused, and so are
-    more than 4096 of them."""
+    Squares are summed in 64 bits.  A tensor listed twice counts once; dense tensors that overlap otherwise are refused,
+    and so are more than 4096 tensors."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not eps >= 0:

@@ -51,25 +51,27 @@ class ChapterRouter(nn.Module):
                           "renormalize": renormalize}
         self.by_logits = (score, renormalize) != ("softmax", True) or balance_bias or top_groups not in (None, num_groups)
         self.last_load: Optional[torch.Tensor] = None
+        self._last_shared = 0
         self.register_buffer("balance_bias", torch.zeros(num_chapters) if balance_bias else None)
 
     def select(self, logits: torch.Tensor, num_shared: int, routed_scale: float = 1.0) -> F_moc.ChapterSelection:
         """This router's selection from logits [rows, num_chapters]."""
         got = F_moc.select_chapters(logits, self.top_k, balance_bias=self.balance_bias, num_shared=num_shared,
                                     routed_scale=routed_scale, **self.selection)
-        self.last_load = got.load
+        self.last_load, self._last_shared = got.load, num_shared
         return got
 
-    def update_balance(self, rate: float = 1e-3, load: Optional[torch.Tensor] = None, num_shared: int = 0) -> None:
+    def update_balance(self, rate: float = 1e-3, load: Optional[torch.Tensor] = None,
+                       num_shared: Optional[int] = None) -> None:
         """Moves the balance bias of every chapter behind the shared ones by ``rate`` towards the mean load: up where fewer rows
-        chose it, down where more did.  ``load`` [C] int32: the counts of a step (summed over ranks, say); the latest call's by
-        default."""
+        chose it, down where more did.  ``load`` [C] int32: the counts of a step (summed over ranks, say); they and ``num_shared`` are
+        the latest call's by default."""
         if self.balance_bias is None:
             raise ValueError("this router has no balance bias")
         load = self.last_load if load is None else load
         if load is None:
             raise ValueError("no load yet: route first, or pass the counts")
-        F_moc.ops.balance_bias_step(self.balance_bias, load, num_shared, rate)
+        F_moc.ops.balance_bias_step(self.balance_bias, load, self._last_shared if num_shared is None else num_shared, rate)
 
     def forward(self, hidden_states: torch.Tensor, return_losses: bool = True, exclude_prefix_chapters: int = 0,
                 rolling_window_size: Optional[int] = None
