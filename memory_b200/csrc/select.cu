@@ -230,22 +230,35 @@ __device__ __noinline__ bool rank_wide(const SelectParams& p, const unsigned lon
   }
   return unclear;
 }
-// The value of a group by 64-bit keys of the candidates that may be among its best, by one warp.
+// The value of a group by 64-bit keys of the candidates that may be among its best, by one warp.  (Eight loads in flight a lane: one
+// row that comes here would otherwise end after all others, 20 us late for groups of 512.)
 template <typename LT>
 __device__ __noinline__ uint64_t group_value64(const SelectParams& p, const LT* z, int g, float m, float inv_total, double total) {
-  const int lane = threadIdx.x & 31;
-  auto rough = [&](int c) {
-    const float v = logit_of(z, c);
-    if (masked(v)) return -INFINITY;
-    const float sc = p.sigmoid ? fast_sigmoid(v) : expf(v - m) * inv_total;
-    return p.bias != nullptr ? sc + p.bias[p.S + c] : p.top2 ? sc : v;
+  constexpr int kFlight = 8;
+  const int lane = threadIdx.x & 31, end = (g + 1) * p.per;
+  const bool biased = p.bias != nullptr;
+  const float* bias = biased ? p.bias + p.S : nullptr;
+  auto each = [&](auto go) {                           // go(candidate, its fast key), kFlight of a lane at a time
+    for (int c0 = g * p.per + lane; c0 < end; c0 += 32 * kFlight) {
+      float v[kFlight], b[kFlight];
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const bool in = c0 + 32 * i < end;
+        v[i] = in ? logit_of(z, c0 + 32 * i) : -INFINITY;
+        b[i] = in && biased ? bias[c0 + 32 * i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kFlight; ++i) {
+        const float sc = p.sigmoid ? fast_sigmoid(v[i]) : expf(v[i] - m) * inv_total;
+        go(c0 + 32 * i, masked(v[i]) ? -INFINITY : biased ? sc + b[i] : p.top2 ? sc : v[i]);
+      }
+    }
   };
   float a = -INFINITY, b = -INFINITY;
-  for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32) {
-    const float v = rough(c);
+  each([&](int, float v) {
     b = fmaxf(b, fminf(a, v));
     a = fmaxf(a, v);
-  }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
@@ -255,8 +268,9 @@ __device__ __noinline__ uint64_t group_value64(const SelectParams& p, const LT* 
   const float last = p.top2 ? b : a;
   const float edge = last - 2.f * key_error(p, last, inv_total);
   Best2<uint64_t> t{0, 0};
-  for (int c = g * p.per + lane; c < (g + 1) * p.per; c += 32)
-    if (rough(c) >= edge) take(t, key64(p, z, c, m, total, true));
+  each([&](int c, float v) {
+    if (c < end && v >= edge) take(t, key64(p, z, c, m, total, true));
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const uint64_t ka = __shfl_xor_sync(0xffffffffu, t.a, o), kb = __shfl_xor_sync(0xffffffffu, t.b, o);
@@ -643,6 +657,21 @@ struct StreamShared {
   uint16_t hits[kStreamHits];
 };
 // (explicit operations: the same number when a run is read again)
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 template <bool SIG> __device__ __forceinline__ float stream_score(float z, float m, float inv_total) {
   return SIG ? fast_sigmoid(z) : __fmul_rn(expf(__fsub_rn(z, m)), inv_total);
 }
@@ -652,7 +681,7 @@ template <bool SIG, bool BIAS> __device__ __forceinline__ float stream_key(float
 
 // SIG: sigmoid scores; BIAS: with a balance bias; GROUPS: some groups go.
 template <typename LT, int S, bool SIG, bool BIAS, bool GROUPS>
-__global__ void __launch_bounds__(32 * kWarpRows)
+__global__ void __launch_bounds__(32 * kWarpRows, 7)
 select_stream_kernel(const SelectParams p, const int chunks) {
   extern __shared__ uint32_t tops_all[];               // [kWarpRows][chunks][32] keys of the runs' maxima
   __shared__ StreamShared shared[kWarpRows];
@@ -698,30 +727,45 @@ select_stream_kernel(const SelectParams p, const int chunks) {
     for (int bt = 0; bt < batches; ++bt) {
       const int c0 = bt * 32 * kBatch + lane;          // within the group
       const LT* zg = zr + static_cast<long long>(g) * per + c0;
+      const float* bg = BIAS ? bias + g * per + c0 : nullptr;
       float z[kBatch], v[kBatch];
+      if ((bt + 1) * 32 * kBatch <= per) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) z[i] = c0 + 32 * i < per ? logit_of(zg, 32 * i) : -INFINITY;
-      if (BIAS) {
-        const float* bg = bias + g * per + c0;
+        for (int i = 0; i < kBatch; ++i) z[i] = logit_of(zg, 32 * i);
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) v[i] = c0 + 32 * i < per ? bg[32 * i] : 0.f;
+        for (int i = 0; i < kBatch; ++i) v[i] = BIAS ? bg[32 * i] : 0.f;
+      } else {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) z[i] = c0 + 32 * i < per ? logit_of(zg, 32 * i) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) v[i] = BIAS && c0 + 32 * i < per ? bg[32 * i] : 0.f;
       }
+      float low = z[0];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) v[i] = stream_key<SIG, BIAS>(z[i], BIAS ? v[i] : 0.f, m, inv_total);
+      for (int i = 1; i < kBatch; i += 2) low = i + 1 < kBatch ? min3(low, z[i], z[i + 1]) : fminf(low, z[i]);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) v[i] = BIAS ? __fadd_rn(stream_score<SIG>(z[i], m, inv_total), v[i]) : z[i];
+      if (masked(low)) {                               // (as stream_key has it)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) v[i] = masked(z[i]) ? -INFINITY : v[i];
+      }
 #pragma unroll
       for (int q = 0; q < kRuns; ++q) {
         float top = v[q * S];
 #pragma unroll
-        for (int i = 1; i < S; ++i) top = max_nan(top, v[q * S + i]);
+        for (int i = 1; i < S; i += 2) top = i + 1 < S ? max3_nan(top, v[q * S + i], v[q * S + i + 1]) : max_nan(top, v[q * S + i]);
         tops[((g * batches + bt) * kRuns + q) * 32 + lane] = to_key(top);
       }
       if (GROUPS) {
+        if (!BIAS && p.top2) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          float u = v[i];
-          if (!BIAS && p.top2) u = masked(z[i]) ? -INFINITY : stream_score<SIG>(z[i], m, inv_total);
-          b = fmaxf(b, fminf(a, u));
-          a = fmaxf(a, u);
+          for (int i = 0; i < kBatch; ++i) v[i] = masked(z[i]) ? -INFINITY : stream_score<SIG>(z[i], m, inv_total);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; i += 2) {          // the two largest of four, two of which are in order
+          const float hi = fmaxf(v[i], v[i + 1]), lo = fminf(v[i], v[i + 1]);
+          b = max3(b, lo, fminf(a, hi));
+          a = fmaxf(a, hi);
         }
       }
     }
