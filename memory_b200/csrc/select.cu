@@ -682,7 +682,7 @@ template <bool SIG, bool BIAS> __device__ __forceinline__ float stream_key(float
 // SIG: sigmoid scores; BIAS: with a balance bias; GROUPS: some groups go.
 template <typename LT, int S, bool SIG, bool BIAS, bool GROUPS>
 __global__ void __launch_bounds__(32 * kWarpRows, 7)
-select_stream_kernel(const SelectParams p, const int chunks) {
+select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group_batches) {
   extern __shared__ uint32_t tops_all[];               // [kWarpRows][chunks][32] keys of the runs' maxima
   __shared__ StreamShared shared[kWarpRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -693,9 +693,14 @@ select_stream_kernel(const SelectParams p, const int chunks) {
   const LT* zr = static_cast<const LT*>(p.logits) + row * p.ld + p.S;
   const float* bias = BIAS ? p.bias + p.S : nullptr;
   const int groups = GROUPS ? p.groups : 1, per = GROUPS ? p.per : p.N;
-  const int batches = (per + 32 * kBatch - 1) / (32 * kBatch);         // of a group
+  const int batches = group_batches.d;                                 // of a group
   constexpr int kRuns = kBatch / S;                                    // of a batch
   constexpr uint32_t kNone = 0x007FFFFFu;                              // key of -inf
+  if (lane == 0) {                                     // the row on its way to L2 as a whole (its 16-byte pieces)
+    const uintptr_t first = (reinterpret_cast<uintptr_t>(zr) + 15) & ~uintptr_t{15}, end = reinterpret_cast<uintptr_t>(zr + p.N) & ~uintptr_t{15};
+    if (end > first)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(first), "r"(static_cast<uint32_t>(end - first)) : "memory");
+  }
 
   float m = 0.f, total = 1.f, inv_total = 1.f;
   if (!SIG) {                                          // maximum and sum, a lane's own until the end
@@ -770,12 +775,11 @@ select_stream_kernel(const SelectParams p, const int chunks) {
       }
     }
     if (GROUPS) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-        b = fmaxf(fminf(a, oa), fmaxf(b, ob));
-        a = fmaxf(a, oa);
-      }
+      // (neither is NaN) the largest, then the largest of what is left: its lane's second, the others' first
+      const uint32_t mine = to_key(a), best = __reduce_max_sync(0xffffffffu, mine);
+      const uint32_t holders = __ballot_sync(0xffffffffu, mine == best);
+      a = of_key(best);
+      if (p.top2) b = of_key(__reduce_max_sync(0xffffffffu, lane == __ffs(holders) - 1 ? to_key(b) : mine));
       if (lane == (g & 31)) value[g >> 5] = p.top2 && b > -INFINITY ? a + b : a;
     }
   }
@@ -803,7 +807,7 @@ select_stream_kernel(const SelectParams p, const int chunks) {
       stays[1] = static_cast<uint32_t>(kept >> 32);
     }
     for (int i = 0; i < chunks; ++i) {
-      const int g = i / (batches * kRuns);
+      const int g = div_of(i / kRuns, group_batches);
       // (NaN stays to be seen)
       if (!((g < 32 ? stays[0] >> g : stays[1] >> (g - 32)) & 1) && tops[i * 32 + lane] != 0xFFFFFFFFu) tops[i * 32 + lane] = kNone;
     }
@@ -854,18 +858,30 @@ select_stream_kernel(const SelectParams p, const int chunks) {
     __syncwarp();
     sure = runs <= kStreamHits && edge < INFINITY;
     if (sure) {
-      for (int h = 0; h < runs; h += 32 / S) {
-        const int j = h + lane / S;
-        const int run = j < runs ? s.hits[j] : 0, i = run >> 5;
-        const int bt = i / kRuns, g = GROUPS ? bt / batches : 0;
-        const int c = ((bt - g * batches) * kBatch + (i - bt * kRuns) * S + lane % S) * 32 + (run & 31);     // within the group
-        float v = -INFINITY;
-        if (j < runs && c < per) v = stream_key<SIG, BIAS>(logit_of(zr, static_cast<long long>(g) * per + c), BIAS ? bias[g * per + c] : 0.f, m, inv_total);
-        const bool in = v >= edge && v > -INFINITY;
-        const uint32_t votes = __ballot_sync(0xffffffffu, in);
-        const int pos = n + __popc(votes & ((1u << lane) - 1u));
-        if (in && pos < kStreamCand) s.cand[pos] = static_cast<unsigned long long>(to_key(v)) << 32 | ~static_cast<uint32_t>(g * per + c);
-        n += __popc(votes);
+      constexpr int kFlight = 4;
+      for (int h = 0; h < runs; h += kFlight * 32 / S) {
+        float z[kFlight], add[kFlight];
+        int id[kFlight];
+#pragma unroll
+        for (int q = 0; q < kFlight; ++q) {
+          const int j = h + q * (32 / S) + lane / S;
+          const int run = j < runs ? s.hits[j] : 0, i = run >> 5;
+          const int bt = i / kRuns, g = GROUPS ? div_of(bt, group_batches) : 0;
+          const int c = ((bt - g * batches) * kBatch + (i - bt * kRuns) * S + lane % S) * 32 + (run & 31);     // within the group
+          const bool real = j < runs && c < per;
+          id[q] = g * per + c;
+          z[q] = real ? logit_of(zr, id[q]) : -INFINITY;
+          add[q] = BIAS && real ? bias[id[q]] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < kFlight; ++q) {
+          const float v = stream_key<SIG, BIAS>(z[q], add[q], m, inv_total);
+          const bool in = v >= edge && v > -INFINITY;
+          const uint32_t votes = __ballot_sync(0xffffffffu, in);
+          const int pos = n + __popc(votes & ((1u << lane) - 1u));
+          if (in && pos < kStreamCand) s.cand[pos] = static_cast<unsigned long long>(to_key(v)) << 32 | ~static_cast<uint32_t>(id[q]);
+          n += __popc(votes);
+        }
       }
       __syncwarp();
       sure = n <= kStreamCand && n >= min(need, p.k);
@@ -1422,14 +1438,14 @@ int check(const moc_select_shape* s) {
 template <typename LT, int S> int select_stream(const SelectParams& p, cudaStream_t stream) {
   const bool grouped = p.keep < p.groups, biased = p.bias != nullptr;
   const int per = grouped ? p.per : p.N;
-  const int chunks = (grouped ? p.groups : 1) * ((per + 32 * kBatch - 1) / (32 * kBatch)) * (kBatch / S);
+  const int batches = ceil_div(per, 32 * kBatch), chunks = (grouped ? p.groups : 1) * batches * (kBatch / S);
   auto kern = grouped ? (p.sigmoid ? (biased ? select_stream_kernel<LT, S, true, true, true> : select_stream_kernel<LT, S, true, false, true>)
                                    : (biased ? select_stream_kernel<LT, S, false, true, true> : select_stream_kernel<LT, S, false, false, true>))
                       : (p.sigmoid ? (biased ? select_stream_kernel<LT, S, true, true, false> : select_stream_kernel<LT, S, true, false, false>)
                                    : (biased ? select_stream_kernel<LT, S, false, true, false> : select_stream_kernel<LT, S, false, false, false>));
   const size_t bytes = static_cast<size_t>(kWarpRows) * chunks * 128;
   MOC_CUDA_OK(allow_shared(kern, bytes, 128 * 1024));
-  kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, bytes, stream>>>(p, chunks);
+  kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, bytes, stream>>>(p, chunks, fast_div(batches));
   MOC_CUDA_OK(cudaGetLastError());
   return MOC_OK;
 }
