@@ -927,22 +927,20 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
       }
       n = left;
     }
-    bool close = false;
     for (int t = lane; t < n; t += 32) {
       const unsigned long long mine = s.cand[t];
-      unsigned long long next = 0;                     // the largest below it
       int rank = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const unsigned long long o = s.cand[j];
-        rank += o > mine;
-        if (BIAS && o < mine && o > next) next = o;
-      }
-      if (rank < p.k) {
-        s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
-        if (BIAS && next != 0 &&
-            !apart(p, of_key(static_cast<uint32_t>(mine >> 32)), of_key(static_cast<uint32_t>(next >> 32)), inv_total)) close = true;
-      }
+      for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+      if (BIAS) s.wide[rank] = mine;                   // in order
+      if (rank < p.k) s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
+    }
+    bool close = false;
+    if (BIAS) {
+      __syncwarp();
+      for (int t = lane; t < p.k && t + 1 < n; t += 32)
+        if (!apart(p, of_key(static_cast<uint32_t>(s.wide[t] >> 32)), of_key(static_cast<uint32_t>(s.wide[t + 1] >> 32)), inv_total)) close = true;
+      __syncwarp();
     }
     if (BIAS && __any_sync(0xffffffffu, close)) {      // again by 64-bit keys
       double t64 = total;
@@ -1251,19 +1249,16 @@ select_cta_kernel(const SelectParams p) {
     if (sure) {
       for (int t = threadIdx.x; t < n; t += TH) {
         const unsigned long long mine = s.cand[t];
-        unsigned long long next = 0;                // the largest below it
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-          const unsigned long long o = s.cand[j];
-          rank += o > mine;
-          if (biased && o < mine && o > next) next = o;
-        }
-        if (rank < p.k) {
-          s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
-          if (next != 0 && !apart(p, of_key(static_cast<uint32_t>(mine >> 32)), of_key(static_cast<uint32_t>(next >> 32)), inv_total))
-            s.close = 1;
-        }
+        for (int j = 0; j < n; ++j) rank += s.cand[j] > mine;
+        if (biased) keys[rank] = mine;              // in order
+        if (rank < p.k) s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
+      }
+      if (biased) {
+        __syncthreads();
+        for (int t = threadIdx.x; t < p.k && t + 1 < n; t += TH)
+          if (!apart(p, of_key(static_cast<uint32_t>(keys[t] >> 32)), of_key(static_cast<uint32_t>(keys[t + 1] >> 32)), inv_total)) s.close = 1;
       }
       __syncthreads();
       if (s.close) {                                // the candidates again by 64-bit keys
