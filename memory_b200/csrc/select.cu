@@ -13,8 +13,10 @@
 // concerned are ranked again by 64-bit keys.  Rows that this does not settle (groups that close, NaN, fewer candidates than
 // places) run through the same selection in 64 bits as a whole.  Bare logits need no arithmetic and are always sure.
 //
-// Bound by HBM for many rows (4 bytes a logit read), by latency for a few.  Up to 512 candidates and k < 32 a warp has a
-// row in registers, beyond that a CTA.  Either way the k + 1 largest lie among the values above a bound that at least k + 1 of
+// Bound by HBM for many rows (4 bytes a logit read) by right, by issuing in fact, and by latency for a few.  Up to 512 candidates and
+// k < 32 a warp has a row in registers (257 chapters, k = 8, sigmoid, bias, groups: 1 row 8 us, 1,000 rows 12, 8,192 rows 31; by a CTA
+// a row 10, 27 and 107; 513 chapters, k = 31, softmax, bias: 12, 18.5 and 105 against 10, 29 and 119), beyond that a CTA, or a warp
+// that streams it where there are many.  Either way the k + 1 largest lie among the values above a bound that at least k + 1 of
 // the threads' own maxima reach, found by bisection; what lies above it is ranked.
 #include "moc_common.cuh"
 
@@ -642,9 +644,13 @@ select_warp_kernel(const SelectParams p) {
 // ---- a warp a row, many rows of many candidates -----------------------------------------------
 // The row streams by (16 loads a lane in flight); what stays of it are the maxima of runs of S candidates a lane, in shared
 // memory.  A bound on those that k + 1 of them reach leaves some dozens of runs, which are read again for the candidates.  No
-// barrier, a third of the instructions of a CTA a row.
+// barrier, a third of the instructions of a CTA a row.  Bound by issuing: 8,192 rows of 4,097 fp32 logits, sigmoid with a bias, 4 of 8
+// groups, k = 16: 68 us (2.0 TB/s; 4,840 instructions a row, 0.59 a cycle and scheduler, two rounds of rows).
+// Against a CTA a row (4,097 chapters, us): k = 16, sigmoid, bias, groups: 300 rows 20.5 / 20.5 CTA, 600 rows 23 / 26, 1,200 rows 27 / 42,
+// 2,400 rows 33 / 66; k = 16, plain softmax: 300 rows 23 / 16, 600 rows 23 / 23, 2,400 rows 33 / 55; k = 64, softmax, bias: 600 rows
+// 55 / 39, 1,200 rows 59 / 53, 2,400 rows 74 / 86, 8,192 rows 151 / 184.
 constexpr int kStreamMostK = 64, kStreamHits = 256, kStreamCand = 256, kBatch = 16;
-constexpr int kStreamRows = 600;
+constexpr int kStreamRows = 600, kStreamRowsManyPicks = 1500;      // k <= 32, and more
 struct StreamShared {
   union {
     struct {
@@ -1450,7 +1456,7 @@ template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream
     auto kern = p.N <= 64 ? select_warp_kernel<LT, 2> : p.N <= 128 ? select_warp_kernel<LT, 4>
                 : p.N <= 256 ? select_warp_kernel<LT, 8> : select_warp_kernel<LT, 16>;
     kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, 0, stream>>>(p);
-  } else if (p.rows >= kStreamRows && p.k <= kStreamMostK && p.N > kWarpMostN && (!grouped || p.per >= 256)) {
+  } else if (p.rows >= (p.k <= 32 ? kStreamRows : kStreamRowsManyPicks) && p.k <= kStreamMostK && p.N > kWarpMostN && (!grouped || p.per >= 256)) {
     return p.N > 2048 ? select_stream<LT, 16>(p, stream) : select_stream<LT, 4>(p, stream);
   } else {
     const bool big = p.N > 4096;
