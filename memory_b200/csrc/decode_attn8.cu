@@ -22,6 +22,9 @@
 // distributed shared memory.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+#include <climits>
+
 #include "host_pass.cuh"
 
 namespace moc {
@@ -35,13 +38,13 @@ struct Attn8Params {
   const __nv_bfloat16* q;
   const uint8_t* values;
   const float* scales;                 // [bank_rows / scale_rows, 2 * HK]
-  long long bank_rows;
+  int chapters;                        // of the cache
   const int* comb_idx;
   const float* comb_w;
   const int* counts;                   // chapters of each list that count (NULL: all)
   __nv_bfloat16* out;
   float* lse;
-  int n_q, H, HK, n_ch, T, split, tiles;        // tiles of columns of a KV head
+  int n_q, H, HK, n_ch, T, split, tiles, blocks;       // tiles of columns of a KV head; blocks of scales of a chapter
   float scale;
   FastDiv scale_rows, runs;
   int* status;
@@ -94,7 +97,7 @@ decode_attn8_kernel(const Attn8Params p) {
   const int rank = static_cast<int>(blockIdx.x) % split, tile = static_cast<int>(blockIdx.x) / split % p.tiles;
   const int kh = static_cast<int>(blockIdx.x) / split / p.tiles, b = blockIdx.y;
   const int per_kv = p.H / HK, columns = min(kCols, p.n_q * per_kv - tile * kCols);      // column j: token j / per_kv, head kh per_kv + j % per_kv
-  const long long row_bytes = 2ll * HK * kDD;
+  const int row_bytes = 2 * HK * kDD;
   auto q_row = [&](int col) {
     const int j = tile * kCols + col, iq = j / per_kv;
     return (static_cast<long long>(b) * p.n_q + iq) * p.H + kh * per_kv + (j - iq * per_kv);
@@ -151,32 +154,33 @@ decode_attn8_kernel(const Attn8Params p) {
   for (int unit = rank * kWarps + warp; unit < n_ch * p.runs.d; unit += split * kWarps) {
     const int c = div_of(unit, p.runs), r0 = (unit - c * p.runs.d) * kRows;
     const int ch = list[c];
-    if (ch < 0 || (static_cast<long long>(ch) + 1) * T > p.bank_rows) {
+    if (static_cast<unsigned>(ch) >= static_cast<unsigned>(p.chapters)) {
       if (lane == 0) atomicMax(p.status, MOC_DEV_BAD_INDEX);
       continue;
     }
     const float u = weights[c];
     const bool whole = r0 + kRows <= T;
-    const uint8_t* chapter = p.values + static_cast<long long>(ch) * T * row_bytes + kh * kDD;
+    const uint8_t* rows = p.values + (static_cast<long long>(ch) * T + r0) * row_bytes + kh * kDD;
     uint4 kr[2][2];                    // rows 16 mt + g and + 8, bytes 16 t ..
     uint2 vr[2][4];                    // rows 16 ks + {2 t, 2 t + 1, 2 t + 8, 2 t + 9}, bytes 8 g ..
+    if (whole) {
+      const uint8_t* k_at = rows + (g * row_bytes + 16 * t);
+      const uint8_t* v_at = rows + (2 * t * row_bytes + HK * kDD + 8 * g);
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+      for (int i = 0; i < 4; ++i) kr[i >> 1][i & 1] = *reinterpret_cast<const uint4*>(k_at + 8 * i * row_bytes);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = r0 + 16 * mt + 8 * h + g;
-        kr[mt][h] = *reinterpret_cast<const uint4*>(chapter + (r < T ? r : 0) * row_bytes + 16 * t);
-      }
+      for (int i = 0; i < 8; ++i) vr[i >> 2][i & 3] = *reinterpret_cast<const uint2*>(v_at + ((i & 1) + 8 * (i >> 1)) * row_bytes);
+    } else {                           // (what lies behind the chapter: its last row again, whose probability is 0)
+      const int last = T - 1 - r0;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+      for (int i = 0; i < 4; ++i) kr[i >> 1][i & 1] = *reinterpret_cast<const uint4*>(rows + min(8 * i + g, last) * row_bytes + 16 * t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 16 * ks + 2 * t + (i & 1) + 8 * (i >> 1);
-        vr[ks][i] = *reinterpret_cast<const uint2*>(chapter + (r < T ? r : 0) * row_bytes + HK * kDD + 8 * g);
-      }
+      for (int i = 0; i < 8; ++i)
+        vr[i >> 2][i & 3] = *reinterpret_cast<const uint2*>(rows + min((i & 1) + 8 * (i >> 1) + 2 * t, last) * row_bytes + HK * kDD + 8 * g);
+    }
     // row factors of this lane's four rows (mt, h): scores, and values relative to `w_top`
     float kf[2][2], vf[2][2], w_top;
-    const long long blk0 = static_cast<long long>(ch) * (T / p.scale_rows.d);
+    const long long blk0 = static_cast<long long>(ch) * p.blocks;
     if (one_block) {
       const float* sc = p.scales + (blk0 + div_of(r0, p.scale_rows)) * 2 * HK + kh;
       const float ks = sc[0] * u;
@@ -439,6 +443,7 @@ int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* value
   const long long columns = static_cast<long long>(s->n_q) * (s->num_heads / s->num_kv_heads);
   const int wide = columns <= 4 ? 4 : columns <= 8 ? 8 : 16, runs = ceil_div(s->tokens_per_chapter, kRows);
   const long long tiles = (columns + wide - 1) / wide, units = static_cast<long long>(s->n_chapters) * runs;
+  MOC_REQUIRE(s->num_kv_heads <= (1 << 18), "too many KV heads");          // (32 rows are below 2^31 bytes)
   MOC_REQUIRE(tiles * s->num_kv_heads < (1ll << 27) && units < (1ll << 30), "decode-attention problem too large for one launch");
   auto kern = wide == 4 ? decode_attn8_kernel<1, 1> : wide == 8 ? decode_attn8_kernel<1, 2> : decode_attn8_kernel<2, 2>;
   // a cluster per (sequence, KV head, tile of columns) while all of them are resident at once and every warp has a unit to take
@@ -446,7 +451,8 @@ int decode_attn_e4m3(const moc_decode_shape* s, const void* q, const void* value
   int split = 8;
   while (split > 1 && (split / 2 * kWarps >= units || groups > resident_clusters(kern, kThreads, 0, split))) split /= 2;
   Attn8Params p{};
-  p.q = static_cast<const __nv_bfloat16*>(q); p.values = static_cast<const uint8_t*>(values); p.scales = scales; p.bank_rows = bank_rows;
+  p.q = static_cast<const __nv_bfloat16*>(q); p.values = static_cast<const uint8_t*>(values); p.scales = scales;
+  p.chapters = static_cast<int>(std::min<int64_t>(bank_rows / s->tokens_per_chapter, INT_MAX)); p.blocks = s->tokens_per_chapter / scale_rows;
   p.comb_idx = comb_idx; p.comb_w = comb_w; p.counts = counts; p.out = static_cast<__nv_bfloat16*>(out); p.lse = lse;
   p.n_q = s->n_q; p.H = s->num_heads; p.HK = s->num_kv_heads; p.n_ch = s->n_chapters; p.T = s->tokens_per_chapter;
   p.split = split; p.tiles = static_cast<int>(tiles); p.scale = s->scale; p.scale_rows = fast_div(scale_rows); p.runs = fast_div(runs);
