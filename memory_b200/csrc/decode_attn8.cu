@@ -151,14 +151,26 @@ decode_attn8_kernel(const Attn8Params p) {
   }
 
   const bool one_block = p.scale_rows.d % kRows == 0;          // a unit lies in one block of scales
-  for (int unit = rank * kWarps + warp; unit < n_ch * p.runs.d; unit += split * kWarps) {
-    const int c = div_of(unit, p.runs), r0 = (unit - c * p.runs.d) * kRows;
-    const int ch = list[c];
+  const int units = n_ch * p.runs.d, stride = split * kWarps;
+  int next_ch = 0, next_r0 = 0;                  // of the unit that follows, fetched while one is worked on
+  float next_u = 0.f;
+  auto look_up = [&](int unit) {
+    if (unit < units) {
+      const int c = div_of(unit, p.runs);
+      next_r0 = (unit - c * p.runs.d) * kRows;
+      next_ch = list[c];
+      next_u = weights[c];
+    }
+  };
+  look_up(rank * kWarps + warp);
+  for (int unit = rank * kWarps + warp; unit < units; unit += stride) {
+    const int ch = next_ch, r0 = next_r0;
+    const float u = next_u;
     if (static_cast<unsigned>(ch) >= static_cast<unsigned>(p.chapters)) {
       if (lane == 0) atomicMax(p.status, MOC_DEV_BAD_INDEX);
+      look_up(unit + stride);
       continue;
     }
-    const float u = weights[c];
     const bool whole = r0 + kRows <= T;
     const uint8_t* rows = p.values + (static_cast<long long>(ch) * T + r0) * row_bytes + kh * kDD;
     uint4 kr[2][2];                    // rows 16 mt + g and + 8, bytes 16 t ..
@@ -178,6 +190,7 @@ decode_attn8_kernel(const Attn8Params p) {
       for (int i = 0; i < 8; ++i)
         vr[i >> 2][i & 3] = *reinterpret_cast<const uint2*>(rows + min((i & 1) + 8 * (i >> 1) + 2 * t, last) * row_bytes + HK * kDD + 8 * g);
     }
+    look_up(unit + stride);
     // row factors of this lane's four rows (mt, h): scores, and values relative to `w_top`
     float kf[2][2], vf[2][2], w_top;
     const long long blk0 = static_cast<long long>(ch) * p.blocks;
