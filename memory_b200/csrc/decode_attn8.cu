@@ -4,12 +4,14 @@
 // products, so the values go into them as they are stored (u_c: the weight of chapter c):
 //   s_r = scale * u_c * ks_r * <q, K8[r]>,   out = sum_r softmax(s)_r * u_c * vs_r * V8[r]   (one joint softmax).
 //
-// A full batch should be bound by HBM (one byte an element) and is bound by issuing; a few sequences by latency.  All queries on a KV
-// head (its heads, the tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted once for up to
-// 16 of them; e4m3 -> fp16 is exact.  64 sequences of 4,160 rows, 12 heads: 84 us (3.2 TB/s of HBM; 410 instructions a unit of 32
-// rows at 0.56 a cycle and scheduler, the conversions being the most of them); 13 sequences of 3 tokens, 12 heads on 4, 47 chapters of
-// 64 rows: 15.4 us.  On CUDA cores that took 95 and 19 us; units by bulk tensor copies into a ring 99 and 16.5 (92 and 15.4 without);
-// e4m3 matrix instructions of single warps, queries and probabilities in three terms, 102 and 33.
+// A full batch should be bound by HBM (one byte an element) and is bound by latency and issuing; a few sequences by latency.  All
+// queries on a KV head (its heads, the tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted
+// once for up to 16 of them; e4m3 -> fp16 is exact.  64 sequences of 4,160 rows, 12 heads: 70 us (3.8 TB/s of HBM, 6.3 from L2's side;
+// 340 instructions a unit of 32 rows at 0.51 a cycle and scheduler, 24 warps on an SM); 13 sequences of 3 tokens, 12 heads on 4, 47
+// chapters of 64 rows: 15 us; one sequence of 4,160 rows, 12 heads: 7.4 us.  Measured on the way, of these kernels' own stages: on CUDA
+// cores 95 us against 97 and 19 against 16; units by bulk tensor copies into a ring 99 against 92; e4m3 matrix instructions of single
+// warps (16 of them take 175 instructions, fp16 ones 66: they convert too), queries and probabilities in three terms, 102 against 97 and
+// 33 against 16; the next unit's rows in registers too, with 16 warps on an SM, 79 against 70; 32 warps at 64 registers 90 against 70.
 //   - scores: A = 16 keys x 16 dims, B = dims x 8 queries.  The order of the dims is free, so a lane's 16 bytes of its row are
 //     the A fragments of four steps as they come.  Queries are scaled by a power of two into fp16's range (their largest to
 //     128..256; what falls below fp16's smallest number is 2^-31 of the largest).
@@ -17,7 +19,7 @@
 //     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
 //     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
 // The softmax's reference of a column is a score already met; it moves to the largest only when a score passes it by 2^8, which saves
-// most units the reduction across lanes and the rescaling (92 us with, 97 without).  References, sums and accumulators are fp32.  A
+// most units the reduction across lanes and the rescaling (92 us with, 97 without, before the steps on addresses).  References, sums and accumulators are fp32.  A
 // cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through shared memory, then
 // distributed shared memory.
 #include <cuda_fp16.h>
@@ -85,7 +87,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // NT: tiles of 8 columns.  Lane (g, t) = (lane / 4, lane % 4) has the scores of columns 2 t and 2 t + 1; NJ = 1: up to four queries take
-// the even ones and the odd ones' work is left out (one query a KV head: 84 us against 92).
+// the even ones and the odd ones' work is left out (one query a KV head: 84 us against 92, likewise).
 template <int NT, int NJ>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 decode_attn8_kernel(const Attn8Params p) {
