@@ -211,8 +211,9 @@ decode_attn_kernel(const DecodeParams p) {
         a = a * f0 + ((e & 1) ? ab.y : ab.x) * f1;
         mt = m_new;
       }
-      p.out[(q_row + h0 + g) * kDD + e] = __float2bfloat16(lt > 0.f ? a / lt : 0.f);
-      if (e == 0 && p.lse != nullptr) p.lse[q_row + h0 + g] = lt > 0.f ? (mt + log2f(lt)) / kDecLog2e : -INFINITY;
+      const bool any = lt != 0.f;                // (a list without rows has no sum; a NaN in the cache or the query stays one)
+      p.out[(q_row + h0 + g) * kDD + e] = __float2bfloat16(any ? a / lt : 0.f);
+      if (e == 0 && p.lse != nullptr) p.lse[q_row + h0 + g] = any ? (mt + log2f(lt)) / kDecLog2e : -INFINITY;
     }
   }
   if (split > 1) cluster_sync();       // nobody leaves while its part is read

@@ -19,9 +19,9 @@
 //     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
 //     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
 // The softmax's reference of a column is a score already met; it moves to the largest only when a score passes it by 2^8, which saves
-// most units the reduction across lanes and the rescaling (92 us with, 97 without, before the steps on addresses).  References, sums and accumulators are fp32.  A
-// cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through shared memory, then
-// distributed shared memory.
+// most units the reduction across lanes and the rescaling (92 us with, 97 without, before the steps on addresses).  References, sums
+// and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through
+// shared memory, then distributed shared memory.
 #include <cuda_fp16.h>
 
 #include <algorithm>

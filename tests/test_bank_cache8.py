@@ -163,6 +163,27 @@ def test_a_nan_query_or_block_gives_nan():
     assert got[0, 1].isfinite().all() and got[1, 0].isfinite().all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("chapters", [2, 40])
+def test_nan_shows_over_either_cache(dtype, chapters):
+    """A query, a key row or a value row with a NaN gives NaN and touches nothing else; one warp's unit among many, or all there is."""
+    import memory_b200 as M
+    kv = _kv(chapters * 16, 2, 1)
+    kv[16 + 3, 5] = float("nan")                          # a key row of head 0, chapter 1
+    kv[8, 3 * 64 + 7] = float("nan")                      # a value row of head 1, chapter 0
+    cache = M.ProjectedBankCache.from_rows(kv, 16, cache_dtype=dtype)
+    q = torch.randn(3, 2, 128, device="cuda").bfloat16()
+    q[2, 1, 64 + 9] = float("nan")                        # sequence 2, token 1, head 1
+    idx = torch.stack([torch.arange(chapters), torch.arange(chapters).clamp(min=1), torch.full((chapters,), 1)]).cuda()
+    out, lse = cache.attend(q, idx, torch.full(idx.shape, 0.5, device="cuda"), 2, return_lse=True)
+    out = out.view(3, 2, 2, 64)                           # [sequence, token, head, dim]
+    assert out[:, :, 0].isnan().all() and lse[:, :, 0].isnan().all()
+    assert out[0, :, 1].isnan().any(-1).all() and lse[0, :, 1].isfinite().all()
+    assert out[1, :, 1].isfinite().all() and out[2, 0, 1].isfinite().all()
+    assert out[2, 1, 1].isnan().all() and lse[2, 1, 1].isnan()
+
+
 def _decoder(cache_kw, router=None, kv_heads=4):
     import memory_b200 as M
     torch.manual_seed(3)
