@@ -16,8 +16,10 @@
 //     the A fragments of four steps as they come.  Queries are scaled by a power of two into fp16's range (their largest to
 //     128..256; what falls below fp16's smallest number is 2^-31 of the largest).
 //   - values: A = 16 dims x 16 rows, transposed from rows by byte permutations within a lane; B = the probabilities, which a matrix
-//     transposition brings from the scores' layout.  They are rounded to fp16 (2^-11 of their own, below the result's bf16; those
-//     under 6e-8 of the largest vanish).  Row scales that differ within a unit go in relative to the unit's largest.
+//     transposition brings from the scores' layout.  They go in as two fp16 terms (the second in the odd columns where those are idle,
+//     else by instructions of its own): 2^-21 of their own, not below 2^-32 of the largest.  With one term results that cancel lose
+//     their last bits and one in ten elements rounds to the neighbouring bf16 number; it costs 73.7 us against 71.8 (64 sequences),
+//     28.7 against 26.6 (six queries a KV head).  Row scales that differ within a unit go in relative to the unit's largest.
 // The softmax's reference of a column is a score already met; it moves to the largest only when a score passes it by 2^8, which saves
 // most units the reduction across lanes and the rescaling (92 us with, 97 without, before the steps on addresses).  References, sums
 // and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through
@@ -34,7 +36,8 @@ namespace {
 
 constexpr int kDD = 64, kThreads = 256, kWarps = kThreads / 32, kRows = 32;      // rows of a unit
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kHeadroom = 8.f;       // a score may pass its column's reference by 2^8 before that moves: fp16 probabilities reach 65504
+constexpr float kHeadroom = 8.f;       // a score may pass its column's reference by 2^8 before that moves
+constexpr float kLift = 128.f;         // on probabilities on their way into fp16: at most 2^8 of them, so 2^15 of 65,504; normal from 2^-21 on
 
 struct Attn8Params {
   const __nv_bfloat16* q;
@@ -80,6 +83,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// x = first + rest to 2^-21 of x (2^-25 where x is below fp16's normal range): both go into the products
+__device__ __forceinline__ float leading11(float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFFE000u); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -199,9 +204,9 @@ decode_attn8_kernel(const Attn8Params p) {
     if (one_block) {
       const float* sc = p.scales + (blk0 + div_of(r0, p.scale_rows)) * 2 * HK + kh;
       const float ks = sc[0] * u;
-      w_top = sc[HK] * u;
+      w_top = sc[HK] * (u * (1.f / kLift));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { kf[i >> 1][i & 1] = ks; vf[i >> 1][i & 1] = 1.f; }
+      for (int i = 0; i < 4; ++i) { kf[i >> 1][i & 1] = ks; vf[i >> 1][i & 1] = kLift; }
     } else {
       w_top = 0.f;
 #pragma unroll
@@ -210,16 +215,18 @@ decode_attn8_kernel(const Attn8Params p) {
         const float* sc = p.scales + (blk0 + div_of(r < T ? r : 0, p.scale_rows)) * 2 * HK + kh;
         kf[i >> 1][i & 1] = sc[0] * u;
         vf[i >> 1][i & 1] = sc[HK];
-        w_top = max_nan(w_top, sc[HK]);
+        w_top = fmaxf(w_top, fabsf(sc[HK]));
       }
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) w_top = max_nan(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
-      const float inv = w_top > 0.f ? 1.f / w_top : 0.f;
+      for (int o = 4; o < 32; o <<= 1) w_top = fmaxf(w_top, __shfl_xor_sync(0xffffffffu, w_top, o));
+      w_top = fmaxf(w_top, 0x1p-100f);           // (its reciprocal is finite; an infinite or NaN scale makes its row's factor NaN)
+      const float inv = kLift / w_top;
 #pragma unroll
       for (int i = 0; i < 4; ++i) vf[i >> 1][i & 1] *= inv;
-      w_top *= u;
+      w_top *= u * (1.f / kLift);
     }
     uint32_t pb[NT][2][2];             // probabilities as B fragments: rows 16 ks + 2 t + {0, 1} and + 8, column g
+    uint32_t rest[NJ == 2 ? NT : 1][2][2];       // ... and what fp16 leaves of them (NJ = 1: in the odd columns)
     float sc[2][NT][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -282,8 +289,16 @@ decode_attn8_kernel(const Attn8Params p) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pb[nt][i >> 1][i & 1] = transpose8(pack_f16(sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], NJ == 2 ? sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1] : 0.f));
+      for (int i = 0; i < 4; ++i) {
+        const float p0 = sc[i >> 1][nt][2 * (i & 1)] * vf[i >> 1][i & 1], h0 = leading11(p0);
+        if constexpr (NJ == 2) {
+          const float p1 = sc[i >> 1][nt][2 * (i & 1) + 1] * vf[i >> 1][i & 1], h1 = leading11(p1);
+          pb[nt][i >> 1][i & 1] = transpose8(pack_f16(h0, h1));
+          rest[nt][i >> 1][i & 1] = transpose8(pack_f16(p0 - h0, p1 - h1));
+        } else {
+          pb[nt][i >> 1][i & 1] = transpose8(pack_f16(h0, p0 - h0));
+        }
+      }
     }
     // values: tile i of 16 dims, dims 8 g + 2 i (fragment row g) and 8 g + 2 i + 1 (row g + 8)
 #pragma unroll
@@ -299,14 +314,15 @@ decode_attn8_kernel(const Attn8Params p) {
         for (int nt = 0; nt < NT; ++nt) {
           if (ks == 0) mma_f16_new(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
           else mma_f16(d[nt], a0, a1, a2, a3, pb[nt][ks][0], pb[nt][ks][1]);
+          if constexpr (NJ == 2) mma_f16(d[nt], a0, a1, a2, a3, rest[nt][ks][0], rest[nt][ks][1]);
         }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          acc[nt][i][0][j] = fmaf(w_top, d[nt][j], acc[nt][i][0][j]);
-          acc[nt][i][1][j] = fmaf(w_top, d[nt][2 + j], acc[nt][i][1][j]);
+          acc[nt][i][0][j] = fmaf(w_top, NJ == 2 ? d[nt][j] : d[nt][0] + d[nt][1], acc[nt][i][0][j]);
+          acc[nt][i][1][j] = fmaf(w_top, NJ == 2 ? d[nt][2 + j] : d[nt][2] + d[nt][3], acc[nt][i][1][j]);
         }
     }
   }

@@ -125,7 +125,11 @@ class ProjectedBankCache:
         scaled by the chapters' weights ([B, n] ids and weights: a router's joint list).  ``counts`` [B] int32: how many entries of
         each list count (what lies behind them is not read; none: zeros, lse -inf).  Returns [B, n_q, H*64] bf16, with
         ``return_lse`` also the natural log of the softmax's denominator [B, n_q, H] fp32.  A chapter id outside the cache raises the
-        device status and is left out.  For generation: no gradients."""
+        device status and is left out.  For generation: no gradients.
+
+        Scores, softmax and sums are fp32 over either cache.  Over an 8-bit one, queries and probabilities go into the products as fp16
+        numbers and what those leave of them: exact queries but for elements below 2^-31 of a head's largest, probabilities to 2^-21 of
+        their own and 2^-32 of the largest among 32 neighbouring rows (times their scales)."""
         heads, kv_heads = int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads)
         L.require_cuda(q, chapter_indices, chapter_weights, counts)
         if q.dtype != torch.bfloat16 or q.dim() != 3:
