@@ -496,11 +496,11 @@ typedef struct {
   void *stream, *side_stream;
   int32_t hidden_dim;      /* width of hidden; 0: that of the routing states */
   int32_t launches;        /* written by the call: the kernels it launched */
-  const float* kv_scale;   /* kv_bank is held in 8 bits (moc_quantize_rows), in blocks of scale_rows; NULL: bf16 */
-  int32_t scale_rows;
 } moc_decode_step_desc;
 int64_t moc_decode_step_arena_bytes(const moc_decode_step_desc* s);
 int moc_decode_step(moc_decode_step_desc* s);
+/* The same over a kv_bank held in 8 bits (moc_quantize_rows) with its scales, in blocks of scale_rows; kv_scale NULL: bf16. */
+int moc_decode_step_cache(moc_decode_step_desc* s, const float* kv_scale, int32_t scale_rows);
 
 /* Token-routed memory attention with per-token chapter weights, projections included, in one call per pass (bf16 arithmetic,
  * head_dim 64, 64-row chapters): h [rows, hidden_dim], shared [shared_rows, hidden_dim] (shared_rows 0: none), routed

@@ -89,7 +89,7 @@ class DecodeStepDesc(C.Structure):
     _fields_ = [("router", RouterShape), ("attn", DecodeShape)] + _fields(
         "i: hidden_dtype out_dim; l: bank_rows;"
         "p: routing_states hidden router_w router_b wq wo kv_bank idx weights comb_idx comb_w out arena status stream"
-        " side_stream; i: hidden_dim launches; p: kv_scale; i: scale_rows")
+        " side_stream; i: hidden_dim launches")
 
 
 class SelectShape(C.Structure):
@@ -240,6 +240,7 @@ _PROTOTYPES = {
     "moc_roll_window": (C.c_int, [P, C.c_int64, C.c_int32, P, C.c_int64, C.c_int32, P, C.c_int32, C.c_int32, C.c_int32, P]),
     "moc_decode_step_arena_bytes": (C.c_int64, [C.POINTER(DecodeStepDesc)]),
     "moc_decode_step": (C.c_int, [C.POINTER(DecodeStepDesc)]),
+    "moc_decode_step_cache": (C.c_int, [C.POINTER(DecodeStepDesc), P, C.c_int32]),
     "moc_norm_bwd_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "moc_norm_fwd": (C.c_int, [P, P, P, C.c_int32, C.c_float, C.c_int64, C.c_int32, P, P, P, P]),
     "moc_norm_bwd": (C.c_int, [P, P, P, P, P, C.c_int32, C.c_int64, C.c_int32, P, P, P, P, P]),

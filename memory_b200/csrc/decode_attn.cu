@@ -329,7 +329,9 @@ extern "C" int64_t moc_decode_step_arena_bytes(const moc_decode_step_desc* s) {
   return s ? carve(s, &a) : -1;
 }
 
-extern "C" int moc_decode_step(moc_decode_step_desc* s) {
+extern "C" int moc_decode_step(moc_decode_step_desc* s) { return moc_decode_step_cache(s, nullptr, 0); }
+
+extern "C" int moc_decode_step_cache(moc_decode_step_desc* s, const float* kv_scale, int32_t scale_rows) {
   MOC_REQUIRE(s && s->routing_states && s->hidden && s->router_w && s->wq && s->wo && s->kv_bank && s->out && s->arena &&
               s->status, "NULL decode-step buffer");
   MOC_REQUIRE(s->attn.head_dim == kDD, "decode attention needs head_dim 64");
@@ -361,7 +363,7 @@ extern "C" int moc_decode_step(moc_decode_step_desc* s) {
   }
   if (!few) MOC_TRY(route_fwd_impl(r, nullptr, &run));
   MOC_TRY(join.done());
-  MOC_TRY(moc_decode_attn_cache(&s->attn, a.q, s->kv_bank, s->kv_scale, s->scale_rows, s->bank_rows, s->comb_idx, s->comb_w, nullptr, a.o,
+  MOC_TRY(moc_decode_attn_cache(&s->attn, a.q, s->kv_bank, kv_scale, scale_rows, s->bank_rows, s->comb_idx, s->comb_w, nullptr, a.o,
                                 nullptr, s->status, s->stream));
   Gemm go(MOC_BF16, rows, s->out_dim, width, true, true, s->hidden_dtype);
   MOC_TRY(moc_gemm(&go, a.o, s->wo, s->out, nullptr, nullptr, s->status, s->stream));

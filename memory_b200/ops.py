@@ -1496,7 +1496,7 @@ def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: to
             L.RouterShape(b, window, rd, c, top_k, num_shared, routed_scale, L.dtype_code(states.dtype)),
             L.DecodeShape(b, n_q, num_heads, num_kv_heads, head_dim, num_shared + k, tokens_per_chapter, scale),
             L.dtype_code(h.dtype), wo.shape[0], kv_bank.shape[0], None, None, p(w), p(bias), p(wq), p(wo), p(kv_bank), None,
-            None, None, None, None, None, p(L.status_word(dev)), stream, _side_stream(L.device_index(dev), stream), d, 0, p(kv_scale), scale_rows)
+            None, None, None, None, None, p(L.status_word(dev)), stream, _side_stream(L.device_index(dev), stream), d)
         plan = bytes(s), _size("moc_decode_step_arena_bytes", s), (b, k), (b, num_shared + k), (b, n_q, wo.shape[0])
         if plans is not None:
             if len(plans) >= _DECODE_PLANS_MAX:
@@ -1513,8 +1513,9 @@ def decode_step(hidden: torch.Tensor, routing_states: torch.Tensor, router_w: to
     s = L.DecodeStepDesc.from_buffer_copy(image)
     s.routing_states, s.hidden, s.out, s.arena = states.data_ptr(), h.data_ptr(), out.data_ptr(), arena.data_ptr()
     s.idx, s.weights, s.comb_idx, s.comb_w = idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(), comb_w.data_ptr()
-    rc = (L.lib().moc_decode_step(C.byref(s)) if TIMER is None
-          else _timed("decode_step", lambda: L.lib().moc_decode_step(C.byref(s))))
+    call = (lambda: L.lib().moc_decode_step(C.byref(s))) if kv_scale is None else (
+        lambda: L.lib().moc_decode_step_cache(C.byref(s), kv_scale.data_ptr(), scale_rows))
+    rc = call() if TIMER is None else _timed("decode_step", call)
     if rc:
         L.check(rc, "moc_decode_step")
     _report(s.launches, lambda: ("router_fwd:" + _TAG_OF_CODE[s.router.h_dtype], "gemm:bf16",
