@@ -186,8 +186,8 @@ int moc_token_route_bwd(const moc_token_route_desc* s, const float* g_weights, c
  * order of exact arithmetic.  weights = s of the chosen, divided by max(their sum, 1e-12) with renormalize.  A logit at or below
  * -3.3895e38 (the lowest finite bfloat16; -inf too) is masked: chosen after all others, lowest id first, with weight 0.
  * idx [rows, top_k] int64, weights [rows, top_k]; joint list as in moc_router_fwd: comb_idx / comb_w [rows, num_shared + top_k];
- * row_stats [rows, 4] (16-byte aligned; NULL: no backward pass) goes to the backward pass; load [num_chapters] int32 (NULL: not wanted) = rows that chose
- * each chapter.  Limits: 16384 chapters to choose from, top_k 128, 64 groups of equal size, top_k <= chapters of top_groups groups. */
+ * row_stats [rows, 4] (16-byte aligned; NULL: no backward pass) goes to the backward pass; load [num_chapters] int32 (NULL: not wanted) = rows that list
+ * each chapter, places that were filled up for want of candidates among them.  Limits: 16384 chapters to choose from, top_k 128, 64 groups of equal size, top_k <= chapters of top_groups groups. */
 #define MOC_SCORE_SOFTMAX 0
 #define MOC_SCORE_SIGMOID 1
 typedef struct {
@@ -199,6 +199,9 @@ typedef struct {
 } moc_select_shape;
 int moc_select_fwd(const moc_select_shape* s, const void* logits, const float* balance_bias, int64_t* idx, float* weights,
                    int32_t* comb_idx, float* comb_w, float* row_stats, int32_t* load, void* stream);
+/* load [num_chapters] int32 = how often each chapter stands in idx (n ids of moc_select_fwd; others are not checked) with a weight
+ * other than 0 (weights NULL: at all). */
+int moc_select_load(const int64_t* idx, const float* weights, int64_t n, int32_t num_chapters, int32_t* load, void* stream);
 /* d_logits [rows, num_chapters] (dense, written whole) from the gradients of weights and comb_w (either may be NULL). */
 int moc_select_bwd(const moc_select_shape* s, const void* logits, const int64_t* idx, const float* weights, const float* comb_w,
                    const float* row_stats, const float* g_weights, const float* g_comb, void* d_logits, void* stream);

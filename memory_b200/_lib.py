@@ -221,6 +221,7 @@ _PROTOTYPES = {
     "moc_grad_clip": (C.c_int, [C.c_int32, C.c_int32] + [P] * 8 + [C.c_double, C.c_double, P, P, C.c_int64, P]),
     "moc_select_fwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
     "moc_select_bwd": (C.c_int, [C.POINTER(SelectShape)] + [P] * 9),
+    "moc_select_load": (C.c_int, [P, P, C.c_int64, C.c_int32, P, P]),
     "moc_balance_bias_step": (C.c_int, [P, P, C.c_int32, C.c_int32, C.c_float, P]),
     "moc_gated_residual_fwd": (C.c_int, [C.POINTER(ResidualShape)] + [P] * 11),
     "moc_gated_residual_bwd_scratch_bytes": (C.c_int64, [C.POINTER(ResidualShape), C.c_int32]),

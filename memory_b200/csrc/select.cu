@@ -1376,18 +1376,21 @@ select_bwd_kernel(const SelectGrads p) {
     }
 }
 
-// load[c] = how many of the `n` picks are c, by one cluster of kLoadCtas CTAs: each counts its share in shared memory, then adds up
+// load[c] = how many of the `n` picks are c (with `weights`: of those whose weight is not 0), by one cluster of kLoadCtas CTAs: each counts its share in shared memory, then adds up
 // a share of the chapters over all of them.  (Counted by the selecting CTAs with atomics in global memory, 65,536 picks among 64
 // chapters took 30 us: the counters share two cache lines.)
 constexpr int kLoadCtas = 8;
 __global__ void __launch_bounds__(1024)
-select_load_kernel(const long long* __restrict__ idx, long long n, int C, int* __restrict__ load) {
+select_load_kernel(const long long* __restrict__ idx, const float* __restrict__ weights, long long n, int C, int* __restrict__ load) {
   extern __shared__ int counts[];          // [C]
   const int rank = blockIdx.x;
   for (int c = threadIdx.x; c < C; c += 1024) counts[c] = 0;
   __syncthreads();
 #pragma unroll 4
-  for (long long i = rank * 1024 + threadIdx.x; i < n; i += kLoadCtas * 1024) atomicAdd(counts + static_cast<int>(idx[i]), 1);
+  for (long long i = rank * 1024 + threadIdx.x; i < n; i += kLoadCtas * 1024) {
+    if (weights != nullptr && weights[i] == 0.f) continue;
+    atomicAdd(counts + static_cast<int>(idx[i]), 1);
+  }
   cluster_sync();
   const uint32_t base = smem_u32(counts);
   for (int c = rank * 1024 + threadIdx.x; c < C; c += kLoadCtas * 1024) {
@@ -1468,6 +1471,12 @@ template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream
   MOC_CUDA_OK(cudaGetLastError());
   return MOC_OK;
 }
+int select_load(const long long* idx, const float* weights, long long n, int C, int* load, cudaStream_t stream) {
+  const size_t bytes = static_cast<size_t>(C) * sizeof(int32_t);
+  if (bytes > 48 * 1024) MOC_CUDA_OK(allow_shared(select_load_kernel, bytes, kSharedMost));
+  MOC_CUDA_OK(launch_clustered(select_load_kernel, dim3(kLoadCtas), 1024, static_cast<int>(bytes), kLoadCtas, stream, idx, weights, n, C, load));
+  return MOC_OK;
+}
 template <typename LT> int select_bwd(const SelectGrads& p, cudaStream_t stream) {
   // a warp a row up to 512 chapters, a CTA beyond
   if (p.C <= 512) select_bwd_kernel<LT, 32><<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, 0, stream>>>(p);
@@ -1499,11 +1508,13 @@ extern "C" int moc_select_fwd(const moc_select_shape* s, const void* logits, con
   p.count_here = load != nullptr && p.rows <= (warps ? kWarpRows : 1);
   const int done = s->dtype == MOC_F32 ? select_fwd<float>(p, stream) : select_fwd<__nv_bfloat16>(p, stream);
   if (done != MOC_OK || load == nullptr || p.count_here) return done;
-  const size_t bytes = static_cast<size_t>(s->num_chapters) * sizeof(int32_t);
-  if (bytes > 48 * 1024) MOC_CUDA_OK(allow_shared(select_load_kernel, bytes, kSharedMost));
-  MOC_CUDA_OK(launch_clustered(select_load_kernel, dim3(kLoadCtas), 1024, static_cast<int>(bytes), kLoadCtas, stream,
-                               static_cast<const long long*>(p.idx), static_cast<long long>(p.rows) * p.k, s->num_chapters, load));
-  return MOC_OK;
+  return select_load(p.idx, nullptr, static_cast<long long>(p.rows) * p.k, s->num_chapters, load, stream);
+}
+
+extern "C" int moc_select_load(const int64_t* idx, const float* weights, int64_t n, int32_t num_chapters, int32_t* load, void* stream) {
+  MOC_REQUIRE(idx && load, "NULL selection buffer");
+  MOC_REQUIRE(n >= 0 && num_chapters > 0 && num_chapters <= 2 * kMostN, "a count of chosen chapters takes 1..32768 chapters");
+  return select_load(reinterpret_cast<const long long*>(idx), weights, n, num_chapters, load, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int moc_select_bwd(const moc_select_shape* s, const void* logits, const int64_t* idx, const float* weights,

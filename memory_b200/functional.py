@@ -936,7 +936,7 @@ def token_routed_attention_joint(h, shared_memory, routed_memory, token_chapter_
 # --------------------------------------------------------------------------------------------
 class ChapterSelection(NamedTuple):
     """What :func:`select_chapters` returns: for every row the chosen ids (int64) and weights, the joint list with the shared
-    chapters in front (int32 ids and weights, as ``memory_layer`` and the decoder take them), and how many rows chose each
+    chapters in front (int32 ids and weights, as ``memory_layer`` and the decoder take them), and how many rows list each
     chapter (int32 [C])."""
     indices: torch.Tensor
     weights: torch.Tensor
@@ -958,9 +958,9 @@ def _differentiated(*tensors) -> bool:
 
 class _Select(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, s):
+    def forward(ctx, logits, bias, s, count_filled):
         ctx.set_materialize_grads(False)
-        idx, w, cidx, cw, load, stats = ops.select_fwd(logits, bias, s, True)
+        idx, w, cidx, cw, load, stats = ops.select_fwd(logits, bias, s, True, count_filled)
         ctx.s = s
         ctx.save_for_backward(logits, idx, w, cw, stats)
         ctx.mark_non_differentiable(idx, cidx, load)
@@ -970,11 +970,11 @@ class _Select(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, _idx, g_w, _cidx, g_cw, _load):
         if g_w is None and g_cw is None:
-            return None, None, None
+            return None, None, None, None
         logits, idx, w, cw, stats = ctx.saved_tensors
         g_w = None if g_w is None else ops._contig(g_w.float())
         g_cw = None if g_cw is None else ops._contig(g_cw.float())
-        return ops.select_bwd(logits, ctx.s, idx, w, cw, stats, g_w, g_cw), None, None
+        return ops.select_bwd(logits, ctx.s, idx, w, cw, stats, g_w, g_cw), None, None, None
 
 
 _MOST_SELECTED, _MOST_ROUTED, _MOST_GROUPS = 128, 16384, 64
@@ -1010,7 +1010,7 @@ def _select_image(chapters: int, top_k: int, score: str, num_shared: int, routed
 
 def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax", balance_bias: Optional[torch.Tensor] = None,
                     num_shared: int = 0, routed_scale: float = 1.0, num_groups: int = 1, top_groups: Optional[int] = None,
-                    group_score: str = "max", renormalize: bool = True) -> ChapterSelection:
+                    group_score: str = "max", renormalize: bool = True, count_filled: bool = True) -> ChapterSelection:
     """Top-k chapters of every row of ``logits`` [..., C] (fp32 or bf16), by rules beyond the reference router's.
 
     The first ``num_shared`` chapters are not chosen from; the others score ``softmax`` or ``sigmoid`` of their logits.
@@ -1021,7 +1021,9 @@ def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     the others by ``routed_scale`` and divides by the sum.
 
     A logit at or below -3.3895e38 (the lowest bfloat16; -inf too) masks its chapter: it comes after all others, lowest id first, with
-    weight 0, so a row that is masked as a whole gets the first ids and zero weights.  A NaN makes its row's weights NaN (softmax)
+    weight 0, so a row that is masked as a whole gets the first ids and zero weights.  ``load`` counts such places as well;
+    ``count_filled=False`` leaves out those of weight 0, which is what a balance bias should follow (padded rows would push the first
+    chapters down).  A NaN makes its row's weights NaN (softmax)
     or its own (sigmoid) and comes first.  Differentiable in ``logits`` through both weights."""
     if logits.dim() < 2:
         raise ValueError(f"logits must be [..., num_chapters], got shape {tuple(logits.shape)}")
@@ -1045,9 +1047,9 @@ def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
                 z.new_empty(0, joint, dtype=torch.int32), z.new_empty(0, joint, dtype=torch.float32),
                 torch.zeros(c, dtype=torch.int32, device=z.device))
     elif _differentiated(z):
-        flat = _Select.apply(z, balance_bias, s)
+        flat = _Select.apply(z, balance_bias, s, count_filled)
     else:
-        flat = ops.select_fwd(z, balance_bias, s, False)[:5]
+        flat = ops.select_fwd(z, balance_bias, s, False, count_filled)[:5]
     if logits.dim() == 2:
         return ChapterSelection(*flat)
     lead = logits.shape[:-1]

@@ -304,9 +304,10 @@ def agree_probe(device, late_warps: int, poll_limit: int):
 SCORES = {"softmax": 0, "sigmoid": 1}
 
 
-def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, want_stats: bool):
+def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, want_stats: bool, count_filled: bool = True):
     """``moc_select_fwd`` on logits [rows, C] (fp32 or bf16, unit column stride); ``s``: the filled ``SelectShape``.  Returns (idx
-    int64, weights, joint idx int32, joint weights, load, row stats or None)."""
+    int64, weights, joint idx int32, joint weights, load, row stats or None).  ``count_filled`` False: places of weight 0 do not count
+    in the load."""
     dev, rows, k, joint = logits.device, s.rows, s.top_k, s.num_shared + s.top_k
     f32, i32 = torch.float32, torch.int32
     idx = torch.empty((rows, k), dtype=torch.int64, device=dev)
@@ -316,9 +317,11 @@ def select_fwd(logits: torch.Tensor, balance_bias: Optional[torch.Tensor], s, wa
     load = torch.empty(s.num_chapters, dtype=i32, device=dev)
     stats = torch.empty((rows, 4), dtype=f32, device=dev) if want_stats else None
     alone = 4 if s.num_chapters - s.num_shared <= 512 and k <= 31 else 1          # rows of one CTA, which counts its own picks
-    _issue("select_fwd", _DTYPE_TAG[logits.dtype], 2 if rows > alone else 1, dev,
+    _issue("select_fwd", _DTYPE_TAG[logits.dtype], 2 if count_filled and rows > alone else 1, dev,
            (C.byref(s), logits.data_ptr(), L.ptr(balance_bias), idx.data_ptr(), weights.data_ptr(), comb_idx.data_ptr(), comb_w.data_ptr(),
-            L.ptr(stats), load.data_ptr()))
+            L.ptr(stats), load.data_ptr() if count_filled else None))
+    if not count_filled:
+        _issue("select_load", "f32", 1, dev, (idx.data_ptr(), weights.data_ptr(), rows * k, s.num_chapters, load.data_ptr()))
     return idx, weights, comb_idx, comb_w, load, stats
 
 

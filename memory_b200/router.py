@@ -21,7 +21,8 @@ class ChapterRouter(nn.Module):
     Beyond the reference: ``score="sigmoid"``, ``balance_bias=True`` (a buffer that :meth:`update_balance` moves towards equal
     load; it counts in the selection alone), ``num_groups`` / ``top_groups`` / ``group_score`` (group-limited selection over the chapters
     behind the excluded prefix) and ``renormalize=False`` select by :func:`memory_b200.select_chapters`.  Such a router returns no loss terms (an empty
-    dict): the bias takes the place of the balance loss.  ``last_load`` holds the latest call's count of rows per chapter.
+    dict): the bias takes the place of the balance loss.  ``last_load`` holds the latest call's count of rows per chapter
+    (rows that give it a weight).
     """
 
     def __init__(self, hidden_dim: int, num_chapters: int, top_k: int = 1, routing_strategy: str = "sequence", *,
@@ -55,16 +56,17 @@ class ChapterRouter(nn.Module):
         self.register_buffer("balance_bias", torch.zeros(num_chapters) if balance_bias else None)
 
     def select(self, logits: torch.Tensor, num_shared: int, routed_scale: float = 1.0) -> F_moc.ChapterSelection:
-        """This router's selection from logits [rows, num_chapters]."""
+        """This router's selection from logits [rows, num_chapters].  Rows and chapters may be masked; places of weight 0 do not count in
+        the load, so padding does not move the balance bias."""
         got = F_moc.select_chapters(logits, self.top_k, balance_bias=self.balance_bias, num_shared=num_shared,
-                                    routed_scale=routed_scale, **self.selection)
+                                    routed_scale=routed_scale, count_filled=False, **self.selection)
         self.last_load, self._last_shared = got.load, num_shared
         return got
 
     def update_balance(self, rate: float = 1e-3, load: Optional[torch.Tensor] = None,
                        num_shared: Optional[int] = None) -> None:
         """Moves the balance bias of every chapter behind the shared ones by ``rate`` towards the mean load: up where fewer rows
-        chose it, down where more did.  ``load`` [C] int32: the counts of a step (summed over ranks, say); they and ``num_shared`` are
+        chose it, down where more did (and up at every step where a mask keeps all rows away).  ``load`` [C] int32: the counts of a step (summed over ranks, say); they and ``num_shared`` are
         the latest call's by default."""
         if self.balance_bias is None:
             raise ValueError("this router has no balance bias")
