@@ -23,7 +23,8 @@ class SparseBankAdamW:
     """AdamW for one bank parameter ([rows, d] fp32) driven by compact gradients.
 
     ``step(grad)`` takes the ``SparseBankGrad`` a backward pass (or ``GradReducer``) filled; its ``scale`` and the
-    optional ``grad_scale`` (a number, or the coefficient ``clip_grad_norm_`` left on the device) multiply the gradient.  ``state_dict`` / ``load_state_dict``
+    optional ``grad_scale`` (a number, or a tensor of one: the coefficient ``clip_grad_norm_`` left on the device, or one formed by hand, in
+    any type and on any device) multiply the gradient.  ``state_dict`` / ``load_state_dict``
     use torch.optim.AdamW's per-parameter keys (``step``, ``exp_avg``, ``exp_avg_sq``), so optimizer state moves
     between the two."""
 
@@ -52,8 +53,8 @@ class SparseBankAdamW:
         if t != self.t:
             raise ValueError("gradient rows were produced with a different chapter size")
         on_device = torch.is_tensor(grad_scale) and grad_scale.is_cuda
-        if on_device and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.device != self.param.device):
-            raise TypeError("a gradient scale on the device must be one fp32 number beside the parameter")
+        if on_device:
+            grad_scale = _device_scale(grad_scale, self.param.device)
         self.step_count += 1
         if self._ws is None:
             self._ws = torch.empty(4 * (self.param.shape[0] // self.t), dtype=torch.uint8, device=self.param.device)
@@ -76,6 +77,13 @@ class SparseBankAdamW:
         self.step_count = int(state["step"])
         self.exp_avg.copy_(state["exp_avg"])
         self.exp_avg_sq.copy_(state["exp_avg_sq"])
+
+
+def _device_scale(scale: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """One number of any type on a GPU as fp32 on ``device``, without a host round trip."""
+    if scale.numel() != 1 or scale.is_complex() or (scale.dim() > 0 and scale.dtype == torch.float64):
+        raise TypeError("a gradient scale on the device must be one number: a 0-d tensor, or one element of at most 32 bits")
+    return scale.detach().to(device=device, dtype=torch.float32)
 
 
 class GradClip(NamedTuple):
