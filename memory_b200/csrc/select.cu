@@ -110,11 +110,18 @@ __device__ __forceinline__ float fast_sigmoid(float z) {
 }
 
 // How far fast keys can be off.  Sigmoid: the exponential is off by 2 + 1.2 |z| ulp, which the slope s (1 - s) <= 1/4 brings
-// below 4e-8, the sum and the reciprocal by another 3 ulp of at most 1: 2.5e-7.  Softmax: 2 ulp of the exponential, |z - m| 2^-24 e^-|z - m| of its
-// argument, 2e-6 of the sum (terms off by up to 25 ulp each), all against the largest score 1 / total.  The bias's addition: half
-// an ulp of the key.  A sum of two keys adds theirs.
+// below 4e-8, the sum and the reciprocal by another 3 ulp of at most 1: 2.5e-7.
+// Softmax, in units u = 2^-24 of the largest score 1 / total.  The sum of the exponentials: 4 u of a term's exponential (2 ulp); |z - m| u of its
+// argument, which averages over the terms by their size: n terms of e^-x against one of 1 make x n e^-x / (1 + n e^-x), 6.8 u at most for
+// n = 16,384, 8 u where m is rounded up to a whole number; additions one after another, 16 of a thread's, 5 across a warp, 5 across
+// warps.  That is 38 u where a thread has its logits in registers.  Streaming, a lane's sum moves to a larger reference with a factor
+// of 4 u each time; references are whole numbers, so what has moved j times is e^(1-j) of the sum or less: the average of j over the 512
+// terms of a lane is below 4.7, 19 u; 4 u more across lanes and 6.5 u back to the largest logit, but 5 u of additions alone (16 terms
+// by a tree, the rest in 64 bits): 46.5 u = 2.8e-6.  The key's own exponential, argument, quotient and product: 6.5 u, together 3.2e-6.
+// The bias's addition: half an ulp of the key.  A sum of two keys adds theirs.
+constexpr float kSumError = 3.0e-6f, kKeyError = 3.5e-6f;
 __device__ __forceinline__ float key_error(const SelectParams& p, float v, float inv_total) {
-  return (p.sigmoid ? 3e-7f : 3e-6f * inv_total) + 6.1e-8f * fabsf(v);
+  return (p.sigmoid ? 3e-7f : kKeyError * inv_total) + 6.1e-8f * fabsf(v);
 }
 // whether a > b for certain (NaN: no)
 __device__ __forceinline__ bool apart(const SelectParams& p, float a, float b, float inv_total) {
@@ -196,12 +203,12 @@ template <typename LT> __device__ __noinline__ uint64_t key64(const SelectParams
 }
 
 // Candidates ranked by 64-bit keys: whether a, the next above b, is before it for certain.  Softmax keys may have been formed with
-// the fp32 sum of the exponentials, off by 2e-6 at most: it scales the difference of the scores, not that of the biases.
+// the fp32 sum of the exponentials, off by kSumError at most: it scales the difference of the scores, not that of the biases.
 __device__ __forceinline__ bool apart64(const SelectParams& p, uint64_t a, int ia, uint64_t b, int ib) {
   if (p.sigmoid || a == b) return p.sigmoid || p.bias[p.S + ia] == p.bias[p.S + ib];
   const double sa = of_key(a), sb = of_key(b);
   const double da = sa - static_cast<double>(p.bias[p.S + ia]), db = sb - static_cast<double>(p.bias[p.S + ib]);
-  return sa - sb > 2.2e-6 * fabs(da - db);
+  return sa - sb > kSumError * (1 + kSumError) * fabs(da - db);
 }
 // Whether fp32 values tell the groups that stay (least of them) from those that go: two keys each, or bare logits.  (Groups without a
 // candidate are behind all others, in the order of their ids.)
@@ -709,24 +716,31 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
   }
 
   float m = 0.f, total = 1.f, inv_total = 1.f;
-  if (!SIG) {                                          // maximum and sum, a lane's own until the end
+  if (!SIG) {                                          // maximum and sum against it, rounded up to a whole number; a lane's own until the end
     m = -INFINITY;
-    total = 0.f;
+    float ref = -INFINITY;
+    double sums = 0.0;
     for (int c0 = lane; c0 < p.N; c0 += 32 * kBatch) {
       float z[kBatch], most = m;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) z[i] = c0 + 32 * i < p.N ? logit_of(zr, c0 + 32 * i) : -INFINITY;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) most = fmaxf(most, masked(z[i]) ? -INFINITY : z[i]);
-      float sum = 0.f;
+      const float up = ceilf(most);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) sum += masked(z[i]) ? 0.f : expf(z[i] - most);
-      total = (m == -INFINITY ? total : total * expf(m - most)) + sum;
+      for (int i = 0; i < kBatch; ++i) z[i] = masked(z[i]) ? 0.f : expf(z[i] - up);
+#pragma unroll
+      for (int n = kBatch / 2; n > 0; n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) z[i] += z[i + n];
+      sums = (ref == up || ref == -INFINITY ? sums : sums * static_cast<double>(expf(ref - up))) + static_cast<double>(z[0]);
       m = most;
+      ref = up;
     }
-    const float all = of_key(__reduce_max_sync(0xffffffffu, to_key(m)));
-    total = warp_total(m == -INFINITY ? total : total * expf(m - all));        // (a lane with NaN alone keeps its NaN)
-    m = all;
+    m = of_key(__reduce_max_sync(0xffffffffu, to_key(m)));
+    const float up = ceilf(m);
+    sums = warp_total(ref == up || ref == -INFINITY ? sums : sums * static_cast<double>(expf(ref - up)));        // (a lane with NaN alone keeps its NaN)
+    total = static_cast<float>(m == -INFINITY ? sums : sums * static_cast<double>(expf(up - m)));
     if (total == 0.f) total = 1.f;                     // (every logit masked)
     inv_total = 1.f / total;
   }
@@ -978,9 +992,7 @@ template <typename K, int TH> __device__ __forceinline__ K cta_total(K v, K* red
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  K t = K(0);
-  for (int w = 0; w < TH / 32; ++w) t += red[w];
-  return t;
+  return warp_total((threadIdx.x & 31) < TH / 32 ? red[threadIdx.x & 31] : K(0));
 }
 struct CtaShared {
   unsigned long long cand[kSelCand];       // key, then the id's complement: larger is earlier
