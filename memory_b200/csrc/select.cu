@@ -10,14 +10,18 @@
 //
 // The order is that of exact arithmetic.  With a bias, or sums of two, fp32 keys carry errors of the exponential and the
 // quotient; where neighbours in the order are closer than those errors allow (a row in some hundreds), the few candidates
-// concerned are ranked again by 64-bit keys.  Rows that this does not settle (groups that close, NaN, fewer candidates than
-// places) run through the same selection in 64 bits as a whole.  Bare logits need no arithmetic and are always sure.
+// concerned are ranked again by 64-bit keys.  Rows that this does not settle (NaN, more keys that are equal or infinite than the lists
+// hold) run through the same selection in 64 bits as a whole.  Bare logits need no arithmetic and are always sure.
 //
 // Bound by HBM for many rows (4 bytes a logit read) by right, by issuing in fact, and by latency for a few.  Up to 512 candidates and
 // k < 32 a warp has a row in registers (257 chapters, k = 8, sigmoid, bias, groups: 1 row 8 us, 1,000 rows 12, 8,192 rows 31; by a CTA
 // a row 10, 27 and 107; 513 chapters, k = 31, softmax, bias: 12, 18.5 and 105 against 10, 29 and 119), beyond that a CTA, or a warp
 // that streams it where there are many.  Either way the k + 1 largest lie among the values above a bound that at least k + 1 of
-// the threads' own maxima reach, found by bisection; what lies above it is ranked.
+// the threads' own maxima reach, found by bisection; what lies above it is ranked.  (Where fewer threads have a candidate, or fewer
+// candidates are there than k + 1, all of them are: 8,192 rows of 64 chapters in 8 groups, 2 kept, k = 16: 29 us; in 64 bits 124.)
+#include <algorithm>
+#include <cfloat>
+
 #include "moc_common.cuh"
 
 namespace moc {
@@ -41,6 +45,7 @@ struct SelectParams {
   int* load;                      // [C] or NULL
   long long ld;
   int rows, N, S, k, groups, keep, per;
+  int need;                       // values that a bound has to leave: k + 1, or all there can be (of the groups that stay)
   FastDiv per_group;
   int sigmoid, top2, renorm;
   int count_here;                 // the launch is one CTA, which counts as well (`load` from zero)
@@ -288,6 +293,21 @@ __device__ __noinline__ uint64_t group_value64(const SelectParams& p, const LT* 
   }
   return group_value(p, t);
 }
+// Places n .. k - 1 of a row that has n < k candidates (their ids in place[0 .. n)), by one warp: the lowest other ids, complemented.
+// They lie below k, as at most n of those are candidates.
+__device__ __forceinline__ void fill_up(int* place, int n, int k) {
+  const int lane = threadIdx.x & 31;
+  for (int id0 = 0, at = n; at < k; id0 += 32) {
+    const int id = id0 + lane;
+    bool free = id < k;
+    for (int j = 0; j < n; ++j) free &= place[j] != id;
+    const uint32_t votes = __ballot_sync(0xffffffffu, free);
+    const int pos = at + __popc(votes & ((1u << lane) - 1u));
+    if (free && pos < k) place[pos] = ~id;
+    at += __popc(votes);
+  }
+  __syncwarp();
+}
 // Which groups stay, where fp32 values (of groups lane and lane + 32) close at the border between `least` and `most`: those near it
 // again in 64 bits.  The others are ahead of, or behind, all of them in any case.
 template <typename LT>
@@ -526,30 +546,41 @@ select_warp_kernel(const SelectParams p) {
   const uint32_t mine = to_key(best), none = 0x007FFFFFu;          // (the key of -inf)
   uint32_t hi = __reduce_max_sync(0xffffffffu, mine);
   const int some = __popc(__ballot_sync(0xffffffffu, mine > none));
-  const int need = min(p.k + 1, p.N);
+  int need = p.need;
   if (some == 0) {                                           // nothing to choose from: the lowest ids
     pick = lane;
-  } else if (hi == 0xFFFFFFFFu || some < need) {             // NaN, or candidates in too few lanes
+  } else if (hi == 0xFFFFFFFFu) {                            // NaN
     sure = false;
   } else if (sure) {
-    // count(lanes >= lo) >= need, count(> hi) == 0
-    uint32_t lo = __reduce_min_sync(0xffffffffu, mine > none ? mine : 0xFFFFFFFFu);
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      const int n = __popc(__ballot_sync(0xffffffffu, mine >= mid));
-      if (n >= need) {
-        lo = mid;
-        if (n <= need + 2) break;
-      } else {
-        hi = mid - 1;
+    uint32_t lo;
+    if (some >= need) {
+      // count(lanes >= lo) >= need, count(> hi) == 0
+      lo = __reduce_min_sync(0xffffffffu, mine > none ? mine : 0xFFFFFFFFu);
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        const int n = __popc(__ballot_sync(0xffffffffu, mine >= mid));
+        if (n >= need) {
+          lo = mid;
+          if (n <= need + 2) break;
+        } else {
+          hi = mid - 1;
+        }
       }
+    } else {                                                 // candidates in few lanes (few groups, masks): all of them to begin with
+      float least = INFINITY;
+      int count = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (v[i] > -INFINITY) { least = fminf(least, v[i]); ++count; }
+      lo = __reduce_min_sync(0xffffffffu, to_key(least));
+      need = min(need, __reduce_add_sync(0xffffffffu, count));
     }
     hi = 0xFF7FFFFFu;                                        // (the largest finite number's key)
     float edge;
     int n;
     while (true) {
       edge = of_key(lo);
-      if (p.bias != nullptr) edge -= 2.f * key_error(p, edge, inv_total);        // what may yet turn out to reach the bound
+      if (p.bias != nullptr) edge = fmaxf(edge - 2.f * key_error(p, edge, inv_total), -FLT_MAX);        // what may yet turn out to reach the bound
       int count = 0;
 #pragma unroll
       for (int i = 0; i < NV; ++i) count += v[i] >= edge;
@@ -626,10 +657,12 @@ select_warp_kernel(const SelectParams p) {
         out[32 + rank] = __float_as_uint(logit);
       }
       __syncwarp();
-      if (lane < n) {
-        pick = out[lane];
-        chosen = __uint_as_float(out[32 + lane]);
-        ok = true;
+      if (n < p.k) fill_up(reinterpret_cast<int*>(out), n, p.k);
+      if (lane < max(n, p.k)) {
+        const int at = static_cast<int>(out[lane]);
+        ok = at >= 0;
+        pick = ok ? at : ~at;
+        chosen = ok ? __uint_as_float(out[32 + lane]) : 0.f;
       }
     }
   }
@@ -844,14 +877,15 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
   some = __reduce_add_sync(0xffffffffu, some);
   hi = __reduce_max_sync(0xffffffffu, hi);
   lo = __reduce_min_sync(0xffffffffu, lo);
-  const int need = min(p.k + 1, p.N);
+  const int need = p.need;
   int n = 0;
   if (some == 0) {                                     // nothing to choose from: the lowest ids
     for (int j = lane; j < p.k; j += 32) s.place[j] = ~j;
-  } else if (hi == 0xFFFFFFFFu || some < need) {
-    sure = false;                                      // NaN, or candidates in too few runs
+  } else if (hi == 0xFFFFFFFFu) {
+    sure = false;                                      // NaN
   } else if (sure) {
-    while (lo < hi) {                                  // count(>= lo) >= need, count(> hi) == 0
+    if (some < need) lo = 0x00800000u;                 // candidates in few runs (masks): all of them (the lowest finite number's key)
+    while (some >= need && lo < hi) {                  // count(>= lo) >= need, count(> hi) == 0
       const uint32_t mid = lo + (hi - lo + 1) / 2;
       int count = 0;
 #pragma unroll 8
@@ -865,7 +899,7 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
       }
     }
     float edge = of_key(lo);
-    if (BIAS) edge -= 2.f * key_error(p, edge, inv_total);       // what may yet turn out to reach the bound
+    if (BIAS) edge = fmaxf(edge - 2.f * key_error(p, edge, inv_total), -FLT_MAX);       // what may yet turn out to reach the bound
     const uint32_t from = to_key(edge);
     int runs = 0;
     for (int i = 0; i < chunks; ++i) {
@@ -904,7 +938,7 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
         }
       }
       __syncwarp();
-      sure = n <= kStreamCand && n >= min(need, p.k);
+      sure = n <= kStreamCand;
     }
   }
   if (sure && some > 0) {
@@ -955,6 +989,8 @@ select_stream_kernel(const SelectParams p, const int chunks, const FastDiv group
       if (BIAS) s.wide[rank] = mine;                   // in order
       if (rank < p.k) s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
     }
+    __syncwarp();
+    if (n < p.k) fill_up(s.place, n, p.k);
     bool close = false;
     if (BIAS) {
       __syncwarp();
@@ -1207,7 +1243,7 @@ select_cta_kernel(const SelectParams p) {
   for (int i = 0; i < NV; ++i) top = max_nan(top, v[i]);
   tops[threadIdx.x] = top;
   __syncthreads();
-  const int need = min(p.k + 1, p.N);
+  const int need = p.need;
   if (warp == 0) {
     uint32_t key[TH / 32], lo = 0xFFFFFFFFu, hi = 0;
     constexpr uint32_t kNone = 0x007FFFFFu;                // of -inf
@@ -1221,9 +1257,10 @@ select_cta_kernel(const SelectParams p) {
     some = __reduce_add_sync(0xffffffffu, some);
     hi = __reduce_max_sync(0xffffffffu, hi);
     lo = __reduce_min_sync(0xffffffffu, lo);
-    // NaN, or candidates in too few threads, unless there is none at all: not for this bound
-    if (hi == 0xFFFFFFFFu || (some < need && some > 0)) {
+    if (hi == 0xFFFFFFFFu) {                               // NaN
       if (lane == 0) s.unsure = 1;
+    } else if (some < need) {                              // candidates in few threads (masks): all of them (the lowest finite number's key)
+      lo = 0x00800000u;
     } else if (some > 0) {
       // count(>= lo) >= need, count(> hi) == 0
       while (lo < hi) {
@@ -1243,7 +1280,7 @@ select_cta_kernel(const SelectParams p) {
     // (with a bias: what may yet turn out to reach the bound)
     const float e = some > 0 ? of_key(lo) : INFINITY;
     if (lane == 0) {
-      s.edge = biased && some > 0 ? e - 2.f * key_error(p, e, inv_total) : e;
+      s.edge = biased && some > 0 ? fmaxf(e - 2.f * key_error(p, e, inv_total), -FLT_MAX) : e;
       if (some > 0 && !(s.edge < INFINITY)) s.unsure = 1;          // (more infinite keys than places)
     }
     if (some == 0)
@@ -1273,11 +1310,11 @@ select_cta_kernel(const SelectParams p) {
         if (biased) keys[rank] = mine;              // in order
         if (rank < p.k) s.place[rank] = static_cast<int>(~static_cast<uint32_t>(mine));
       }
-      if (biased) {
-        __syncthreads();
+      __syncthreads();
+      if (biased)
         for (int t = threadIdx.x; t < p.k && t + 1 < n; t += TH)
           if (!apart(p, of_key(static_cast<uint32_t>(keys[t] >> 32)), of_key(static_cast<uint32_t>(keys[t + 1] >> 32)), inv_total)) s.close = 1;
-      }
+      if (warp == 0 && n < p.k) fill_up(s.place, n, p.k);
       __syncthreads();
       if (s.close) {                                // the candidates again by 64-bit keys
         double t64 = total;
@@ -1465,13 +1502,18 @@ template <typename LT, int S> int select_stream(const SelectParams& p, cudaStrea
   MOC_CUDA_OK(cudaGetLastError());
   return MOC_OK;
 }
+// Runs of `size` candidates of the groups that stay, at least.  Streaming takes its bound from their maxima and needs as many as
+// values that are to reach it: 2,000 rows, one of 8 groups of 512 kept (32 runs), sigmoid, bias: k = 28 37 us against 62 by a CTA a row,
+// k = 32 (a 33rd is needed) 225 against 62; two kept (64 runs): k = 48 45 against 67, k = 64 336 against 71.
+int kept_runs(const SelectParams& p, int size) { return p.keep * 32 * ceil_div(p.per / 32, size); }
 template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream) {
   const bool grouped = p.keep < p.groups;
   if (p.N <= kWarpMostN && p.k <= kWarpMostK) {
     auto kern = p.N <= 64 ? select_warp_kernel<LT, 2> : p.N <= 128 ? select_warp_kernel<LT, 4>
                 : p.N <= 256 ? select_warp_kernel<LT, 8> : select_warp_kernel<LT, 16>;
     kern<<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, 0, stream>>>(p);
-  } else if (p.rows >= (p.k <= 32 ? kStreamRows : kStreamRowsManyPicks) && p.k <= kStreamMostK && p.N > kWarpMostN && (!grouped || p.per >= 256)) {
+  } else if (p.rows >= (p.k <= 32 ? kStreamRows : kStreamRowsManyPicks) && p.k <= kStreamMostK && p.N > kWarpMostN && (!grouped || p.per >= 256) &&
+             kept_runs(p, p.N > 2048 ? 16 : 4) >= p.need) {
     return p.N > 2048 ? select_stream<LT, 16>(p, stream) : select_stream<LT, 4>(p, stream);
   } else {
     const bool big = p.N > 4096;
@@ -1514,6 +1556,7 @@ extern "C" int moc_select_fwd(const moc_select_shape* s, const void* logits, con
   p.comb_idx = comb_idx; p.comb_w = comb_w; p.row_stats = row_stats; p.load = load; p.ld = s->ld;
   p.rows = s->rows; p.N = s->num_chapters - s->num_shared; p.S = s->num_shared; p.k = s->top_k;
   p.groups = s->num_groups; p.keep = s->top_groups; p.per = p.N / p.groups;
+  p.need = std::min(p.k + 1, p.keep * p.per);
   p.per_group = fast_div(p.per);
   p.sigmoid = s->score == MOC_SCORE_SIGMOID; p.top2 = s->group_top2 != 0; p.renorm = s->renormalize != 0; p.rho = s->routed_scale;
   const bool warps = p.N <= kWarpMostN && p.k <= kWarpMostK;
