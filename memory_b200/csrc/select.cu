@@ -1234,7 +1234,8 @@ select_cta_kernel(const SelectParams p) {
     choose_groups<TH>(p, s, sk, zr, m, inv_total);
     const float* off = reinterpret_cast<const float*>(s.group) + kMostGroups;          // 0 where the group stays, else -inf
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] += off[min(div_of(threadIdx.x + TH * i, p.per_group), kMostGroups - 1)];     // (NaN stays)
+    for (int i = 0; i < NV; ++i)
+      if (threadIdx.x + TH * i < p.N) v[i] += off[div_of(threadIdx.x + TH * i, p.per_group)];     // (NaN stays)
   }
   // A bound that at least k + 1 of the threads' own maxima reach, and few more.
   float* tops = reinterpret_cast<float*>(s.cand);          // [TH] <= kSelCand * 2
