@@ -164,28 +164,28 @@ __device__ __forceinline__ void write_row(const SelectParams& p, long long row, 
     }
   }
   mass = warp_total(mass);
-  const float over = 1.f / max_nan(mass, 1e-12f);
+  const float floor_mass = max_nan(mass, 1e-12f);          // (divided by, not multiplied with its reciprocal: one rounding)
   float sum = 0.f;
 #pragma unroll
   for (int q = 0; q < EACH; ++q) {
     const int j = lane + 32 * q;
     if (j >= p.k) break;
-    if (p.renorm) w[q] *= over;
+    if (p.renorm) w[q] /= floor_mass;
     sum += p.rho * w[q];
     p.idx[row * p.k + j] = id[q] + p.S;
     p.weights[row * p.k + j] = w[q];
   }
   sum = static_cast<float>(p.S) + warp_total(sum);
-  const float joint = 1.f / max_nan(sum, 1e-12f);
+  const float joint = max_nan(sum, 1e-12f);
   int* ci = p.comb_idx + row * (p.S + p.k);
   float* cw = p.comb_w + row * (p.S + p.k);
-  for (int j = lane; j < p.S; j += 32) { ci[j] = j; cw[j] = joint; }
+  for (int j = lane; j < p.S; j += 32) { ci[j] = j; cw[j] = 1.f / joint; }
 #pragma unroll
   for (int q = 0; q < EACH; ++q) {
     const int j = lane + 32 * q;
     if (j >= p.k) break;
     ci[p.S + j] = id[q] + p.S;
-    cw[p.S + j] = p.S > 0 ? p.rho * w[q] * joint : w[q];
+    cw[p.S + j] = p.S > 0 ? p.rho * w[q] / joint : w[q];
   }
   if (lane == 0 && p.row_stats != nullptr) reinterpret_cast<float4*>(p.row_stats)[row] = make_float4(m, total, mass, sum);
 }
