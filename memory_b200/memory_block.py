@@ -88,12 +88,19 @@ class MemorySubBlock(nn.Module):
                 a.num_heads, a.num_kv_heads, a._compute_dtype(hidden_states),
                 pre_norm="rms" if self.use_rms_norm else "layernorm", norm_weight=self.memory_layernorm.weight,
                 norm_bias=getattr(self.memory_layernorm, "bias", None), norm_eps=self.norm_eps, add_residual=False)
-            return F_moc.gated_residual_norm(
+            # states of another type than the kernels take go through fp32, as they go through the compute type in front of the block
+            dtype = hidden_states.dtype
+            if dtype not in F_moc._KERNEL_DTYPES:
+                hidden_states, branch = hidden_states.float(), branch.float()
+            got = F_moc.gated_residual_norm(
                 hidden_states, branch, self.post_norm.weight, getattr(self.post_norm, "bias", None),
                 norm_type="rms" if self.use_rms_norm else "layernorm", eps=self.norm_eps,
                 gate=self.gate if gate is None else gate, residual_scale=self.residual_scale,
                 next_weight=None if next_norm is None else next_norm.weight, next_bias=getattr(next_norm, "bias", None),
                 next_eps=None if next_norm is None else next_norm.eps)
+            if hidden_states.dtype == dtype:
+                return got
+            return got.to(dtype) if next_norm is None else (got[0].to(dtype), got[1].to(dtype))
         if gate is not None or next_norm is not None:
             raise ValueError("gate and next_norm go with post_norm")
         return F_moc.cross_attention(
