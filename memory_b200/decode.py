@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import functional as F_moc
@@ -125,13 +126,16 @@ class ProjectedBankCache:
         scaled by the chapters' weights ([B, n] ids and weights: a router's joint list).  ``counts`` [B] int32: how many entries of
         each list count (what lies behind them is not read; none: zeros, lse -inf).  Returns [B, n_q, H*64] bf16, with
         ``return_lse`` also the natural log of the softmax's denominator [B, n_q, H] fp32.  A chapter id outside the cache raises the
-        device status and is left out.  For generation: no gradients.
+        device status and is left out.  For generation: it has no gradients; a query or a cache that requires
+        one is refused, and the chapters' weights are taken as numbers (a router's, whatever graph they hang on).
 
         Scores, softmax and sums are fp32 over either cache.  Over an 8-bit one, queries and probabilities go into the products as fp16
         numbers and what those leave of them: exact queries but for elements below 2^-31 of a head's largest, probabilities to 2^-21 of
         their own and 2^-32 of the largest among 32 neighbouring rows (times their scales)."""
         heads, kv_heads = int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads)
         L.require_cuda(q, chapter_indices, chapter_weights, counts)
+        if any(map(_carries_gradient, (q, self.kv_bank, self.kv_scale))):
+            raise RuntimeError("attention over the cache has no gradients: call it under torch.no_grad(), or on detached tensors")
         if q.dtype != torch.bfloat16 or q.dim() != 3:
             raise TypeError("attend takes bf16 queries [B, n_q, H * head_dim]")
         b, n_q, hd = q.shape
@@ -155,6 +159,13 @@ class ProjectedBankCache:
                                          _as(chapter_weights, torch.float32), None if counts is None else _as(counts, torch.int32),
                                          heads, kv_heads, self.tokens_per_chapter, 0.125 if scale is None else float(scale), return_lse)
         return (out, lse) if return_lse else out
+
+
+def _carries_gradient(t: Optional[torch.Tensor]) -> bool:
+    if t is None:
+        return False
+    return (t.requires_grad and torch.is_grad_enabled()) or (
+        forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
 
 
 def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
