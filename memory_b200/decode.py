@@ -21,7 +21,6 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib as L
-from . import functional as F_moc
 from . import ops
 
 
@@ -216,10 +215,10 @@ class MemoryDecoder:
     def __init__(self, cache: ProjectedBankCache, router_weight: torch.Tensor, router_bias: Optional[torch.Tensor],
                  wq: torch.Tensor, wo: torch.Tensor, *, num_heads: int, num_kv_heads: Optional[int] = None,
                  top_k: int, num_shared_chapters: int = 1, routed_scaling_factor: float = 2.5, router=None):
-        """``router``: a ``ChapterRouter`` that selects by other rules than the reference's (its scores, balance bias and groups); its
-        weights and ``top_k`` stand for ``router_weight``, ``router_bias`` and ``top_k`` then, which are not read."""
+        """``router``: a ``ChapterRouter``; its weights, ``top_k`` and rules (scores, balance bias, groups) stand for ``router_weight``,
+        ``router_bias`` and ``top_k`` then, which are not read.  One of the reference's rules is part of the native step."""
         self.cache = cache
-        self.router = router if router is not None and router.by_logits else None
+        self.router = router
         self.router_weight, self.router_bias = router_weight, router_bias
         self.num_heads = int(num_heads)
         self.num_kv_heads = int(num_kv_heads or num_heads)
@@ -234,12 +233,16 @@ class MemoryDecoder:
         """``hidden_states`` [B, n_q, d]: the tokens being decoded (input of the cross attention);
         ``routing_states`` [B, W, d]: the states the router mean-pools (a :class:`RoutingWindow` result).
         Returns (output [B, n_q, d] in the dtype of ``hidden_states``, routing info)."""
+        weight, bias, top_k = self.router_weight, self.router_bias, self.top_k
         if self.router is not None:
-            return self._step_by_router(hidden_states, routing_states)
+            if self.router.by_logits:
+                return self._step_by_router(hidden_states, routing_states)
+            linear = self.router.router
+            weight, bias, top_k = linear.weight.detach(), None if linear.bias is None else linear.bias.detach(), self.router.top_k
         out, idx, w, cidx, cw = ops.decode_step(
-            hidden_states, routing_states, self.router_weight, self.router_bias, self.wq_c, self.wo_c, self.cache.kv_bank,
+            hidden_states, routing_states, weight, bias, self.wq_c, self.wo_c, self.cache.kv_bank,
             num_heads=self.num_heads, num_kv_heads=self.num_kv_heads, tokens_per_chapter=self.cache.tokens_per_chapter,
-            top_k=self.top_k, num_shared=self.num_shared, routed_scale=self.routed_scale, scale=self.scale,
+            top_k=top_k, num_shared=self.num_shared, routed_scale=self.routed_scale, scale=self.scale,
             plans=self._plans, kv_scale=getattr(self.cache, "kv_scale", None), scale_rows=getattr(self.cache, "scale_rows", 0))
         return out, {"indices": idx, "weights": w, "combined_indices": cidx, "combined_weights": cw}
 
