@@ -141,7 +141,7 @@ __device__ __forceinline__ void load_row(const RowGroup& g, const T* p, int d, f
 // (V = 1) are not staged: they are read from their place when they are needed.
 template <typename T, int NV, int V> __host__ __device__ constexpr int row_bytes() { return V == 1 ? 0 : NV * V * static_cast<int>(sizeof(T)) * kResThreads; }
 __device__ __forceinline__ void cp_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 template <typename T, int NV, int V>
 __device__ __forceinline__ void stage_row(const RowGroup& g, const T* p, int d, char* slots) {
