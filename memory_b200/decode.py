@@ -153,9 +153,9 @@ class ProjectedBankCache:
         if b == 0 or n_q == 0 or chapter_indices.shape[1] == 0:
             out, lse = torch.zeros_like(q), q.new_full((b, n_q, heads), float("-inf"), dtype=torch.float32)
             return (out, lse) if return_lse else out
-        idx = _as(chapter_indices, torch.int32)
+        idx = _whole(chapter_indices)
         out, lse = ops.decode_attn_cache(ops._contig(q), self.kv_bank, self.kv_scale, self.scale_rows, idx,
-                                         _as(chapter_weights, torch.float32), None if counts is None else _as(counts, torch.int32),
+                                         _as(chapter_weights, torch.float32), None if counts is None else _whole(counts),
                                          heads, kv_heads, self.tokens_per_chapter, 0.125 if scale is None else float(scale), return_lse)
         return (out, lse) if return_lse else out
 
@@ -165,6 +165,11 @@ def _carries_gradient(t: Optional[torch.Tensor]) -> bool:
         return False
     return (t.requires_grad and torch.is_grad_enabled()) or (
         forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
+
+
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """Ids or counts as int32; what does not fit stays out of range instead of wrapping into it."""
+    return _as(t if t.dtype == torch.int32 else t.clamp(-(2 ** 31), 2 ** 31 - 1) if t.dtype == torch.int64 else t, torch.int32)
 
 
 def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
