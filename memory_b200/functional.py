@@ -1030,6 +1030,8 @@ def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
     c = logits.shape[-1]
     s = L.SelectShape.from_buffer_copy(_select_image(c, top_k, score, num_shared, routed_scale, num_groups, top_groups, group_score,
                                                      renormalize))
+    if logits.numel() // c >= 2 ** 31:
+        raise ValueError(f"at most 2^31 - 1 rows in one call, got {logits.numel() // c}")
     L.require_cuda(logits, balance_bias)
     if balance_bias is not None:
         _check_numel("balance_bias", balance_bias, c)
