@@ -1008,6 +1008,11 @@ def _select_image(chapters: int, top_k: int, score: str, num_shared: int, routed
                                int(bool(renormalize)), 0, 0, float(routed_scale)))
 
 
+def _nothing(*tensors) -> torch.Tensor:
+    """0 times the tensors' sums (fp32): what a call without rows adds to its empty results, so that their gradients are zeros."""
+    return sum(0.0 * t.float().sum() for t in tensors if t is not None)
+
+
 def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax", balance_bias: Optional[torch.Tensor] = None,
                     num_shared: int = 0, routed_scale: float = 1.0, num_groups: int = 1, top_groups: Optional[int] = None,
                     group_score: str = "max", renormalize: bool = True, count_filled: bool = True) -> ChapterSelection:
@@ -1044,9 +1049,9 @@ def select_chapters(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
         z = z.contiguous()
     s.rows, s.dtype, s.ld = z.shape[0], L.dtype_code(z.dtype), max(c, z.stride(0))
     if s.rows == 0:
-        joint = s.num_shared + s.top_k
-        flat = (z.new_empty(0, s.top_k, dtype=torch.int64), z.new_empty(0, s.top_k, dtype=torch.float32),
-                z.new_empty(0, joint, dtype=torch.int32), z.new_empty(0, joint, dtype=torch.float32),
+        joint, none = s.num_shared + s.top_k, _nothing(z)
+        flat = (z.new_empty(0, s.top_k, dtype=torch.int64), z.new_empty(0, s.top_k, dtype=torch.float32) + none,
+                z.new_empty(0, joint, dtype=torch.int32), z.new_empty(0, joint, dtype=torch.float32) + none,
                 torch.zeros(c, dtype=torch.int32, device=z.device))
     elif _differentiated(z):
         flat = _Select.apply(z, balance_bias, s, count_filled)
@@ -1201,8 +1206,9 @@ def gated_residual_norm(x: torch.Tensor, branch: torch.Tensor, weight: torch.Ten
     s = L.ResidualShape(rows, d, L.NORM_CODES[norm_type], L.dtype_code(x.dtype), L.dtype_code(branch.dtype), gate_seq,
                         residual_scale, eps, eps if next_eps is None else next_eps)
     if rows == 0:
-        y = x * residual_scale + 0.0 * branch.to(x.dtype)          # (nothing to compute; a graph that gives zero gradients)
-        return (y, 0.0 * branch) if next_weight is not None else y
+        # nothing to compute; a graph that gives every input zero gradients
+        y = x + _nothing(branch, gate, weight, bias).to(x.dtype)
+        return (y, branch + _nothing(x, gate, *params).to(branch.dtype)) if next_weight is not None else y
     if gate_seq and shape[0] > 65534:
         raise ValueError("at most 65,534 sequences with a gate of their own")
     if _differentiated(x, branch, gate, *params):
