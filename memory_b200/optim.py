@@ -13,8 +13,8 @@ from operator import attrgetter
 from typing import Iterable, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd.graph import increment_version
 
-from . import _lib as L
 from . import ops
 from .functional import SparseBankGrad
 
@@ -143,6 +143,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
         grads, outs, copies = _distinct_and_dense(grads, outs)
         ptrs = list(map(torch.Tensor.data_ptr, grads))
     result = ops.grad_clip(grads, ptrs, outs, banks, max_norm, eps, device)
+    increment_version(outs)          # (written behind autograd's back: a graph that saved one of them has to notice)
     if copies:
         with torch.no_grad():
             for o, dense in copies:
