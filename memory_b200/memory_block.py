@@ -73,6 +73,13 @@ class MemorySubBlock(nn.Module):
             self.post_norm = RMSNorm(hidden_dim, eps=norm_eps) if use_rms_norm else nn.LayerNorm(hidden_dim, eps=norm_eps)
         self.gate = nn.Parameter(torch.ones(hidden_dim)) if gate else None
 
+    def __setstate__(self, state):
+        """Modules that were saved whole before there was a norm behind the block have none."""
+        super().__setstate__(state)
+        for name, value, kept in (("residual_scale", 1.0, {}), ("post_norm", None, self._modules), ("gate", None, self._parameters)):
+            if name not in kept:
+                self.__dict__.setdefault(name, value)
+
     def forward(self, hidden_states: torch.Tensor, memory: torch.Tensor, *, gate: Optional[torch.Tensor] = None,
                 next_norm: Optional[nn.Module] = None):
         """``gate`` [B, d]: a gate for every sequence instead of the module's own; ``next_norm``: the norm in front of the block that

@@ -55,6 +55,14 @@ class ChapterRouter(nn.Module):
         self._last_shared = 0
         self.register_buffer("balance_bias", torch.zeros(num_chapters) if balance_bias else None)
 
+    def __setstate__(self, state):
+        """Modules that were saved whole before there were other rules than the reference's follow those."""
+        super().__setstate__(state)
+        rules = {"score": "softmax", "num_groups": 1, "top_groups": None, "group_score": "max", "renormalize": True}
+        for name, value in (("selection", rules), ("by_logits", False), ("last_load", None), ("_last_shared", 0)):
+            self.__dict__.setdefault(name, value)
+        self._buffers.setdefault("balance_bias", None)
+
     def _apply(self, fn, recurse=True):
         """Casts and moves of the module; the balance bias moves along and stays fp32 (steps of 0.001 vanish beside 0.3 in bf16)."""
         bias = self._buffers.get("balance_bias")
