@@ -11,8 +11,8 @@
 // y is formed again from x and f (it was rounded on its way out, and the sums over rows would carry that rounding): the same
 // bytes as reading y.
 //
-// Bound by HBM (f, x -> y, n; backward d_y, d_n, x, f -> d_x, d_f).  A row belongs to one warp (up to 768 columns; 2 to 8 warps
-// beyond), which holds it in registers between the passes, so every tensor is read once and a row's sums are shuffles.  The
+// Bound by HBM (f, x -> y, n; backward d_y, d_n, x, f -> d_x, d_f).  A row belongs to one warp (up to 384 columns forward, 768
+// backward, 512 of a LayerNorm; 2 to 8 warps beyond), which holds it in registers between the passes, so every tensor is read once and a row's sums are shuffles.  The
 // warps stay for many rows; while one is worked on, the next ones are on their way into shared memory (asynchronous copies,
 // each thread its own columns, so nobody waits for anybody else).  The backward pass runs one CTA an SM; its warps keep the
 // column sums of their rows in registers.
@@ -511,8 +511,13 @@ residual_sums_kernel(const ResSums s) {
 struct Plan {
   int v, each, group;              // columns of an access, of a thread; warps of a row
 };
-// Pieces of four columns wherever rows and base addresses allow 16-byte (fp32) accesses, single columns otherwise.  24 columns a
-// lane fill a row of 768 with one warp; the backward pass of a LayerNorm keeps four sums a column and takes 16.
+// Pieces of four columns wherever rows and base addresses allow 16-byte (fp32) accesses, single columns otherwise.  Backward, 24 columns
+// a lane fill a row of 768 with one warp; a LayerNorm keeps four sums a column and takes 16.  Forward, 12 make two warps a row.
+// Backward plans of 32 columns (rows above 4,096) spill: 156 bytes a thread for RMS, 900 for LayerNorm; single columns from 24 bytes (16
+// columns) to 1,880 (LayerNorm, 32).  Per element they cost up to twice (vector) and six times (single) what the others do.  fp32 stream, bf16
+// branch, next norm, gate [d], us forward / backward: 8,192 x 768 RMS 20 / 39, LayerNorm 31 / 57, with a gate per sequence 21 / 47 and 31 / 65;
+// 2,048 x 4,096 25 / 60 and 39 / 69; 1,024 x 8,192 29 / 70 and 47 / 104; single columns: 8,192 x 767 31 / 76 and 47 / 106, 1,024 x 8,191
+// LayerNorm 115 / 288.
 Plan plan_of(int d, bool wide, bool lean, bool fwd = false) {
   Plan p;
   p.v = wide ? 4 : 1;
@@ -521,16 +526,22 @@ Plan plan_of(int d, bool wide, bool lean, bool fwd = false) {
   while (p.group * 32 * p.each < d) p.group *= 2;
   return p;
 }
-template <int V, typename Go> int with_each(int each, Go go) {
+// go(columns a thread / V, V, whether LayerNorm) for what plan_of gives: MIDDLE is its number of columns between 257 and 768
+template <int V, int MIDDLE, bool LN, typename Go> int with_each(int each, Go go) {
   using std::integral_constant;
   using W = integral_constant<int, V>;
-  if (each == 8) return go(integral_constant<int, 8 / V>{}, W{});
-  if (each == 12) return go(integral_constant<int, 12 / V>{}, W{});
-  if (each == 16) return go(integral_constant<int, 16 / V>{}, W{});
-  if (each == 24) return go(integral_constant<int, 24 / V>{}, W{});
-  return go(integral_constant<int, 32 / V>{}, W{});
+  using N = integral_constant<bool, LN>;
+  if (each == 8) return go(integral_constant<int, 8 / V>{}, W{}, N{});
+  if constexpr (MIDDLE != 16)
+    if (each == MIDDLE) return go(integral_constant<int, MIDDLE / V>{}, W{}, N{});
+  if (each == 16) return go(integral_constant<int, 16 / V>{}, W{}, N{});
+  MOC_REQUIRE(each == 32, "no residual kernel for this number of columns a thread");
+  return go(integral_constant<int, 32 / V>{}, W{}, N{});
 }
-template <typename Go> int with_plan(const Plan& p, Go go) { return p.v == 4 ? with_each<4>(p.each, go) : with_each<1>(p.each, go); }
+template <int RMS, int LN, typename Go> int with_plan(const Plan& p, bool ln, Go go) {
+  if (ln) return p.v == 4 ? with_each<4, LN, true>(p.each, go) : with_each<1, LN, true>(p.each, go);
+  return p.v == 4 ? with_each<4, RMS, false>(p.each, go) : with_each<1, RMS, false>(p.each, go);
+}
 // Rows in flight a warp group: as many of `bytes` a CTA as fit, four at most
 int depth_of(const Plan& p, int bytes, int room) {
   if (p.v == 1) return 1;
@@ -607,9 +618,8 @@ extern "C" int moc_gated_residual_fwd(const moc_residual_shape* s, const void* x
   const long long most = (p.rows + groups - 1) / groups;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(most, static_cast<long long>(kResCtas) * ctas));
   return with_types(s, [&](auto xt, auto ft) {
-    return with_plan(plan, [&](auto nv, auto v) {
-      auto kern = p.ln ? residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, true>
-                       : residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, false>;
+    return with_plan<12, 12>(plan, p.ln, [&](auto nv, auto v, auto ln) {
+      auto kern = residual_fwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, decltype(ln)::value>;
       const size_t shared = plan.v == 1 ? 0 : static_cast<size_t>(depth) * bytes;
       MOC_CUDA_OK(allow_shared(kern, shared, 216 * 1024));
       kern<<<grid, kResThreads, shared, static_cast<cudaStream_t>(stream)>>>(p, depth);
@@ -654,9 +664,8 @@ extern "C" int moc_gated_residual_bwd(const moc_residual_shape* s, const void* x
   const int bytes = 2 * plan.each * kResThreads * ((s->x_dtype == MOC_F32 ? 4 : 2) + (s->f_dtype == MOC_F32 ? 4 : 2));
   const int depth = depth_of(plan, bytes, 216 * 1024);
   rc = with_types(s, [&](auto xt, auto ft) {
-    return with_plan(plan, [&](auto nv, auto v) {
-      auto kern = p.ln ? residual_bwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, true>
-                       : residual_bwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, false>;
+    return with_plan<24, 16>(plan, p.ln, [&](auto nv, auto v, auto ln) {
+      auto kern = residual_bwd_kernel<decltype(xt), decltype(ft), decltype(nv)::value, decltype(v)::value, decltype(ln)::value>;
       const int groups = kResThreads / (32 * p.group);
       const size_t shared = std::max(plan.v == 1 ? size_t{0} : static_cast<size_t>(depth) * bytes,
                                      groups > 1 ? static_cast<size_t>(groups) * p.d * sizeof(float) : size_t{0});
