@@ -1506,6 +1506,8 @@ template <typename LT, int S> int select_stream(const SelectParams& p, cudaStrea
 // Runs of `size` candidates of the groups that stay, at least.  Streaming takes its bound from their maxima and needs as many as
 // values that are to reach it: 2,000 rows, one of 8 groups of 512 kept (32 runs), sigmoid, bias: k = 28 37 us against 62 by a CTA a row,
 // k = 32 (a 33rd is needed) 225 against 62; two kept (64 runs): k = 48 45 against 67, k = 64 336 against 71.
+// Runs of 4 up to 2,048 chapters, of 16 beyond (3,000 rows, us, 4 / 16): 1,024 chapters k = 8 20 / 20, k = 64 51 / 63; 2,048 k = 8 plain
+// softmax 29 / 25, k = 32 31 / 29, k = 64 sigmoid with a bias 53 / 61; 4,096 k = 8 43 / 35, k = 32 44 / 39, k = 64 64 / 68.
 int kept_runs(const SelectParams& p, int size) { return p.keep * 32 * ceil_div(p.per / 32, size); }
 template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream) {
   const bool grouped = p.keep < p.groups;
@@ -1517,6 +1519,9 @@ template <typename LT> int select_fwd(const SelectParams& p, cudaStream_t stream
              kept_runs(p, p.N > 2048 ? 16 : 4) >= p.need) {
     return p.N > 2048 ? select_stream<LT, 16>(p, stream) : select_stream<LT, 4>(p, stream);
   } else {
+    // 1,024 threads where 256 with 16 logits each do not hold a row (us, 256 / 1,024 threads, k = 16: 1,024 chapters 1 row 8.3 / 12.4, 500 rows 19 / 45;
+    // 4,096 chapters 1 row 10.4 / 12.4, 148 rows 21 / 25, 500 rows 26 / 53).  The 48 registers of five CTAs an SM spill: 170 to 470 bytes a
+    // thread, most of it on the way through 64-bit keys.
     const bool big = p.N > 4096;
     auto kern = p.N <= 1024 ? select_cta_kernel<LT, 4, 256> : p.N <= 2048 ? select_cta_kernel<LT, 8, 256>
                 : !big ? select_cta_kernel<LT, 16, 256> : p.N <= 8192 ? select_cta_kernel<LT, 8, 1024> : select_cta_kernel<LT, 16, 1024>;
@@ -1533,7 +1538,9 @@ int select_load(const long long* idx, const float* weights, long long n, int C, 
   return MOC_OK;
 }
 template <typename LT> int select_bwd(const SelectGrads& p, cudaStream_t stream) {
-  // a warp a row up to 512 chapters, a CTA beyond
+  // A warp a row up to 512 chapters, a CTA beyond (us, warp / CTA): 512 chapters 8,192 rows sparse 8 / 26, dense 15 / 33, 500 rows dense 8.3 / 6.2;
+  // 1,024 chapters 8,192 rows sparse 10 / 25, dense 26 / 39, but 500 rows dense 12.4 / 6.2 and 1 row dense 12.3 / 4.2; 4,096 chapters 500 rows
+  // dense 35 / 9.
   if (p.C <= 512) select_bwd_kernel<LT, 32><<<ceil_div(p.rows, kWarpRows), 32 * kWarpRows, 0, stream>>>(p);
   else select_bwd_kernel<LT, 256><<<p.rows, 256, 0, stream>>>(p);
   MOC_CUDA_OK(cudaGetLastError());

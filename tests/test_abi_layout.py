@@ -33,6 +33,14 @@ def test_the_header_ends_the_descriptor_at_its_earlier_last_field():
     assert body.split()[-2:] == ["int32_t", "launches;"]
 
 
+def test_the_clipping_workspace_grows_with_every_table():
+    """A launch holds 64 tensors, or 680: one more asks for the partial sums of another launch."""
+    from memory_b200 import _lib as L
+    size = L.lib().moc_grad_clip_workspace_bytes
+    assert size(0) == size(63) > 0 and size(65) == size(679)
+    assert size(64 + 2 * 680) > size(64 + 680) > size(65) and size(680 * 3) > size(680 * 2) > size(680 * 1 - 1)
+
+
 def test_the_8_bit_step_refuses_without_a_gpu():
     from memory_b200 import _lib as L
     assert L.lib().moc_decode_step_cache(None, None, 0) == -1
