@@ -199,10 +199,11 @@ typedef struct {
 } moc_select_shape;
 int moc_select_fwd(const moc_select_shape* s, const void* logits, const float* balance_bias, int64_t* idx, float* weights,
                    int32_t* comb_idx, float* comb_w, float* row_stats, int32_t* load, void* stream);
-/* load [num_chapters] int32 = how often each chapter stands in idx (n ids of moc_select_fwd; others are not checked) with a weight
- * other than 0 (weights NULL: at all). */
+/* load [num_chapters] int32 = how often each chapter stands in idx (n ids; those outside 0..num_chapters - 1 are left out) with
+ * a weight other than 0 (weights NULL: at all). */
 int moc_select_load(const int64_t* idx, const float* weights, int64_t n, int32_t num_chapters, int32_t* load, void* stream);
-/* d_logits [rows, num_chapters] (dense, written whole) from the gradients of weights and comb_w (either may be NULL). */
+/* d_logits [rows, num_chapters] (dense, written whole) from the gradients of weights and comb_w (either may be NULL).  idx: what the
+ * forward pass wrote; ids outside the chapters to choose from have no gradient. */
 int moc_select_bwd(const moc_select_shape* s, const void* logits, const int64_t* idx, const float* weights, const float* comb_w,
                    const float* row_stats, const float* g_weights, const float* g_comb, void* d_logits, void* stream);
 /* bias[c] += rate * sign(mean load - load[c]) over the chapters behind the shared ones: balance without a loss term. */

@@ -1379,7 +1379,8 @@ select_bwd_kernel(const SelectGrads p) {
     ds[q] = sc[q] = 0.f;
     id[q] = 0;
     if (j >= p.k) continue;
-    id[q] = static_cast<int>(p.idx[row * p.k + j]);
+    const long long chosen = p.idx[row * p.k + j];
+    id[q] = chosen >= p.S && chosen < p.C ? static_cast<int>(chosen) : -1;          // (no chapter: no gradient)
     float g = p.g_weights != nullptr ? p.g_weights[row * p.k + j] : 0.f;
     if (p.g_comb != nullptr) {
       const float gc = p.g_comb[row * (p.S + p.k) + p.S + j];
@@ -1397,8 +1398,8 @@ select_bwd_kernel(const SelectGrads p) {
     const int j = lane + 32 * q;
     if (j >= p.k) continue;
     // (a place that was filled up has weight 0 and no score; a chosen score that underflowed to 0 has no gradient either)
-    const bool live = p.weights[row * p.k + j] != 0.f;
-    const float v = logit_of(z, id[q]);
+    const bool live = p.weights[row * p.k + j] != 0.f && id[q] >= 0;
+    const float v = logit_of(z, max(id[q], 0));
     sc[q] = !live ? 0.f : p.sigmoid ? 1.f / (1.f + expf(-v)) : expf(v - st.x) / st.y;
     ds[q] = !live ? 0.f : !p.renorm ? ds[q] : clamped ? ds[q] * 1e12f : (ds[q] - dot) / st.z;
     lean = fmaf(ds[q], sc[q], lean);
@@ -1438,8 +1439,9 @@ select_load_kernel(const long long* __restrict__ idx, const float* __restrict__ 
   __syncthreads();
 #pragma unroll 4
   for (long long i = rank * 1024 + threadIdx.x; i < n; i += kLoadCtas * 1024) {
-    if (weights != nullptr && weights[i] == 0.f) continue;
-    atomicAdd(counts + static_cast<int>(idx[i]), 1);
+    const unsigned long long c = static_cast<unsigned long long>(idx[i]);
+    if (c >= static_cast<unsigned long long>(C) || (weights != nullptr && weights[i] == 0.f)) continue;
+    atomicAdd(counts + static_cast<int>(c), 1);
   }
   cluster_sync();
   const uint32_t base = smem_u32(counts);

@@ -63,3 +63,26 @@ def test_the_count_refuses_without_a_gpu():
     from memory_b200 import _lib as L
     for idx, n, c, load in ((None, 4, 8, 4096), (4096, 4, 8, None), (4096, -1, 8, 4096), (4096, 4, 0, 4096), (4096, 4, 40000, 4096)):
         assert L.lib().moc_select_load(idx, None, n, c, load, None) == -1
+
+
+@pytest.mark.gpu
+def test_ids_from_elsewhere_stay_in_bounds():
+    """The C entries take ids as they come: those of no chapter are neither counted nor read."""
+    from memory_b200 import _lib as L, functional as F, ops
+    rows, c, k = 50, 40, 4
+    z = torch.randn(rows, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    s = L.SelectShape.from_buffer_copy(F._select_image(c, k, "sigmoid", 2, 1.0, 1, None, "max", True))
+    s.rows, s.dtype, s.ld = rows, 0, c
+    idx, w, _, cw, _, stats = ops.select_fwd(z, None, s, True)
+    g = torch.randn_like(w)
+    want = ops.select_bwd(z, s, idx, w, cw, stats, g, None)
+    bad = idx.clone()
+    bad[3, 0], bad[7, 1], bad[9, 2], bad[11, 3] = -1, c, 2 ** 40, 1          # (1 is a shared chapter)
+    got = ops.select_bwd(z, s, bad, w, cw, stats, g, None)
+    for r, j in ((3, 0), (7, 1), (9, 2), (11, 3)):
+        want[r, idx[r, j]] = 0
+    assert torch.equal(got, want)
+    load = torch.empty(c, dtype=torch.int32, device="cuda")
+    ops._issue("select_load", "f32", 1, z.device, (bad.data_ptr(), None, bad.numel(), c, load.data_ptr()))
+    good = bad[(bad >= 0) & (bad < c)]
+    assert torch.equal(load, torch.bincount(good, minlength=c).int())
