@@ -6,10 +6,10 @@
 //
 // A full batch should be bound by HBM (one byte an element) and is bound by latency and issuing; a few sequences by latency.  All
 // queries on a KV head (its heads, the tokens of the step) are the columns of one matrix instruction, so a row is fetched and converted
-// once for up to 16 of them; e4m3 -> fp16 is exact.  64 sequences of 4,160 rows, 12 heads: 70 us (3.8 TB/s of HBM, 6.3 from L2's side;
-// 340 instructions a unit of 32 rows at 0.51 a cycle and scheduler, 24 warps on an SM); 13 sequences of 3 tokens, 12 heads on 4, 47
-// chapters of 64 rows: 15 us; one sequence of 4,160 rows, 12 heads: 7.4 us.  Measured on the way, of these kernels' own stages: on CUDA
-// cores 95 us against 97 and 19 against 16; units by bulk tensor copies into a ring 99 against 92; e4m3 matrix instructions of single
+// once for up to 16 of them; e4m3 -> fp16 is exact.  64 sequences of 4,160 rows, 12 heads: 71 us (3.8 TB/s of HBM, 6.3 from L2's side;
+// 356 instructions a unit of 32 rows at 0.53 a cycle and scheduler, 24 warps on an SM); 13 sequences of 3 tokens, 12 heads on 4, 47
+// chapters of 64 rows: 17 us from launch to launch; one sequence of 4,160 rows, 12 heads: 10 us.  Measured on the way, of these kernels'
+// own stages, with one term of the probabilities: on CUDA cores 95 us against 97 and 19 against 16; units by bulk tensor copies into a ring 99 against 92; e4m3 matrix instructions of single
 // warps (16 of them take 175 instructions, fp16 ones 66: they convert too), queries and probabilities in three terms, 102 against 97 and
 // 33 against 16; the next unit's rows in registers too, with 16 warps on an SM, 79 against 70; 32 warps at 64 registers 90 against 70.
 //   - scores: A = 16 keys x 16 dims, B = dims x 8 queries.  The order of the dims is free, so a lane's 16 bytes of its row are
@@ -18,8 +18,8 @@
 //   - values: A = 16 dims x 16 rows, transposed from rows by byte permutations within a lane; B = the probabilities, which a matrix
 //     transposition brings from the scores' layout.  They go in as two fp16 terms (the second in the odd columns where those are idle,
 //     else by instructions of its own): 2^-21 of their own, not below 2^-32 of the largest.  With one term results that cancel lose
-//     their last bits and one in ten elements rounds to the neighbouring bf16 number; it costs 73.7 us against 71.8 (64 sequences),
-//     28.7 against 26.6 (six queries a KV head).  Row scales that differ within a unit go in relative to the unit's largest.
+//     their last bits and one in ten elements rounds to the neighbouring bf16 number; it costs 70.7 us against 70.3 (64 sequences,
+//     12 heads of their own), 25.1 against 23.7 (six queries a KV head), 16.8 against 16.5 (nine queries, scales of 16 rows).  Row scales that differ within a unit go in relative to the unit's largest.
 // The softmax's reference of a column is a score already met; it moves to the largest only when a score passes it by 2^8, which saves
 // most units the reduction across lanes and the rescaling (92 us with, 97 without, before the steps on addresses).  References, sums
 // and accumulators are fp32.  A cluster of CTAs takes the units of one (sequence, KV head) in turns, warp by warp; parts merge through

@@ -1427,8 +1427,8 @@ select_bwd_kernel(const SelectGrads p) {
     }
 }
 
-// load[c] = how many of the `n` picks are c (with `weights`: of those whose weight is not 0), by one cluster of kLoadCtas CTAs: each counts its share in shared memory, then adds up
-// a share of the chapters over all of them.  (Counted by the selecting CTAs with atomics in global memory, 65,536 picks among 64
+// load[c] = how many of the `n` picks are c (with `weights`: of those whose weight is not 0), by one cluster of kLoadCtas CTAs: each
+// counts its share in shared memory, then adds up a share of the chapters over all of them.  (Counted by the selecting CTAs with atomics in global memory, 65,536 picks among 64
 // chapters took 30 us: the counters share two cache lines.)
 constexpr int kLoadCtas = 8;
 __global__ void __launch_bounds__(1024)

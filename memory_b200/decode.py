@@ -128,9 +128,9 @@ class ProjectedBankCache:
         device status and is left out.  For generation: it has no gradients; a query or a cache that requires
         one is refused, and the chapters' weights are taken as numbers (a router's, whatever graph they hang on).
 
-        Scores, softmax and sums are fp32 over either cache.  Over an 8-bit one, queries and probabilities go into the products as fp16
-        numbers and what those leave of them: exact queries but for elements below 2^-31 of a head's largest, probabilities to 2^-21 of
-        their own and 2^-32 of the largest among 32 neighbouring rows (times their scales)."""
+        Scores, softmax and sums are fp32 over either cache.  Over an 8-bit one, queries go into the products as
+        fp16 numbers (exact but for elements below 2^-24 of their head's largest, which are off by 2^-32 of it at most) and probabilities as two
+        (off by 2^-21 of their own, not below 2^-32 of the largest among 32 neighbouring rows, times those rows' scales)."""
         heads, kv_heads = int(num_heads), int(num_heads if num_kv_heads is None else num_kv_heads)
         L.require_cuda(q, chapter_indices, chapter_weights, counts)
         if any(map(_carries_gradient, (q, self.kv_bank, self.kv_scale))):
